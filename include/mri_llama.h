@@ -124,6 +124,132 @@ mri_status mri_llama_generate_greedy(mri_llama *model, const uint32_t *prompt, s
  * sampling/mod.rs:144-151; idx: device [rows]. */
 mri_status mri_argmax(const float *v, size_t rows, size_t n, uint32_t *idx, void *stream);
 
+/* ===================================================================== */
+/* A KV cache in 4-bit blocks for several sequences, and the operators of  */
+/* a decode loop over it.  Extensions with no counterpart in the           */
+/* reference, whose cache is f32 and holds one sequence                    */
+/* (src/cache/kv_cache.rs), whose decoding is greedy                       */
+/* (src/sampling/mod.rs:144-151) and which evicts nothing.                 */
+/* ===================================================================== */
+
+/* Keys and values of n_layers layers and n_seqs sequences of up to max_seq
+ * positions, in blocks of 32 consecutive dims of a head: an f16 scale d and
+ * quants q in [-8, 7], 18 bytes.  With mx, mn the block's extremes and
+ * a = mx if mx >= -mn else mn: d = f16(a / -8), saturated at +-65504,
+ * q = clamp(rint(x / d), -8, 7) (exact quotients, ties to even; 0 where d is
+ * 0); a block with a value that is not finite reads back as NaN.  A new cache
+ * reads as zeros.  The handle is bound to the device it is created on; calls
+ * with another current device are InvalidArgument.  It owns the workspace of
+ * its attention calls (fixed at creation, so captured graphs hold it as long
+ * as the handle lives): calls on one handle must be ordered, as on
+ * mri_kv_cache; handles are independent.  No call allocates memory.
+ * InvalidShape for a zero size; Unsupported for a head dim other than 64 or
+ * 128, or max_seq above 2^30. */
+typedef struct mri_kv4_cache mri_kv4_cache;
+mri_status mri_kv4_cache_create(size_t n_layers, size_t n_seqs, size_t max_seq,
+                                size_t n_kv_heads, size_t head_dim, mri_kv4_cache **out);
+/* Device bytes of the cached blocks and the workspace. */
+size_t mri_kv4_cache_device_bytes(const mri_kv4_cache *cache);
+void mri_kv4_cache_destroy(mri_kv4_cache *cache);
+
+/* The rows of a call: `rows` per sequence for sequences first_seq ..
+ * first_seq + n_seqs - 1.  Row i of the call's sequence b is at position
+ * (pos ? pos[b] : start) + i.  pos and count are nullable DEVICE arrays
+ * [n_seqs]; with count only the first min(count[b], rows) rows of a sequence
+ * are real.  The other rows, and rows at positions >= max_seq, are neither
+ * read nor written in any tensor.  (start + rows > max_seq without pos is
+ * InvalidShape.) */
+typedef struct mri_kv4_rows {
+    size_t first_seq;
+    size_t n_seqs;
+    size_t rows;
+    size_t start;
+    const uint32_t *pos;
+    const uint32_t *count;
+} mri_kv4_rows;
+
+/* Quantizes the rows' keys and values into the cache: k and v are
+ * [n_seqs * rows] rows of n_kv_heads * head_dim f32, `stride` floats apart.
+ * What the cache held at those positions is replaced. */
+mri_status mri_kv4_append(mri_kv4_cache *cache, size_t layer, const mri_kv4_rows *rows,
+                          const float *k, const float *v, size_t stride, void *stream);
+/* The cached values at the rows' positions, as f32, of layers layer ..
+ * layer + n_layers - 1: k and v are [n_layers][n_seqs * rows] rows, `stride`
+ * floats apart. */
+mri_status mri_kv4_read(const mri_kv4_cache *cache, size_t layer, size_t n_layers,
+                        const mri_kv4_rows *rows, float *k, float *v, size_t stride,
+                        void *stream);
+/* Causal grouped-query attention over the cache: query row i of a sequence at
+ * position p = pos + i sees keys 0 .. p (append first).  q and out are
+ * [n_seqs * rows] rows of n_heads * head_dim f32, q_stride / out_stride
+ * floats apart; head h reads KV head h / (n_heads / n_kv_heads).
+ * InvalidShape when n_heads % n_kv_heads != 0.
+ * weights (nullable): [cache n_seqs][n_kv_heads][max_seq] f32 of this layer,
+ * the attention weight that each cached key has got: key t of a KV head gets
+ * the sum of its probabilities over the call's rows and the head's query
+ * heads, added to what was there for t < pos and stored for the new keys
+ * t >= pos (so a rejected draft's weight is gone with it).  The sums are in a
+ * fixed order: equal calls give equal bits.
+ * Outputs agree with f32 arithmetic on the cached values to f32 rounding. */
+mri_status mri_kv4_attend(mri_kv4_cache *cache, size_t layer, const mri_kv4_rows *rows,
+                          const float *q, size_t q_stride, size_t n_heads, float *out,
+                          size_t out_stride, float *weights, void *stream);
+/* Eviction by accumulated weight, in every layer, sequence and KV head of
+ * `src` by itself, into `dst` (a cache of the same sizes but its max_seq,
+ * which holds at least `keep`; src itself: in place).  Sequence b holds
+ * n = min(lens[b], src max_seq) keys.  If n <= keep all are kept; else the
+ * last `recent` of them and, of the others, the keep - recent with the largest
+ * weight (equal weights: the earlier key; NaN: below every number), in
+ * the order they had.  dst holds them at positions 0 .., weights_out their
+ * weights, kept their positions in src, lens_out[b] = min(n, keep).
+ * Device arrays: weights [n_layers][n_seqs][n_kv_heads][src max_seq],
+ * weights_out the same with dst's max_seq (in place: weights itself),
+ * lens and lens_out [n_seqs] (may be the same array), kept [n_layers][n_seqs]
+ * [n_kv_heads][keep], filled up with MRI_NO_TOKEN.  What dst and weights_out
+ * hold past a sequence's keys stays.  The keys keep the rotation of their
+ * original positions.  InvalidArgument for recent > keep, or weights_out ==
+ * weights other than in place; InvalidShape for keep = 0 or caches that differ
+ * or are too small. */
+mri_status mri_kv4_evict(const mri_kv4_cache *src, mri_kv4_cache *dst, const float *weights,
+                         float *weights_out, const uint32_t *lens, uint32_t *lens_out,
+                         size_t keep, size_t recent, uint32_t *kept, void *stream);
+
+/* mri_llama_forward_cached on sequence `seq` of a 4-bit cache: n tokens whose
+ * rotary positions are start_pos .. and whose cache positions are cache_pos ..
+ * (the same until keys are evicted).  Each row attends to the cached keys
+ * before it, its own included.  weights (nullable): [n_layers][cache n_seqs]
+ * [n_kv_heads][max_seq], added to as by mri_kv4_attend.  logits: device
+ * [n, vocab].  Checks as mri_llama_forward_cached, for both position ranges. */
+mri_status mri_llama_forward_kv4(mri_llama *model, const uint32_t *tokens, size_t n,
+                                 size_t start_pos, mri_kv4_cache *cache, size_t seq,
+                                 size_t cache_pos, float *weights, float *logits, void *stream);
+
+/* Probabilities of rows of n logits (device, x_stride / out_stride floats
+ * apart; out may be x): out = exp((x - max x) / temperature) / sum.  A row of
+ * -inf only becomes zeros.  InvalidArgument unless temperature > 0 and finite;
+ * InvalidShape for n = 0 or a stride below n. */
+mri_status mri_softmax(const float *x, size_t rows, size_t n, size_t x_stride, float temperature,
+                       float *out, size_t out_stride, void *stream);
+
+/* Speculative verification: k drafted tokens a sequence against the target
+ * model's probabilities.  Device arrays: drafts [n_seqs, k], target_probs
+ * [n_seqs, k + 1, n], draft_probs [n_seqs, k, n] (nullable: the drafts were
+ * not sampled, probability 1 each), uniforms [n_seqs, k + 1] in [0, 1),
+ * n_drafts [n_seqs] (nullable: k; above k counts as k).
+ * Draft i is accepted while uniforms[i] * q_i(draft) < p_i(draft) (exact).
+ * With a of them accepted, one token more is drawn with uniforms[k]: from
+ * max(p_a - q_a, 0) where a draft was rejected (from p_a where that has no
+ * mass), from p_a where none was: the first token whose cumulative sum in f64 exceeds
+ * uniforms[k] times the total.  accepted[b] = a; tokens [n_seqs, k + 1] = the
+ * accepted drafts, the drawn token, then MRI_NO_TOKEN.  A draft id >= n is
+ * rejected; where no token has a positive probability the drawn token is
+ * MRI_NO_TOKEN.  NaN probabilities count as 0.  InvalidShape for n = 0. */
+#define MRI_NO_TOKEN 0xffffffffu
+mri_status mri_verify_drafts(const uint32_t *drafts, const float *draft_probs,
+                             const float *target_probs, const float *uniforms,
+                             const uint32_t *n_drafts, size_t n_seqs, size_t k, size_t n,
+                             uint32_t *tokens, uint32_t *accepted, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

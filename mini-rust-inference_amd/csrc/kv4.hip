@@ -1,0 +1,1041 @@
+// kv4.hip — the KV cache in 4-bit blocks: append, read, attention, eviction.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "kv4.hpp"
+
+namespace mri {
+namespace {
+
+constexpr int kWave = 64;
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+
+template <int HD>
+struct Page {
+    static constexpr int NB = HD / 32;
+    static constexpr size_t kBytes = 72 * HD;
+    static constexpr int kV = 32 * HD, kKs = 64 * HD, kVs = 68 * HD;
+    // byte of the K dword with dims 32 b + 8 g .. of key `key`
+    static __device__ int k_dword(int key, int g, int b) {
+        return (key >> 4) * 8 * HD + (g * 16 + (key & 15)) * 4 * NB + 4 * b;
+    }
+    // byte of the V dword with the eight keys of (g, half h) of dim `dim`
+    static __device__ int v_dword(int dim, int g, int h) {
+        const int e = dim >> 4;
+        return kV + (e >> 1) * 1024 + (g * 16 + (dim & 15)) * 16 + (e & 1) * 8 + 4 * h;
+    }
+    // byte of a scale inside the K or V scales
+    static __device__ int scale(int key, int b) {
+        return ((key >> 2) * NB + b) * 8 + 2 * (key & 3);
+    }
+    // where a key's quant sits in a dim's V dwords: (g, h) and element j
+    static __device__ void v_place(int key, int *g, int *h, int *j) {
+        *h = key >> 5;
+        *g = (key >> 2) & 3;
+        *j = (key & 3) + ((key >> 4) & 1) * 4;
+    }
+    // the key that (g, h, j) stands for
+    static __device__ int v_key(int g, int h, int j) {
+        return 32 * h + (j >> 2) * 16 + 4 * g + (j & 3);
+    }
+};
+
+__host__ __device__ inline int nibble_of(int j) { return (j >> 1) + 4 * (j & 1); }
+
+// The real rows of the call's sequence b: positions [*p0, *p0 + count).
+__device__ inline unsigned rows_of(const Kv4Rows &a, int b, unsigned *p0) {
+    const unsigned p = a.pos ? a.pos[b] : a.start;
+    if (p >= a.max_seq || a.row0 >= a.max_seq - p) return *p0 = 0;
+    *p0 = p + a.row0;
+    unsigned n = a.rows;
+    if (a.count) n = min(n, a.count[b] - min(a.row0, a.count[b]));
+    return min(n, a.max_seq - *p0);
+}
+// Row i of sequence b among the call's rows.
+__device__ inline size_t row_index(const Kv4Rows &a, int b, size_t i) {
+    return (size_t)b * a.ld_rows + a.row0 + i;
+}
+
+// ---- append ------------------------------------------------------------------------
+// One workgroup a page of the rows' positions and KV head.  Eight lanes hold a
+// block of 32 values; its extremes are reduced over them.  The quotient x / d
+// is rounded exactly: n = rint(x * (1 / d)) is off by one at most, the rest
+// x - n d is exact in f32 (n d has 15 bits and is near x), and comparing it
+// with d / 2 settles n.  The quants go through LDS, key by key, and leave as
+// the page's dwords; where keys of a V dword are not the call's, their nibbles
+// are kept (a dword has one writer).
+__device__ inline int quant_of(float x, float d, float inv) {
+    float n = rintf(x * inv);
+    n = fminf(fmaxf(n, -9.0f), 9.0f);
+    const float r = fmaf(-n, d, x), h = 0.5f * fabsf(d);
+    const float up = (r < 0.0f) == (d < 0.0f) ? 1.0f : -1.0f;  // where the rest points
+    if (fabsf(r) > h || (fabsf(r) == h && ((int)n & 1))) n = n + up;
+    return (int)fminf(fmaxf(n, -8.0f), 7.0f) + 8;
+}
+
+template <int HD, bool V4>
+__global__ __launch_bounds__(256) void k_kv4_append(Kv4Rows a, const float *__restrict__ k,
+                                                    const float *__restrict__ v, size_t stride,
+                                                    int n_pg) {
+    using P = Page<HD>;
+    constexpr int NB = P::NB, LD = HD + 4, R4 = HD / 4;
+    __shared__ __attribute__((aligned(16))) uint8_t s_q[2][kPageKeys][LD];
+    __shared__ uint16_t s_d[2][kPageKeys][NB];
+    const int t = threadIdx.x;
+    unsigned x = blockIdx.x;
+    const int pg = x % n_pg;
+    x /= n_pg;
+    const int head = x % a.n_kv, b = x / a.n_kv;
+    unsigned p0;
+    const unsigned cnt = rows_of(a, b, &p0);
+    const unsigned page = p0 / kPageKeys + pg, key0 = page * kPageKeys;
+    if (cnt == 0 || key0 >= p0 + cnt) return;
+    const int lo = (int)(max(p0, key0) - key0);
+    const int hi = (int)(min(p0 + cnt, key0 + kPageKeys) - key0);
+    const int items = (hi - lo) * R4;
+    for (int it = t; it < 2 * items; it += 256) {
+        const int which = it >= items, rest = which ? it - items : it;
+        const int key = lo + rest / R4, e = rest % R4;
+        const size_t row = row_index(a, b, key0 + key - p0);
+        const float *src = (which ? v : k) + row * stride + head * HD + 4 * e;
+        float f[4];
+        if constexpr (V4) {
+            const float4 w = *reinterpret_cast<const float4 *>(src);
+            f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = src[i];
+        }
+        float mx = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+        float mn = fminf(fminf(f[0], f[1]), fminf(f[2], f[3]));
+        int bad = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= !(fabsf(f[i]) < INFINITY);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            mx = fmaxf(mx, __shfl_xor(mx, o, kWave));
+            mn = fminf(mn, __shfl_xor(mn, o, kWave));
+            bad |= __shfl_xor(bad, o, kWave);
+        }
+        const float am = mx >= -mn ? mx : mn;
+        const _Float16 d16 = (_Float16)fminf(fmaxf(am * -0.125f, -65504.0f), 65504.0f);
+        const float d = (float)d16;
+        const float inv = 1.0f / d;
+        unsigned w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = bad || d == 0.0f ? 8 : quant_of(f[i], d, inv);
+            w |= (unsigned)q << (8 * i);
+        }
+        *reinterpret_cast<unsigned *>(&s_q[which][key][4 * e]) = w;
+        if ((e & 7) == 0)
+            s_d[which][key][e >> 3] = bad ? 0x7e00 : __builtin_bit_cast(unsigned short, d16);
+    }
+    __syncthreads();
+    uint8_t *pb = a.pages + (((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages + page) *
+                                P::kBytes;
+    for (int w = t; w < 8 * HD; w += 256) {  // K dwords
+        const int tile = w / (64 * NB), l = (w / NB) & 63, blk = w % NB;
+        const int key = 16 * tile + (l & 15), g = l >> 4;
+        if (key < lo || key >= hi) continue;
+        const uint2 q = *reinterpret_cast<const uint2 *>(&s_q[0][key][32 * blk + 8 * g]);
+        // bytes of even elements are nibbles 0..3, of odd ones nibbles 4..7
+        const unsigned e0 = q.x & 0x000f000f, o0 = (q.x >> 8) & 0x000f000f;
+        const unsigned e1 = q.y & 0x000f000f, o1 = (q.y >> 8) & 0x000f000f;
+        const unsigned ev = (e0 & 0xf) | (e0 >> 12) | (e1 & 0xf) << 8 | (e1 >> 4 & 0xf000);
+        const unsigned od = (o0 & 0xf) | (o0 >> 12) | (o1 & 0xf) << 8 | (o1 >> 4 & 0xf000);
+        *reinterpret_cast<unsigned *>(pb + 4 * w) = ev | od << 16;
+    }
+    for (int w = t; w < 8 * HD; w += 256) {  // V dwords
+        const int c = w >> 8, l = (w >> 2) & 63, e = 2 * c + ((w >> 1) & 1), h = w & 1;
+        const int dim = 16 * e + (l & 15), g = l >> 4;
+        unsigned val = 0, mask = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int key = P::v_key(g, h, j), sh = 4 * nibble_of(j);
+            if (key >= lo && key < hi) {
+                val |= (unsigned)s_q[1][key][dim] << sh;
+                mask |= 0xfu << sh;
+            }
+        }
+        unsigned *dst = reinterpret_cast<unsigned *>(pb + P::kV + 4 * w);
+        if (mask == 0xffffffffu) *dst = val;
+        else if (mask) *dst = (*dst & ~mask) | val;
+    }
+    for (int w = t; w < 2 * 64 * NB; w += 256) {  // scales
+        const int which = w >= 64 * NB, rest = which ? w - 64 * NB : w;
+        const int key = rest / NB, blk = rest % NB;
+        if (key < lo || key >= hi) continue;
+        *reinterpret_cast<uint16_t *>(pb + (which ? P::kVs : P::kKs) + P::scale(key, blk)) =
+            s_d[which][key][blk];
+    }
+}
+
+// ---- read ---------------------------------------------------------------------------
+// Four consecutive dims of one row's key and value a thread.
+template <int HD, bool V4>
+__global__ __launch_bounds__(256) void k_kv4_read(Kv4Rows a, size_t layer_bytes,
+                                                  float *__restrict__ k, float *__restrict__ v,
+                                                  size_t stride, int n_pg) {
+    using P = Page<HD>;
+    constexpr int R4 = HD / 4;
+    unsigned x = blockIdx.x;
+    const int pg = x % n_pg;
+    x /= n_pg;
+    const int head = x % a.n_kv;
+    x /= a.n_kv;
+    const int b = x % a.n_seqs, layer = x / a.n_seqs;
+    unsigned p0;
+    const unsigned cnt = rows_of(a, b, &p0);
+    const unsigned page = p0 / kPageKeys + pg, key0 = page * kPageKeys;
+    if (cnt == 0 || key0 >= p0 + cnt) return;
+    const int lo = (int)(max(p0, key0) - key0);
+    const int hi = (int)(min(p0 + cnt, key0 + kPageKeys) - key0);
+    const uint8_t *pb = a.pages + layer * layer_bytes +
+                        (((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages + page) *
+                            P::kBytes;
+    for (int it = threadIdx.x; it < (hi - lo) * R4; it += 256) {
+        const int key = lo + it / R4, e = it % R4, blk = e >> 3;
+        const size_t row =
+            (size_t)layer * a.n_seqs * a.ld_rows + row_index(a, b, key0 + key - p0);
+        const float dk = (float)*reinterpret_cast<const _Float16 *>(pb + P::kKs + P::scale(key, blk));
+        const float dv = (float)*reinterpret_cast<const _Float16 *>(pb + P::kVs + P::scale(key, blk));
+        const unsigned kw =
+            *reinterpret_cast<const unsigned *>(pb + P::k_dword(key, (e >> 1) & 3, blk));
+        int g, h, j;
+        P::v_place(key, &g, &h, &j);
+        float fk[4], fv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            fk[i] = (float)((int)(kw >> (4 * nibble_of(4 * (e & 1) + i)) & 0xf) - 8) * dk;
+            const unsigned vw =
+                *reinterpret_cast<const unsigned *>(pb + P::v_dword(4 * e + i, g, h));
+            fv[i] = (float)((int)(vw >> (4 * nibble_of(j)) & 0xf) - 8) * dv;
+        }
+        float *ko = k + row * stride + head * HD + 4 * e, *vo = v + row * stride + head * HD + 4 * e;
+        if constexpr (V4) {
+            *reinterpret_cast<float4 *>(ko) = float4{fk[0], fk[1], fk[2], fk[3]};
+            *reinterpret_cast<float4 *>(vo) = float4{fv[0], fv[1], fv[2], fv[3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ko[i] = fk[i], vo[i] = fv[i];
+        }
+    }
+}
+
+// ---- attention ----------------------------------------------------------------------
+// Sixteen queries (rows x query heads of one KV head, flattened row-major) are
+// the columns of S^T = K Q^T and O^T = V^T P^T, both on f16 matrix instructions
+// with f32 accuracy: the quants are small whole numbers, exact in f16; q is
+// split into two f16 halves (22 bits) after a power-of-two scaling of its row,
+// and so is p * d_v, the probability times the value block's scale, under a
+// power of two that follows the largest d_v seen (what is below 2^-39 of that
+// largest product is lost).  The key blocks' scales
+// multiply the 32-dim partial products in f32.
+__device__ inline half8_t unpack8(unsigned w) {
+    // 0x6400 | n is the f16 1024 + n, 0x6400 | 16 n is 1024 + 16 n
+    const unsigned w8 = w >> 8;
+    const half2_t lo = {(_Float16)1032.0f, (_Float16)1032.0f};
+    const half2_t m16 = {(_Float16)0.0625f, (_Float16)0.0625f};
+    const half2_t c72 = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const half2_t a0 = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | 0x64006400u) - lo;
+    const half2_t a1 = __builtin_elementwise_fma(
+        __builtin_bit_cast(half2_t, (w & 0x00f000f0u) | 0x64006400u), m16, c72);
+    const half2_t a2 = __builtin_bit_cast(half2_t, (w8 & 0x000f000fu) | 0x64006400u) - lo;
+    const half2_t a3 = __builtin_elementwise_fma(
+        __builtin_bit_cast(half2_t, (w8 & 0x00f000f0u) | 0x64006400u), m16, c72);
+    return half8_t{a0.x, a0.y, a1.x, a1.y, a2.x, a2.y, a3.x, a3.y};
+}
+
+// x in two f16: hi + lo, off by 2^-22 of x at most where lo is not subnormal.
+__device__ inline void split8(const float *x, half8_t *hi, half8_t *lo) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const _Float16 h = (_Float16)x[j];
+        (*hi)[j] = h;
+        (*lo)[j] = (_Float16)(x[j] - (float)h);
+    }
+}
+
+// The query operand of a 16-column tile: column r of lane (g, r).
+template <int HD>
+struct QTile {
+    static constexpr int NB = HD / 32;
+    half8_t hi[NB], lo[NB];
+    float inv;  // what the raw products are multiplied by (log2 units)
+    // src null: an empty column
+    __device__ void load(const float *src, int g) {
+        float x[NB][8];
+        float mx = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[b][j] = src ? src[32 * b + 8 * g + j] : 0.0f;
+                mx = fmaxf(mx, fabsf(x[b][j]));
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+        // the row's largest magnitude to [2^10, 2^11)
+        const int e = mx > 0.0f && mx < INFINITY ? min(10 - ilogbf(mx), 120) : 0;
+        const float up = ldexpf(1.0f, e);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[b][j] = x[b][j] * up;
+            split8(x[b], &hi[b], &lo[b]);
+        }
+        // log2(e) / sqrt(HD), rounded once
+        constexpr float c = HD == 64 ? 0.18033688011112042592f : 0.12751743021347021697f;
+        inv = ldexpf(c, -e);
+    }
+};
+
+// Scores (log2 units) of the 16 keys of tile t of a page: keys 4 g + i of
+// column r in lane (g, r).
+template <int HD>
+__device__ inline float4_t score_tile(const uint8_t *pb, int t, int lane, const QTile<HD> &q) {
+    using P = Page<HD>;
+    constexpr int NB = P::NB;
+    unsigned w[NB];
+    const uint8_t *kp = pb + t * 8 * HD + lane * 4 * NB;
+    const uint8_t *sp = pb + P::kKs + (t * 4 + (lane >> 4)) * NB * 8;
+    uint2 d[NB];
+    if constexpr (NB == 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(kp);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2 *>(kp);
+        w[0] = v.x, w[1] = v.y;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b += 2) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(sp + 8 * b);
+        d[b] = uint2{v.x, v.y};
+        d[b + 1] = uint2{v.z, v.w};
+    }
+    float4_t s = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const half8_t kq = unpack8(w[b]);
+        float4_t c = {0, 0, 0, 0};
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q.lo[b], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q.hi[b], c, 0, 0, 0);
+        const half2_t d01 = __builtin_bit_cast(half2_t, d[b].x),
+                      d23 = __builtin_bit_cast(half2_t, d[b].y);
+        s[0] = fmaf(c[0], (float)d01.x, s[0]);
+        s[1] = fmaf(c[1], (float)d01.y, s[1]);
+        s[2] = fmaf(c[2], (float)d23.x, s[2]);
+        s[3] = fmaf(c[3], (float)d23.y, s[3]);
+    }
+    return s * q.inv;
+}
+
+// The running softmax of a wave's 16 columns.
+template <int HD>
+struct Softmax {
+    float m = -INFINITY, l = 0.0f;  // per column; l of this lane's keys only
+    int ve = -100;                  // 2^ve <= the largest d_v seen; o is in units of 2^(ve - 14)
+    float4_t o[HD / 16];
+    __device__ Softmax() {
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) o[e] = float4_t{0, 0, 0, 0};
+    }
+};
+
+// Adds one page: keys [0, lim) of it are seen by this lane's column (lim <= 0:
+// none), the first n_keys by any; `whole`: all 64 by every column.
+template <int HD>
+__device__ inline void attend_page(const uint8_t *pb, int lane, const QTile<HD> &q, int lim,
+                                   int n_keys, bool whole, Softmax<HD> &st) {
+    using P = Page<HD>;
+    constexpr int NB = P::NB;
+    const int g = lane >> 4;
+    // the page's V scales: their largest sets the power of two
+    float dmax = 0.0f;
+    {
+        const unsigned *sp = reinterpret_cast<const unsigned *>(pb + P::kVs);
+#pragma unroll
+        for (int u = 0; u < NB / 2; ++u) {
+            const int w = u * 64 + lane;
+            half2_t d = __builtin_bit_cast(half2_t, sp[w]);
+            if (!whole) {  // what lies past the end counts for nothing
+                const int key = w / (2 * NB) * 4 + 2 * (w & 1);
+                if (key >= n_keys) d.x = (_Float16)0.0f;
+                if (key + 1 >= n_keys) d.y = (_Float16)0.0f;
+            }
+            dmax = fmaxf(dmax, fmaxf(fabsf((float)d.x), fabsf((float)d.y)));
+        }
+#pragma unroll
+        for (int x = 1; x < kWave; x <<= 1) dmax = fmaxf(dmax, __shfl_xor(dmax, x, kWave));
+    }
+    float s[16];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const float4_t v = score_tile<HD>(pb, t, lane, q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * t + i] = v[i];
+    }
+    if (!whole) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (16 * t + 4 * g + i >= lim) s[4 * t + i] = -INFINITY;
+    }
+    float pm = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[i]);
+    pm = fmaxf(pm, __shfl_xor(pm, 16, kWave));
+    pm = fmaxf(pm, __shfl_xor(pm, 32, kWave));
+    // f16 exponent of the largest scale, 2^ve <= d < 2^(ve + 1)
+    int ve = dmax > 0.0f && dmax < INFINITY ? ilogbf(dmax) : -24;
+    ve = max(ve, st.ve);
+    const float m_new = fmaxf(st.m, pm);
+    if (__any(m_new > st.m || ve > st.ve)) {
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(st.m - m_use);
+        st.l = st.l * alpha;
+        const float f = ldexpf(alpha, st.ve - ve);
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) st.o[e] = st.o[e] * f;
+        st.m = m_new;
+        st.ve = ve;
+    }
+    const float m_use = st.m == -INFINITY ? 0.0f : st.m;
+    const float up = ldexpf(1.0f, 14 - st.ve);  // p * d_v to below 2^15
+    float p[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
+        st.l = st.l + p[i];
+        p[i] = p[i] * up;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        half8_t ph[NB], pl[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float x[8];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint2 d = *reinterpret_cast<const uint2 *>(
+                    pb + P::kVs + (((2 * h + u) * 4 + g) * NB + b) * 8);
+                const half2_t d01 = __builtin_bit_cast(half2_t, d.x),
+                              d23 = __builtin_bit_cast(half2_t, d.y);
+                const float dv[4] = {(float)d01.x, (float)d01.y, (float)d23.x, (float)d23.y};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = 4 * (2 * h + u) + i;
+                    x[4 * u + i] = p[n] * dv[i];
+                    // a key past the end may hold anything, NaN too
+                    if (!whole && 16 * (2 * h + u) + 4 * g + i >= lim) x[4 * u + i] = 0.0f;
+                }
+            }
+            split8(x, &ph[b], &pl[b]);
+        }
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) {
+            const unsigned w = *reinterpret_cast<const unsigned *>(
+                pb + P::kV + (e >> 1) * 1024 + lane * 16 + (e & 1) * 8 + 4 * h);
+            const half8_t vq = unpack8(w);
+            st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, pl[e >> 1], st.o[e], 0, 0, 0);
+            st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, ph[e >> 1], st.o[e], 0, 0, 0);
+        }
+    }
+}
+
+// How the pages of a call's sequences are dealt to `slots` runs of at most
+// `chunk` pages: sequence b takes ceil(pages_b / chunk) runs.  chunk is the
+// least for which the runs suffice (every wave computes the same).
+constexpr int kMinChunk = 4;
+__device__ inline unsigned seq_pages(const Kv4Rows &a, int b) {
+    unsigned p0;
+    const unsigned cnt = rows_of(a, b, &p0);
+    return cnt ? (p0 + cnt + kPageKeys - 1) / kPageKeys : 0;
+}
+__device__ inline unsigned wave_sum_u(unsigned v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+__device__ inline unsigned run_chunk(const Kv4Rows &a, unsigned slots) {
+    const int lane = threadIdx.x & 63;
+    unsigned total = 0;
+    for (int b = lane; b < a.n_seqs; b += kWave) total += seq_pages(a, b);
+    total = wave_sum_u(total);
+    unsigned chunk = max((total + slots - 1) / slots, (unsigned)kMinChunk);
+    for (;;) {
+        unsigned runs = 0;
+        for (int b = lane; b < a.n_seqs; b += kWave) runs += (seq_pages(a, b) + chunk - 1) / chunk;
+        runs = wave_sum_u(runs);
+        if (runs <= slots) return chunk;
+        chunk += max(chunk / 16, 1u);
+    }
+}
+
+// (the runs of one sequence never need more than max_seq / 64 pages, and with
+// slots >= n_seqs the loop above ends)
+
+// The first run and the number of runs of sequence b.
+__device__ inline void runs_of(const Kv4Rows &a, unsigned chunk, int b, unsigned *first,
+                               unsigned *n) {
+    const int lane = threadIdx.x & 63;
+    unsigned before = 0;
+    for (int i = lane; i < b; i += kWave) before += (seq_pages(a, i) + chunk - 1) / chunk;
+    *first = wave_sum_u(before);
+    *n = (seq_pages(a, b) + chunk - 1) / chunk;
+}
+
+constexpr int kFewWaves = 4;
+
+// Grid: slots x (KV heads x query tiles).  SPLIT: a slot is a run of pages of
+// one sequence, whose partial results go to `part`; else it is a sequence.
+// The four waves take every fourth page and meet in LDS.
+template <int HD, bool SPLIT>
+__global__ __launch_bounds__(kFewWaves *kWave) void k_kv4_attend(
+    Kv4Rows a, const float *__restrict__ q, size_t qs, int groups, int n_qt, unsigned slots,
+    float *__restrict__ out, size_t os, float *__restrict__ part, float *__restrict__ lse) {
+    using P = Page<HD>;
+    __shared__ float s_m[kFewWaves][16], s_l[kFewWaves][16];
+    __shared__ __attribute__((aligned(16))) float s_o[kFewWaves][16][HD + 4];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    const int qt = blockIdx.x % n_qt, head = blockIdx.x / n_qt % a.n_kv;
+    const unsigned slot = blockIdx.x / (n_qt * a.n_kv);
+    int b = (int)slot;
+    unsigned pg0 = 0, pg1 = 0;
+    if constexpr (SPLIT) {
+        const unsigned chunk = run_chunk(a, slots);
+        // the sequence of this run
+        unsigned first = 0;
+        for (b = 0; b < a.n_seqs; ++b) {
+            const unsigned np = seq_pages(a, b), n = (np + chunk - 1) / chunk;
+            if (slot < first + n) {
+                pg0 = (slot - first) * chunk;
+                pg1 = min(pg0 + chunk, np);
+                break;
+            }
+            first += n;
+        }
+        if (b == a.n_seqs) return;
+    }
+    unsigned p0;
+    const int cnt = (int)rows_of(a, b, &p0);
+    const int n_q = cnt * groups;       // real queries of the KV head
+    if (qt * 16 >= n_q) return;
+    const int last_row = (min(qt * 16 + 16, n_q) - 1) / groups;
+    const unsigned end = p0 + last_row + 1;  // keys that the tile's last row sees
+    if constexpr (!SPLIT) pg1 = (end + kPageKeys - 1) / kPageKeys;
+    pg1 = min(pg1, (end + kPageKeys - 1) / kPageKeys);
+    const int qi = qt * 16 + r, row = qi / groups;
+    const bool real = qi < n_q;
+    const size_t qrow = row_index(a, b, row);
+    const int qh = head * groups + qi % groups;
+    QTile<HD> qtile;
+    qtile.load(real ? q + qrow * qs + qh * HD : nullptr, g);
+    const long see = real ? (long)p0 + row + 1 : 0;          // keys this column sees
+    const unsigned all = p0 + (qt * 16) / groups + 1;        // keys every real column sees
+    Softmax<HD> st;
+    const uint8_t *base =
+        a.pages + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages * P::kBytes;
+    for (unsigned pg = pg0 + wv; pg < pg1; pg += kFewWaves) {
+        const bool whole = (pg + 1) * kPageKeys <= all;
+        const long lim = see - (long)pg * kPageKeys;
+        attend_page<HD>(base + (size_t)pg * P::kBytes, lane, qtile, (int)min(lim, 64l),
+                        (int)min(end - pg * kPageKeys, 64u), whole, st);
+    }
+    // the column's sum over its four lane groups, then the waves
+    st.l = st.l + __shfl_xor(st.l, 16, kWave);
+    st.l = st.l + __shfl_xor(st.l, 32, kWave);
+    if (g == 0) {
+        s_m[wv][r] = st.m;
+        s_l[wv][r] = st.l;
+    }
+    const float down = ldexpf(1.0f, st.ve - 14);
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e)
+        *reinterpret_cast<float4_t *>(&s_o[wv][r][16 * e + 4 * g]) = st.o[e] * down;
+    __syncthreads();
+    for (int it = threadIdx.x; it < 16 * HD; it += kFewWaves * kWave) {
+        const int c = it / HD, d = it % HD;
+        const int ci = qt * 16 + c;
+        if (ci >= n_q) break;
+        float m = s_m[0][c];
+#pragma unroll
+        for (int w = 1; w < kFewWaves; ++w) m = fmaxf(m, s_m[w][c]);
+        const float m_use = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(s_m[w][c] - m_use);
+            l = l + s_l[w][c] * f;
+            o = o + s_o[w][c][d] * f;
+        }
+        if constexpr (SPLIT) {
+            float *pc = part + ((size_t)blockIdx.x * 16 + c) * (HD + 2);
+            pc[2 + d] = o;
+            if (d == 0) {
+                pc[0] = m;
+                pc[1] = l;
+            }
+        } else {
+            const size_t orow = row_index(a, b, ci / groups);
+            const int oh = head * groups + ci % groups;
+            out[orow * os + oh * HD + d] = o / l;
+            if (lse && d == 0) lse[((size_t)b * a.rows + ci / groups) * (a.n_kv * groups) + oh] = m_use + __log2f(l);
+        }
+    }
+}
+
+// Joins the runs of one (sequence, KV head, query tile, column).
+template <int HD>
+__global__ __launch_bounds__(HD) void k_kv4_join(Kv4Rows a, int groups, int n_qt, unsigned slots,
+                                                 const float *__restrict__ part,
+                                                 float *__restrict__ out, size_t os,
+                                                 float *__restrict__ lse) {
+    const int d = threadIdx.x;
+    const int c = blockIdx.x % 16;
+    const int qt = blockIdx.x / 16 % n_qt, head = blockIdx.x / (16 * n_qt) % a.n_kv;
+    const int b = blockIdx.x / (16 * n_qt * a.n_kv);
+    unsigned p0;
+    const int cnt = (int)rows_of(a, b, &p0);
+    const int ci = qt * 16 + c;
+    if (ci >= cnt * groups) return;
+    const unsigned chunk = run_chunk(a, slots);
+    unsigned first, n;
+    runs_of(a, chunk, b, &first, &n);
+    // runs past the tile's last row wrote nothing useful but m = -inf, l = 0
+    auto at = [&](unsigned i) {
+        return part + ((((size_t)(first + i) * a.n_kv + head) * n_qt + qt) * 16 + c) * (HD + 2);
+    };
+    float m = -INFINITY;
+    for (unsigned i = 0; i < n; ++i) m = fmaxf(m, at(i)[0]);
+    const float m_use = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o = 0.0f;
+    for (unsigned i = 0; i < n; ++i) {
+        const float *pc = at(i);
+        const float f = __builtin_amdgcn_exp2f(pc[0] - m_use);
+        l = l + pc[1] * f;
+        o = o + pc[2 + d] * f;
+    }
+    const size_t orow = row_index(a, b, ci / groups);
+    const int oh = head * groups + ci % groups;
+    out[orow * os + oh * HD + d] = o / l;
+    if (lse && d == 0) lse[((size_t)b * a.rows + ci / groups) * (a.n_kv * groups) + oh] = m_use + __log2f(l);
+}
+
+// The keys' attention weights: one wave a page of a KV head goes over all the
+// queries that see it, with the scores of the attention itself and the
+// rows' log-sum-exps, so each key has one writer and one order of sums.
+template <int HD>
+__global__ __launch_bounds__(kWave) void k_kv4_weights(Kv4Rows a, const float *__restrict__ q,
+                                                       size_t qs, int groups, int n_pages,
+                                                       const float *__restrict__ lse,
+                                                       float *__restrict__ weights) {
+    using P = Page<HD>;
+    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    unsigned x = blockIdx.x;
+    const unsigned pg = x % n_pages;
+    x /= n_pages;
+    const int head = x % a.n_kv, b = x / a.n_kv;
+    unsigned p0;
+    const int cnt = (int)rows_of(a, b, &p0);
+    const unsigned key0 = pg * kPageKeys;
+    if (cnt == 0 || key0 >= p0 + cnt) return;
+    const int n_q = cnt * groups;
+    const uint8_t *pb = a.pages + (((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages + pg) *
+                                      P::kBytes;
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = 0.0f;
+    const int row0 = key0 > p0 ? (int)(key0 - p0) : 0;  // the first row that sees the page
+    for (int qt = row0 * groups / 16; qt * 16 < n_q; ++qt) {
+        const int qi = qt * 16 + r, row = qi / groups;
+        const bool real = qi < n_q;
+        const size_t qrow = row_index(a, b, row);
+        const int qh = head * groups + qi % groups;
+        QTile<HD> qtile;
+        qtile.load(real ? q + qrow * qs + qh * HD : nullptr, g);
+        const float z = real ? lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] : 0.0f;
+        const long lim = real ? (long)p0 + row + 1 - (long)key0 : 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const float4_t s = score_tile<HD>(pb, t, lane, qtile);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (16 * t + 4 * g + i < lim)
+                    w[4 * t + i] = w[4 * t + i] + __builtin_amdgcn_exp2f(s[i] - z);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) w[i] = w[i] + __shfl_xor(w[i], o, kWave);
+    if (r == 0) {
+        float *wr = weights + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.max_seq;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const unsigned key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
+            if (key < p0 + cnt) wr[key] = (key < p0 ? wr[key] : 0.0f) + w[i];
+        }
+    }
+}
+
+// ---- eviction ------------------------------------------------------------------------
+// Weights as unsigned keys in their order; NaN below all, -0 as 0.
+__device__ inline unsigned weight_key(float w) {
+    if (w != w) return 0u;
+    const unsigned b = __float_as_uint(w == 0.0f ? 0.0f : w);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+// The kept positions of one (layer, sequence, KV head) a workgroup: the k-th
+// largest weight by four passes over its bytes (counts in LDS), then the
+// positions above it and the first of those equal to it, in order: each wave
+// counts and writes a contiguous sixteenth.
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / kWave;
+__global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
+    __shared__ unsigned s_hist[256];
+    __shared__ unsigned s_digit, s_left;
+    __shared__ unsigned s_gt[kSelWaves], s_eq[kSelWaves];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    const size_t rowi = blockIdx.x;
+    const int b = (int)(rowi / e.n_kv % e.n_seqs);
+    const unsigned n = min(e.lens[b], e.src_max);
+    uint32_t *kept = e.kept + rowi * e.keep;
+    if (n <= e.keep) {
+        for (unsigned i = t; i < e.keep; i += kSelThreads) kept[i] = i < n ? i : MRI_NO_TOKEN;
+        return;
+    }
+    const float *w = e.w + rowi * e.src_max;
+    const unsigned old = n - e.recent, take = e.keep - e.recent;
+    for (unsigned i = t; i < e.recent; i += kSelThreads) kept[take + i] = old + i;
+    if (take == 0) return;
+    unsigned prefix = 0, left = take;  // the digits so far; how many to take below them
+    for (int pass = 0; pass < 4; ++pass) {
+        const int sh = 24 - 8 * pass;
+        if (t < 256) s_hist[t] = 0;
+        __syncthreads();
+        for (unsigned i = t; i < old; i += kSelThreads) {
+            const unsigned key = weight_key(w[i]);
+            if (pass == 0 || (key >> (sh + 8)) == prefix) atomicAdd(&s_hist[key >> sh & 255], 1u);
+        }
+        __syncthreads();
+        if (wv == 0) {
+            // lane l holds digits 255 - 4 l .. 252 - 4 l, from the largest down
+            unsigned c[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += c[i] = s_hist[255 - 4 * lane - i];
+            unsigned inc = sum;
+#pragma unroll
+            for (int o = 1; o < kWave; o <<= 1) {
+                const unsigned y = __shfl_up(inc, o, kWave);
+                if (lane >= o) inc += y;
+            }
+            unsigned above = inc - sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (above < left && left <= above + c[i]) {
+                    s_digit = 255 - 4 * lane - i;
+                    s_left = left - above;
+                }
+                above += c[i];
+            }
+        }
+        __syncthreads();
+        prefix = prefix << 8 | s_digit;
+        left = s_left;
+        __syncthreads();
+    }
+    // keys > prefix are taken, and the first `left` of those equal to it
+    const unsigned seg = ((old + kSelWaves - 1) / kSelWaves + kWave - 1) / kWave * kWave;
+    const unsigned i0 = min(wv * seg, old), i1 = min(i0 + seg, old);
+    unsigned gt = 0, eq = 0;
+    for (unsigned i = i0; i < i1; i += kWave) {
+        const unsigned key = i + lane < i1 ? weight_key(w[i + lane]) : 0;
+        gt += __popcll(__ballot(i + lane < i1 && key > prefix));
+        eq += __popcll(__ballot(i + lane < i1 && key == prefix));
+    }
+    if (lane == 0) {
+        s_gt[wv] = gt;
+        s_eq[wv] = eq;
+    }
+    __syncthreads();
+    gt = eq = 0;
+    for (int u = 0; u < wv; ++u) {
+        gt += s_gt[u];
+        eq += s_eq[u];
+    }
+    const unsigned long long below = (1ull << lane) - 1;
+    for (unsigned i = i0; i < i1; i += kWave) {
+        const bool in = i + lane < i1;
+        const unsigned key = in ? weight_key(w[i + lane]) : 0;
+        const unsigned long long bg = __ballot(in && key > prefix),
+                                 be = __ballot(in && key == prefix);
+        const unsigned g_at = gt + __popcll(bg & below), e_at = eq + __popcll(be & below);
+        const unsigned at = g_at + min(e_at, left);
+        if (in && (key > prefix || (key == prefix && e_at < left))) kept[at] = i + lane;
+        gt += __popcll(bg);
+        eq += __popcll(be);
+    }
+}
+
+// Moves the kept keys of one (layer, sequence, KV head) to their new places,
+// page by page.  In place one workgroup walks the pages in order: a page's
+// sources lie at it or behind it, so only a page's own loads have to end
+// before its stores begin.  Into another cache every page has a workgroup.
+template <int HD>
+__global__ __launch_bounds__(256) void k_kv4_move(Kv4Evict e, int per_row) {
+    using P = Page<HD>;
+    constexpr int NB = P::NB, KD = 8 * HD / 256, SD = (128 * NB + 255) / 256;
+    __shared__ unsigned s_i[kPageKeys];
+    const int t = threadIdx.x;
+    const size_t rowi = blockIdx.x / per_row;
+    const int b = (int)(rowi / e.n_kv % e.n_seqs);
+    if (rowi < (size_t)e.n_seqs * e.n_kv && rowi % e.n_kv == 0 && blockIdx.x % per_row == 0 &&
+        t == 0)
+        e.lens_out[b] = min(min(e.lens[b], e.src_max), e.keep);
+    const bool in_place = e.src == e.dst;
+    const uint8_t *src = e.src + rowi * e.src_pages * P::kBytes;
+    uint8_t *dst = e.dst + rowi * e.dst_pages * P::kBytes;
+    const float *w = e.w + rowi * e.src_max;
+    float *wo = e.w_out + rowi * e.dst_max;
+    const uint32_t *kept = e.kept + rowi * e.keep;
+    const unsigned n_pg = (e.keep + kPageKeys - 1) / kPageKeys;
+    for (unsigned pg = blockIdx.x % per_row; pg < n_pg; pg += per_row) {
+        const unsigned key0 = pg * kPageKeys;
+        __syncthreads();  // the previous page's indexes are read, its stores issued
+        if (t < kPageKeys) s_i[t] = key0 + t < e.keep ? kept[key0 + t] : MRI_NO_TOKEN;
+        __syncthreads();
+        if (s_i[0] == MRI_NO_TOKEN) return;  // (the kept ones come first)
+        if (in_place && (s_i[kPageKeys - 1] == key0 + kPageKeys - 1)) continue;  // all in place
+        unsigned kq[KD], vq[KD], vm[KD], sc[SD];
+        float wt = 0.0f;
+#pragma unroll
+        for (int u = 0; u < KD; ++u) {
+            const int x = t + 256 * u;
+            const int tile = x / (64 * NB), l = (x / NB) & 63, blk = x % NB;
+            const unsigned i = s_i[16 * tile + (l & 15)];
+            kq[u] = 0;
+            if (i != MRI_NO_TOKEN)
+                kq[u] = *reinterpret_cast<const unsigned *>(
+                    src + (size_t)(i / kPageKeys) * P::kBytes +
+                    P::k_dword(i % kPageKeys, l >> 4, blk));
+        }
+#pragma unroll
+        for (int u = 0; u < KD; ++u) {
+            const int x = t + 256 * u;
+            const int l = (x >> 2) & 63, dim = 16 * (2 * (x >> 8) + ((x >> 1) & 1)) + (l & 15);
+            vq[u] = vm[u] = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const unsigned i = s_i[P::v_key(l >> 4, x & 1, j)];
+                if (i == MRI_NO_TOKEN) continue;
+                int sg, sh, sj;
+                P::v_place(i % kPageKeys, &sg, &sh, &sj);
+                const unsigned d = *reinterpret_cast<const unsigned *>(
+                    src + (size_t)(i / kPageKeys) * P::kBytes + P::v_dword(dim, sg, sh));
+                vq[u] |= (d >> (4 * nibble_of(sj)) & 0xfu) << (4 * nibble_of(j));
+                vm[u] |= 0xfu << (4 * nibble_of(j));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < SD; ++u) {
+            const int x = t + 256 * u, which = x >= 64 * NB, rest = x % (64 * NB);
+            sc[u] = 0;
+            const unsigned i = s_i[rest / NB];
+            if (x < 128 * NB && i != MRI_NO_TOKEN)
+                sc[u] = *reinterpret_cast<const uint16_t *>(
+                    src + (size_t)(i / kPageKeys) * P::kBytes + (which ? P::kVs : P::kKs) +
+                    P::scale(i % kPageKeys, rest % NB));
+        }
+        if (t < kPageKeys && s_i[t] != MRI_NO_TOKEN) wt = w[s_i[t]];
+        uint8_t *pb = dst + (size_t)pg * P::kBytes;
+        unsigned old[KD];
+#pragma unroll
+        for (int u = 0; u < KD; ++u) {
+            old[u] = 0;
+            if (vm[u] != 0xffffffffu && vm[u])
+                old[u] = *reinterpret_cast<const unsigned *>(pb + P::kV + 4 * (t + 256 * u));
+        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's loads have ended
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < KD; ++u) {
+            const int x = t + 256 * u;
+            if (s_i[16 * (x / (64 * NB)) + ((x / NB) & 15)] != MRI_NO_TOKEN)
+                *reinterpret_cast<unsigned *>(pb + 4 * x) = kq[u];
+            if (vm[u])
+                *reinterpret_cast<unsigned *>(pb + P::kV + 4 * x) = (old[u] & ~vm[u]) | vq[u];
+        }
+#pragma unroll
+        for (int u = 0; u < SD; ++u) {
+            const int x = t + 256 * u, which = x >= 64 * NB, rest = x % (64 * NB);
+            if (x < 128 * NB && s_i[rest / NB] != MRI_NO_TOKEN)
+                *reinterpret_cast<uint16_t *>(pb + (which ? P::kVs : P::kKs) +
+                                              P::scale(rest / NB, rest % NB)) = (uint16_t)sc[u];
+        }
+        if (t < kPageKeys && s_i[t] != MRI_NO_TOKEN) wo[key0 + t] = wt;
+    }
+}
+
+inline bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// Workgroups of one launch: 2^32 threads at most.
+mri_status grid_ok(size_t blocks) {
+    return blocks < (1u << 22) ? MRI_OK
+                               : set_error(MRI_ERR_UNSUPPORTED, "kv4: more than 2^22 workgroups");
+}
+
+template <class F>
+void by_head(size_t hd, F &&f) {
+    if (hd == 64) f(std::integral_constant<int, 64>{});
+    else f(std::integral_constant<int, 128>{});
+}
+
+// Pages that `rows` consecutive positions can touch.
+inline size_t pages_touched(const Kv4Rows &a) {
+    if (!a.pos) return (a.start + a.rows - 1) / kPageKeys - a.start / kPageKeys + 1;
+    return ((size_t)a.rows + kPageKeys - 2) / kPageKeys + 1;
+}
+
+}  // namespace
+
+mri_status launch_kv4_append(const Kv4Rows &a, size_t hd, const float *k, const float *v,
+                             size_t stride, hipStream_t s) {
+    if (!a.rows || !a.n_seqs) return MRI_OK;
+    const size_t n_pg = pages_touched(a), blocks = n_pg * a.n_kv * a.n_seqs;
+    if (const mri_status st = grid_ok(blocks)) return st;
+    const bool v4 = stride % 4 == 0 && al16(k) && al16(v);
+    by_head(hd, [&](auto h) {
+        constexpr int HD = decltype(h)::value;
+        if (v4)
+            hipLaunchKernelGGL((k_kv4_append<HD, true>), dim3((unsigned)blocks), dim3(256), 0, s,
+                               a, k, v, stride, (int)n_pg);
+        else
+            hipLaunchKernelGGL((k_kv4_append<HD, false>), dim3((unsigned)blocks), dim3(256), 0, s,
+                               a, k, v, stride, (int)n_pg);
+    });
+    MRI_LAUNCHED("k_kv4_append");
+    return MRI_OK;
+}
+
+mri_status launch_kv4_read(const Kv4Rows &a, size_t hd, size_t n_layers, size_t layer_bytes,
+                           float *k, float *v, size_t stride, hipStream_t s) {
+    if (!a.rows || !a.n_seqs || !n_layers) return MRI_OK;
+    const size_t n_pg = pages_touched(a), blocks = n_pg * a.n_kv * a.n_seqs * n_layers;
+    if (const mri_status st = grid_ok(blocks)) return st;
+    const bool v4 = stride % 4 == 0 && al16(k) && al16(v);
+    by_head(hd, [&](auto h) {
+        constexpr int HD = decltype(h)::value;
+        if (v4)
+            hipLaunchKernelGGL((k_kv4_read<HD, true>), dim3((unsigned)blocks), dim3(256), 0, s, a,
+                               layer_bytes, k, v, stride, (int)n_pg);
+        else
+            hipLaunchKernelGGL((k_kv4_read<HD, false>), dim3((unsigned)blocks), dim3(256), 0, s,
+                               a, layer_bytes, k, v, stride, (int)n_pg);
+    });
+    MRI_LAUNCHED("k_kv4_read");
+    return MRI_OK;
+}
+
+namespace {
+
+// One chunk of rows: at most kKv4LseFloats (row, head) pairs when weights are
+// asked for.
+template <int HD>
+mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_heads, float *out,
+                       size_t os, float *weights, float *part, float *lse, hipStream_t s) {
+    const int groups = (int)(n_heads / a.n_kv);
+    const size_t n_qt = ((size_t)a.rows * groups + 15) / 16;
+    const size_t tiles = n_qt * a.n_kv;
+    float *z = weights ? lse : nullptr;
+    // two workgroups of four waves fit a CU: a call with fewer tiles than that
+    // many splits its keys
+    const size_t fill = std::min<size_t>(2 * (size_t)std::max(device_cus(), 1), kKv4PartTiles);
+    if (tiles * a.n_seqs * 2 <= fill) {
+        const size_t slots = fill / tiles;
+        const size_t blocks = slots * tiles;
+        if (const mri_status st = grid_ok(blocks)) return st;
+        hipLaunchKernelGGL((k_kv4_attend<HD, true>), dim3((unsigned)blocks),
+                           dim3(kFewWaves * kWave), 0, s, a, q, qs, groups, (int)n_qt,
+                           (unsigned)slots, out, os, part, z);
+        MRI_LAUNCHED("k_kv4_attend");
+        hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)(a.n_seqs * tiles * 16)), dim3(HD), 0,
+                           s, a, groups, (int)n_qt, (unsigned)slots, part, out, os, z);
+        MRI_LAUNCHED("k_kv4_join");
+    } else {
+        const size_t blocks = tiles * a.n_seqs;
+        if (const mri_status st = grid_ok(blocks)) return st;
+        hipLaunchKernelGGL((k_kv4_attend<HD, false>), dim3((unsigned)blocks),
+                           dim3(kFewWaves * kWave), 0, s, a, q, qs, groups, (int)n_qt, 0u, out, os,
+                           part, z);
+        MRI_LAUNCHED("k_kv4_attend");
+    }
+    if (weights) {
+        const size_t n_pg = a.pos ? a.n_pages : (a.start + (size_t)a.row0 + a.rows - 1) / kPageKeys + 1;
+        const size_t blocks = n_pg * a.n_kv * a.n_seqs;
+        if (const mri_status st = grid_ok(blocks)) return st;
+        hipLaunchKernelGGL((k_kv4_weights<HD>), dim3((unsigned)blocks), dim3(kWave), 0, s, a, q,
+                           qs, groups, (int)n_pg, lse, weights);
+        MRI_LAUNCHED("k_kv4_weights");
+    }
+    return MRI_OK;
+}
+
+}  // namespace
+
+mri_status launch_kv4_attend(const Kv4Rows &a, size_t hd, const float *q, size_t q_stride,
+                             size_t n_heads, float *out, size_t out_stride, float *weights,
+                             float *part, float *lse, hipStream_t s) {
+    if (!a.rows || !a.n_seqs || !n_heads) return MRI_OK;
+    mri_status st = MRI_OK;
+    auto go = [&](const Kv4Rows &c, const float *cq, float *co) {
+        by_head(hd, [&](auto h) {
+            constexpr int HD = decltype(h)::value;
+            st = attend_rows<HD>(c, cq, q_stride, n_heads, co, out_stride, weights, part, lse, s);
+        });
+    };
+    if (!weights || (size_t)a.n_seqs * a.rows * n_heads <= kKv4LseFloats) {
+        go(a, q, out);
+        return st;
+    }
+    // weights: as many sequences, or rows of one, as their log-sum-exps fit
+    const size_t seqs = std::max<size_t>(1, kKv4LseFloats / (a.rows * n_heads));
+    const size_t rows = std::min<size_t>(a.rows, std::max<size_t>(1, kKv4LseFloats / n_heads));
+    for (size_t b = 0; b < (size_t)a.n_seqs && !st; b += seqs)
+        for (size_t i = 0; i < a.rows && !st; i += rows) {
+            Kv4Rows c = a;
+            c.first_seq += (int)b;
+            c.n_seqs = (int)std::min<size_t>(seqs, a.n_seqs - b);
+            if (c.pos) c.pos += b;
+            if (c.count) c.count += b;
+            c.row0 = (unsigned)i;
+            c.rows = (unsigned)std::min<size_t>(rows, a.rows - i);
+            go(c, q + b * a.ld_rows * q_stride, out + b * a.ld_rows * out_stride);
+        }
+    return st;
+}
+
+mri_status launch_kv4_evict(const Kv4Evict &e, size_t hd, hipStream_t s) {
+    const size_t rows = (size_t)e.n_layers * e.n_seqs * e.n_kv;
+    if (const mri_status st = grid_ok(rows * 4)) return st;
+    hipLaunchKernelGGL(k_kv4_select, dim3((unsigned)rows), dim3(kSelThreads), 0, s, e);
+    MRI_LAUNCHED("k_kv4_select");
+    const size_t per_row = e.src == e.dst ? 1 : (e.keep + kPageKeys - 1) / kPageKeys;
+    if (const mri_status st = grid_ok(rows * per_row)) return st;
+    by_head(hd, [&](auto h) {
+        constexpr int HD = decltype(h)::value;
+        hipLaunchKernelGGL((k_kv4_move<HD>), dim3((unsigned)(rows * per_row)), dim3(256), 0, s, e,
+                           (int)per_row);
+    });
+    MRI_LAUNCHED("k_kv4_move");
+    return MRI_OK;
+}
+
+}  // namespace mri

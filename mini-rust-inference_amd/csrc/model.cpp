@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "common.hpp"
+#include "kv4_cache.hpp"
 #include "mri_llama.h"
 
 struct mri_kv_cache {
@@ -320,6 +321,32 @@ bool row_path(mri_llama *m) {
     return ok;
 }
 
+// Where a forward pass keeps its keys and values: an f32 cache, or sequence
+// `seq` of a 4-bit one from position `pos` on (weights: mri_llama_forward_kv4's).
+struct KvTarget {
+    mri_kv_cache *f32 = nullptr;
+    mri_kv4_cache *c4 = nullptr;
+    size_t seq = 0, pos = 0;
+    float *weights = nullptr;
+    KvTarget(mri_kv_cache *c) : f32(c) {}
+    KvTarget(mri_kv4_cache *c, size_t seq, size_t pos, float *w)
+        : c4(c), seq(seq), pos(pos), weights(w) {}
+};
+
+// A 4-bit cache's part of a block: the rows' rotated keys and values (row
+// stride kvd) into the cache, then the attention over it.
+mri_status attend_kv4(mri_llama *m, size_t li, size_t rows, const KvTarget &kv, const float *k,
+                      const float *v, const float *q, size_t qs, hipStream_t s) {
+    mri_kv4_cache *c = kv.c4;
+    const mri_kv4_rows r{kv.seq, 1, rows, kv.pos, nullptr, nullptr};
+    Kv4Rows a;
+    TRY(kv4_rows(c, li, &r, &a));
+    TRY(launch_kv4_append(a, c->hd, k, v, m->kvd, s));
+    float *w = kv.weights ? kv.weights + li * c->n_seqs * c->n_kv * c->max_seq : nullptr;
+    return launch_kv4_attend(a, c->hd, q, qs, m->cfg.n_heads, m->attn, m->qd, w, c->part, c->lse,
+                             s);
+}
+
 // TransformerBlockInt8::forward_cached (forward_int8.rs:207-216): attention
 // sublayer (:291-323) and FFN sublayer (:350-357).  m->x holds the residual
 // stream.  Rows path (fold false): on entry m->normed holds the block's
@@ -331,7 +358,7 @@ bool row_path(mri_llama *m) {
 // (row_proj); x_in is the block's input row (m->x, or the embedding row of
 // the first block, which the first projection copies into m->x).  Either
 // way the values are those of the separate steps.
-mri_status block(mri_llama *m, size_t li, size_t rows, size_t start, mri_kv_cache *c,
+mri_status block(mri_llama *m, size_t li, size_t rows, size_t start, const KvTarget &kv,
                  const float *next_norm, bool fold, const float *x_in, hipStream_t s) {
     const mri_llama_config &g = m->cfg;
     const Layer &L = m->layers[li];
@@ -392,7 +419,16 @@ mri_status block(mri_llama *m, size_t li, size_t rows, size_t start, mri_kv_cach
         TRY(proj(w, in, rows, m->tmp, s));
         return out_tail(norm);
     };
-    float *kc = c->k + li * c->max_seq * c->kvd, *vc = c->v + li * c->max_seq * c->kvd;
+    // (a 4-bit cache takes the rotated keys and the values from staging rows:
+    // behind the row's q, or in buffers that are free until the attention ends)
+    float *kc, *vc;
+    if (kv.f32) {
+        kc = kv.f32->k + li * kv.f32->max_seq * m->kvd;
+        vc = kv.f32->v + li * kv.f32->max_seq * m->kvd;
+    } else {
+        kc = fold ? m->qkv + m->qd : m->tmp;
+        vc = fold ? kc + m->kvd : m->attn;
+    }
     float *q, *k, *v;
     size_t qs, kvs;
     if (fold) {
@@ -401,7 +437,8 @@ mri_status block(mri_llama *m, size_t li, size_t rows, size_t start, mri_kv_cach
         if (m->hd % 2 || m->hd > 128)
             return set_error(MRI_ERR_UNSUPPORTED, "rope: head_dim must be even and <= 128");
         const size_t half = m->hd / 2;
-        float *krow = kc + start * c->kvd, *vrow = vc + start * c->kvd;
+        const size_t at = kv.f32 ? start * m->kvd : 0;
+        float *krow = kc + at, *vrow = vc + at;
         RowOps o = norm_ops(L.attn_norm);
         o.rope_cos = m->cos_t + start * half;
         o.rope_sin = m->sin_t + start * half;
@@ -444,11 +481,17 @@ mri_status block(mri_llama *m, size_t li, size_t rows, size_t start, mri_kv_cach
         TRY(in_proj(L.w[1], L.attn_norm, k));
         TRY(in_proj(L.w[2], L.attn_norm, v));
     }
-    if (!fold)
-        TRY(launch_rope_qkv(q, k, v, rows, g.n_heads, g.n_kv_heads, m->hd, qs, kvs, m->cos_t,
-                            m->sin_t, start, kc, vc, s));
-    TRY(launch_attention(q, qs, rows, kc, vc, g.n_heads, g.n_kv_heads, m->hd, start, m->attn,
-                         m->attn_part, s));
+    if (!fold) {
+        // (staged rows begin at row 0, with the table's rows from `start` on)
+        const size_t half = m->hd / 2, off = kv.f32 ? 0 : start * half;
+        TRY(launch_rope_qkv(q, k, v, rows, g.n_heads, g.n_kv_heads, m->hd, qs, kvs, m->cos_t + off,
+                            m->sin_t + off, kv.f32 ? start : 0, kc, vc, s));
+    }
+    if (kv.f32)
+        TRY(launch_attention(q, qs, rows, kc, vc, g.n_heads, g.n_kv_heads, m->hd, start, m->attn,
+                             m->attn_part, s));
+    else
+        TRY(attend_kv4(m, li, rows, kv, kc, vc, q, qs, s));
     TRY(out_proj(L.w[3], m->attn, L.ffn_norm));
     xrow = m->x;
     // gate rows, then up rows (one row: the gate projection stores the SiLU
@@ -499,7 +542,7 @@ enum class Emb { kDevice, kHost, kInX, kKeys };
 // arg: for a folded row, the greedy argmax (and next embedding row) that the
 // output projection's epilogue computes (the RowOps arg_* fields).
 mri_status run_rows(mri_llama *m, const uint32_t *tok_dev, size_t rows, size_t start,
-                    mri_kv_cache *c, float *logits, hipStream_t s, Emb emb = Emb::kDevice,
+                    const KvTarget &kv, float *logits, hipStream_t s, Emb emb = Emb::kDevice,
                     uint32_t host_tok = 0, const RowOps *arg = nullptr) {
     const mri_llama_config &g = m->cfg;
     const bool fold = rows == 1 && row_path(m);
@@ -518,7 +561,7 @@ mri_status run_rows(mri_llama *m, const uint32_t *tok_dev, size_t rows, size_t s
         TRY(launch_embed_rmsnorm(m->embd, tok_dev, rows, g.dim, first, g.eps, m->x, m->normed, s));
     }
     for (size_t li = 0; li < g.n_layers; ++li)
-        TRY(block(m, li, rows, start, c,
+        TRY(block(m, li, rows, start, kv,
                   li + 1 < g.n_layers ? m->layers[li + 1].attn_norm : m->out_norm, fold,
                   li == 0 ? x_in : m->x, s));
     if (!fold)
@@ -709,6 +752,38 @@ mri_status mri_llama_forward_cached(mri_llama *m, const uint32_t *tokens, size_t
         return run_rows(m, nullptr, 1, start_pos, c, logits, s, Emb::kHost, tokens[0]);
     MRI_HIP(hipMemcpyAsync(m->tok, tokens, n * sizeof(uint32_t), hipMemcpyHostToDevice, s));
     return run_rows(m, m->tok, n, start_pos, c, logits, s);
+}
+
+mri_status mri_llama_forward_kv4(mri_llama *m, const uint32_t *tokens, size_t n, size_t start_pos,
+                                 mri_kv4_cache *c, size_t seq, size_t cache_pos, float *weights,
+                                 float *logits, void *stream) {
+    if (!m || !c) return set_error(MRI_ERR_INVALID_ARGUMENT, "null model or cache");
+    for (size_t li = 0; li < m->cfg.n_layers; ++li)
+        if (!m->layers[li].set)
+            return set_error(MRI_ERR_INVALID_ARGUMENT, fmt_err("layer %zu is not set", li));
+    if (c->n_layers != m->cfg.n_layers || c->n_kv != m->cfg.n_kv_heads || c->hd != m->hd)
+        return set_error(MRI_ERR_SHAPE_MISMATCH, "KV cache shape does not match the model");
+    if (n == 0) return set_error(MRI_ERR_INVALID_SHAPE, "forward: token list must not be empty");
+    if (seq >= c->n_seqs)
+        return set_error(MRI_ERR_INVALID_SHAPE,
+                         fmt_err("sequence %zu of a cache of %zu", seq, c->n_seqs));
+    if (start_pos > m->cfg.max_seq || n > m->cfg.max_seq - start_pos)
+        return set_error(MRI_ERR_INVALID_SHAPE,
+                         fmt_err("positions %zu + %zu exceed the RoPE length %zu", start_pos, n,
+                                 m->cfg.max_seq));
+    if (cache_pos > c->max_seq || n > c->max_seq - cache_pos)
+        return set_error(MRI_ERR_INVALID_SHAPE,
+                         fmt_err("cache positions %zu + %zu exceed the cache length %zu",
+                                 cache_pos, n, c->max_seq));
+    TRY(check_tokens(m, tokens, n));
+    if (!logits) return set_error(MRI_ERR_INVALID_ARGUMENT, "null logits");
+    TRY(kv4_on_device(c));
+    auto s = static_cast<hipStream_t>(stream);
+    const KvTarget kv(c, seq, cache_pos, weights);
+    if (n == 1 && row_path(m))
+        return run_rows(m, nullptr, 1, start_pos, kv, logits, s, Emb::kHost, tokens[0]);
+    MRI_HIP(hipMemcpyAsync(m->tok, tokens, n * sizeof(uint32_t), hipMemcpyHostToDevice, s));
+    return run_rows(m, m->tok, n, start_pos, kv, logits, s);
 }
 
 mri_status mri_llama_forward_decode(mri_llama *m, uint32_t token, size_t pos, mri_kv_cache *c,

@@ -1,4 +1,5 @@
-"""ctypes binding of the GPU LlamaModelInt8 (include/mri_llama.h).
+"""ctypes binding of the GPU LlamaModelInt8, the 4-bit KV cache and the
+sampling operators (include/mri_llama.h).
 
 Host plumbing for tests and benchmarks over libmri_qmatmul.so: weights are
 the handles of mri_qmatmul (QMatrix / Q8Matrix) or device Q4_0 byte
@@ -28,6 +29,11 @@ class WeightRef(C.Structure):
     _fields_ = [("format", C.c_int), ("ptr", P), ("n_out", SZ), ("k_in", SZ)]
 
 
+class Kv4Rows(C.Structure):
+    _fields_ = [("first_seq", SZ), ("n_seqs", SZ), ("rows", SZ), ("start", SZ), ("pos", P),
+                ("count", P)]
+
+
 _SIGS = {
     "mri_llama_create": ([C.POINTER(Config), P, P, WeightRef, C.POINTER(P)], ST),
     "mri_llama_set_layer": ([P, SZ, P, P, C.POINTER(WeightRef)], ST),
@@ -38,6 +44,16 @@ _SIGS = {
     "mri_llama_forward_decode": ([P, C.c_uint32, SZ, P, P, P], ST),
     "mri_llama_generate_greedy": ([P, P, SZ, SZ, P, P, P, P], ST),
     "mri_argmax": ([P, SZ, SZ, P, P], ST),
+    "mri_kv4_cache_create": ([SZ, SZ, SZ, SZ, SZ, C.POINTER(P)], ST),
+    "mri_kv4_cache_device_bytes": ([P], SZ),
+    "mri_kv4_cache_destroy": ([P], None),
+    "mri_kv4_append": ([P, SZ, C.POINTER(Kv4Rows), P, P, SZ, P], ST),
+    "mri_kv4_read": ([P, SZ, SZ, C.POINTER(Kv4Rows), P, P, SZ, P], ST),
+    "mri_kv4_attend": ([P, SZ, C.POINTER(Kv4Rows), P, SZ, SZ, P, SZ, P, P], ST),
+    "mri_kv4_evict": ([P, P, P, P, P, P, SZ, SZ, P, P], ST),
+    "mri_llama_forward_kv4": ([P, P, SZ, SZ, P, SZ, SZ, P, P, P], ST),
+    "mri_softmax": ([P, SZ, SZ, SZ, C.c_float, P, SZ, P], ST),
+    "mri_verify_drafts": ([P, P, P, P, P, SZ, SZ, SZ, P, P, P], ST),
 }
 EXPORTED = tuple(_SIGS)
 
@@ -87,6 +103,139 @@ class KvCache:
             pass
 
 
+NO_TOKEN = 0xffffffff   # MRI_NO_TOKEN (-1 in int32 tensors)
+
+
+def _bad(kind, msg):
+    return Q.MriError({"InvalidShape": 1, "InvalidArgument": 3}[kind], msg)
+
+
+def _tensor(t, name, dtype, shape=None):
+    """A device pointer of t after its type, place and (contiguous) shape are checked."""
+    import torch
+    if t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+        raise _bad("InvalidArgument", f"{name}: dtype {t.dtype}")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise _bad("InvalidArgument", f"{name}: on {t.device}, not on the current device")
+    if shape is not None:
+        if tuple(t.shape) != tuple(shape):
+            raise _bad("InvalidShape", f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+        if not t.is_contiguous():
+            raise _bad("InvalidArgument", f"{name}: not contiguous")
+    return C.c_void_p(t.data_ptr())
+
+
+def _ints():
+    import torch
+    return (torch.int32, torch.uint32)
+
+
+def _row_stride(t, name):
+    """Floats between consecutive rows of t [..., rows, features]: the rows of all
+    leading indices follow each other at one distance."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise _bad("InvalidArgument", f"{name}: features are not contiguous")
+    stride, n = None, 1
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] > 1:
+            if stride is None:
+                stride = t.stride(d) // n if t.stride(d) % n == 0 else -1
+            if t.stride(d) != stride * n:
+                raise _bad("InvalidArgument", f"{name}: rows are not evenly spaced")
+        n *= t.shape[d]
+    return t.shape[-1] if stride is None else stride
+
+
+class Kv4Cache:
+    """The KV cache in 4-bit blocks (mri_kv4_*).  Rows are f32 tensors
+    [n_seqs, rows, features] (or [rows, features] of one sequence), evenly
+    spaced; `start` is the first row's position, an int or an int32 tensor
+    [n_seqs], `count` (int32 [n_seqs]) how many rows of a sequence are real."""
+
+    def __init__(self, n_layers, n_seqs, max_seq, n_kv_heads, head_dim):
+        h = C.c_void_p()
+        Q.check(lib().mri_kv4_cache_create(n_layers, n_seqs, max_seq, n_kv_heads, head_dim,
+                                           C.byref(h)))
+        self.h = h
+        self.n_layers, self.n_seqs, self.max_seq = n_layers, n_seqs, max_seq
+        self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
+
+    @property
+    def device_bytes(self):
+        return lib().mri_kv4_cache_device_bytes(self.h)
+
+    def _rows(self, t, start, count, first_seq):
+        n_seqs, rows = (1, t.shape[-2]) if t.dim() == 2 else t.shape[-3:-1]
+        r = Kv4Rows(first_seq, n_seqs, rows, 0, None, None)
+        if isinstance(start, int):
+            if start < 0:
+                raise _bad("InvalidShape", f"start {start} is negative")
+            r.start = start
+        else:
+            r.pos = _tensor(start, "start", _ints(), (n_seqs,))
+        if count is not None:
+            r.count = _tensor(count, "count", _ints(), (n_seqs,))
+        return r
+
+    def _kv(self, k, v, dims):
+        import torch
+        if k.dim() not in dims or k.shape != v.shape or \
+                k.shape[-1] != self.n_kv_heads * self.head_dim:
+            raise _bad("InvalidShape", f"k {tuple(k.shape)}, v {tuple(v.shape)}")
+        s = _row_stride(k, "k")
+        if _row_stride(v, "v") != s:
+            raise _bad("InvalidArgument", "k and v differ in their row stride")
+        return _tensor(k, "k", torch.float32), _tensor(v, "v", torch.float32), s
+
+    def append(self, layer, k, v, start, count=None, first_seq=0, stream=None):
+        kp, vp, s = self._kv(k, v, (2, 3))
+        r = self._rows(k, start, count, first_seq)
+        Q.check(lib().mri_kv4_append(self.h, layer, C.byref(r), kp, vp, s, Q._stream(stream)))
+
+    def read(self, layer, k, v, start, count=None, first_seq=0, stream=None):
+        """Into k and v; with a fourth leading axis, of that many layers."""
+        kp, vp, s = self._kv(k, v, (2, 3, 4))
+        r = self._rows(k, start, count, first_seq)
+        Q.check(lib().mri_kv4_read(self.h, layer, k.shape[0] if k.dim() == 4 else 1, C.byref(r),
+                                   kp, vp, s, Q._stream(stream)))
+
+    def attend(self, layer, q, out, start, count=None, first_seq=0, weights=None, stream=None):
+        """weights: f32 [n_seqs of the cache, n_kv_heads, max_seq] of this layer."""
+        import torch
+        if q.dim() not in (2, 3) or q.shape != out.shape or q.shape[-1] % self.head_dim:
+            raise _bad("InvalidShape", f"q {tuple(q.shape)}, out {tuple(out.shape)}")
+        qp, op = _tensor(q, "q", torch.float32), _tensor(out, "out", torch.float32)
+        r = self._rows(q, start, count, first_seq)
+        wp = None if weights is None else _tensor(
+            weights, "weights", torch.float32, (self.n_seqs, self.n_kv_heads, self.max_seq))
+        Q.check(lib().mri_kv4_attend(self.h, layer, C.byref(r), qp, _row_stride(q, "q"),
+                                     q.shape[-1] // self.head_dim, op, _row_stride(out, "out"),
+                                     wp, Q._stream(stream)))
+
+    def evict(self, dst, weights, weights_out, lens, lens_out, keep, recent, kept, stream=None):
+        """Into dst (self: in place, with weights_out = weights)."""
+        import torch
+        lead = (self.n_layers, self.n_seqs, self.n_kv_heads)
+        f = torch.float32
+        Q.check(lib().mri_kv4_evict(
+            self.h, dst.h, _tensor(weights, "weights", f, lead + (self.max_seq,)),
+            _tensor(weights_out, "weights_out", f, lead + (dst.max_seq,)),
+            _tensor(lens, "lens", _ints(), (self.n_seqs,)),
+            _tensor(lens_out, "lens_out", _ints(), (self.n_seqs,)), keep, recent,
+            _tensor(kept, "kept", _ints(), lead + (keep,)), Q._stream(stream)))
+
+    def close(self):
+        if self.h:
+            lib().mri_kv4_cache_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class Llama:
     """LlamaModelInt8 (forward_int8.rs:416-546) on the GPU.  `keep` holds the
     weight objects so that they outlive the model."""
@@ -123,6 +272,26 @@ class Llama:
                                                cache.h, C.c_void_p(logits.data_ptr()),
                                                Q._stream(stream)))
 
+    def kv4_cache(self, n_seqs=1, max_seq=None):
+        c = self.cfg
+        return Kv4Cache(len(self.keep[1]), n_seqs, max_seq or c["max_seq"], c["n_kv_heads"],
+                        c["dim"] // c["n_heads"])
+
+    def forward_kv4(self, tokens, start_pos, cache, logits, seq=0, cache_pos=None, weights=None,
+                    stream=None):
+        """cache_pos: start_pos unless keys were evicted.  weights: f32
+        [n_layers, n_seqs, n_kv_heads, max_seq] of the cache."""
+        import numpy as np
+        import torch
+        t = np.ascontiguousarray(tokens, np.uint32)
+        wp = None if weights is None else _tensor(
+            weights, "weights", torch.float32,
+            (cache.n_layers, cache.n_seqs, cache.n_kv_heads, cache.max_seq))
+        Q.check(lib().mri_llama_forward_kv4(
+            self.h, t.ctypes.data_as(P), t.size, start_pos, cache.h, seq,
+            start_pos if cache_pos is None else cache_pos, wp, C.c_void_p(logits.data_ptr()),
+            Q._stream(stream)))
+
     def forward_decode(self, token, pos, cache, logits, stream=None):
         Q.check(lib().mri_llama_forward_decode(self.h, int(token), pos, cache.h,
                                                C.c_void_p(logits.data_ptr()), Q._stream(stream)))
@@ -152,3 +321,34 @@ def argmax(v, idx, stream=None):
     rows, n = (1, v.numel()) if v.dim() == 1 else tuple(v.shape)
     Q.check(lib().mri_argmax(C.c_void_p(v.data_ptr()), rows, n, C.c_void_p(idx.data_ptr()),
                              Q._stream(stream)))
+
+
+def softmax(x, out, temperature=1.0, stream=None):
+    """Probabilities of rows of logits x [rows, n] (or [n]) into out; may be x."""
+    import torch
+    if x.shape != out.shape or x.dim() not in (1, 2):
+        raise _bad("InvalidShape", f"x {tuple(x.shape)}, out {tuple(out.shape)}")
+    rows, n = (1, x.numel()) if x.dim() == 1 else tuple(x.shape)
+    xp, op = _tensor(x, "x", torch.float32), _tensor(out, "out", torch.float32)
+    Q.check(lib().mri_softmax(xp, rows, n, _row_stride(x, "x"), temperature, op,
+                              _row_stride(out, "out"), Q._stream(stream)))
+
+
+def verify_drafts(drafts, target_probs, uniforms, tokens, accepted, draft_probs=None,
+                  n_drafts=None, stream=None):
+    """drafts int32 [n_seqs, k], target_probs f32 [n_seqs, k + 1, n], uniforms f32
+    [n_seqs, k + 1], draft_probs f32 [n_seqs, k, n], n_drafts int32 [n_seqs]; into
+    tokens int32 [n_seqs, k + 1] and accepted int32 [n_seqs]."""
+    import torch
+    if drafts.dim() != 2 or target_probs.dim() != 3:
+        raise _bad("InvalidShape",
+                   f"drafts {tuple(drafts.shape)}, target_probs {tuple(target_probs.shape)}")
+    (b, k), n, f = drafts.shape, target_probs.shape[2], torch.float32
+    dp = None if draft_probs is None else _tensor(draft_probs, "draft_probs", f, (b, k, n))
+    nd = None if n_drafts is None else _tensor(n_drafts, "n_drafts", _ints(), (b,))
+    Q.check(lib().mri_verify_drafts(
+        _tensor(drafts, "drafts", _ints(), (b, k)), dp,
+        _tensor(target_probs, "target_probs", f, (b, k + 1, n)),
+        _tensor(uniforms, "uniforms", f, (b, k + 1)), nd, b, k, n,
+        _tensor(tokens, "tokens", _ints(), (b, k + 1)),
+        _tensor(accepted, "accepted", _ints(), (b,)), Q._stream(stream)))

@@ -93,6 +93,13 @@ pub struct mri_kv_cache {
     _marker: PhantomData<(*mut u8, PhantomPinned)>,
 }
 
+/// KV cache in 4-bit blocks (`include/mri_llama.h`, an extension).
+#[repr(C)]
+pub struct mri_kv4_cache {
+    _data: [u8; 0],
+    _marker: PhantomData<(*mut u8, PhantomPinned)>,
+}
+
 // ---- model structs ------------------------------------------------------------
 
 /// The `LlamaConfig` fields the forward pass uses
@@ -121,6 +128,22 @@ pub struct mri_weight_ref {
     pub n_out: usize,
     pub k_in: usize,
 }
+
+/// The rows of a 4-bit cache call: `rows` per sequence at positions
+/// `(pos ? pos[b] : start) + i`; `pos` and `count` are nullable device arrays.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct mri_kv4_rows {
+    pub first_seq: usize,
+    pub n_seqs: usize,
+    pub rows: usize,
+    pub start: usize,
+    pub pos: *const u32,
+    pub count: *const u32,
+}
+
+/// `MRI_NO_TOKEN`: fills up token and position lists.
+pub const NO_TOKEN: u32 = 0xffff_ffff;
 
 // ---- include/mri_qmatmul.h ------------------------------------------------------
 
@@ -429,6 +452,98 @@ extern "C" {
         rows: usize,
         n: usize,
         idx: *mut u32,
+        stream: *mut c_void,
+    ) -> mri_status;
+
+    // the 4-bit KV cache and the operators of a decode loop over it
+    // (extensions; device pointers, mri_kv4_rows on the host)
+    pub fn mri_kv4_cache_create(
+        n_layers: usize,
+        n_seqs: usize,
+        max_seq: usize,
+        n_kv_heads: usize,
+        head_dim: usize,
+        out: *mut *mut mri_kv4_cache,
+    ) -> mri_status;
+    pub fn mri_kv4_cache_device_bytes(cache: *const mri_kv4_cache) -> usize;
+    pub fn mri_kv4_cache_destroy(cache: *mut mri_kv4_cache);
+    pub fn mri_kv4_append(
+        cache: *mut mri_kv4_cache,
+        layer: usize,
+        rows: *const mri_kv4_rows,
+        k: *const f32,
+        v: *const f32,
+        stride: usize,
+        stream: *mut c_void,
+    ) -> mri_status;
+    pub fn mri_kv4_read(
+        cache: *const mri_kv4_cache,
+        layer: usize,
+        n_layers: usize,
+        rows: *const mri_kv4_rows,
+        k: *mut f32,
+        v: *mut f32,
+        stride: usize,
+        stream: *mut c_void,
+    ) -> mri_status;
+    pub fn mri_kv4_attend(
+        cache: *mut mri_kv4_cache,
+        layer: usize,
+        rows: *const mri_kv4_rows,
+        q: *const f32,
+        q_stride: usize,
+        n_heads: usize,
+        out: *mut f32,
+        out_stride: usize,
+        weights: *mut f32,
+        stream: *mut c_void,
+    ) -> mri_status;
+    pub fn mri_kv4_evict(
+        src: *const mri_kv4_cache,
+        dst: *mut mri_kv4_cache,
+        weights: *const f32,
+        weights_out: *mut f32,
+        lens: *const u32,
+        lens_out: *mut u32,
+        keep: usize,
+        recent: usize,
+        kept: *mut u32,
+        stream: *mut c_void,
+    ) -> mri_status;
+    // forward_cached on one sequence of a 4-bit cache; tokens are host ids
+    pub fn mri_llama_forward_kv4(
+        model: *mut mri_llama,
+        tokens: *const u32,
+        n: usize,
+        start_pos: usize,
+        cache: *mut mri_kv4_cache,
+        seq: usize,
+        cache_pos: usize,
+        weights: *mut f32,
+        logits: *mut f32,
+        stream: *mut c_void,
+    ) -> mri_status;
+    pub fn mri_softmax(
+        x: *const f32,
+        rows: usize,
+        n: usize,
+        x_stride: usize,
+        temperature: f32,
+        out: *mut f32,
+        out_stride: usize,
+        stream: *mut c_void,
+    ) -> mri_status;
+    pub fn mri_verify_drafts(
+        drafts: *const u32,
+        draft_probs: *const f32,
+        target_probs: *const f32,
+        uniforms: *const f32,
+        n_drafts: *const u32,
+        n_seqs: usize,
+        k: usize,
+        n: usize,
+        tokens: *mut u32,
+        accepted: *mut u32,
         stream: *mut c_void,
     ) -> mri_status;
 }
