@@ -231,35 +231,69 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4Rows a, size_t layer_bytes,
 // ---- attention ----------------------------------------------------------------------
 // Sixteen queries (rows x query heads of one KV head, flattened row-major) are
 // the columns of S^T = K Q^T and O^T = V^T P^T, both on f16 matrix instructions
-// with f32 accuracy: the quants are small whole numbers, exact in f16; q is
-// split into two f16 halves (22 bits) after a power-of-two scaling of its row,
-// and so is p * d_v, the probability times the value block's scale, under a
-// power of two that follows the largest d_v seen (what is below 2^-39 of that
-// largest product is lost).  The key blocks' scales
-// multiply the 32-dim partial products in f32.
-__device__ inline half8_t unpack8(unsigned w) {
-    // 0x6400 | n is the f16 1024 + n, 0x6400 | 16 n is 1024 + 16 n
+// with f32 accuracy.
+//  * A nibble n masked out of a dword is the f16 n 2^-24 (16 n 2^-24 where the
+//    mask leaves it four bits up); one packed FMA makes it (n - 8) 2^-9.  (As
+//    subnormals the quants would go straight into the products, but the matrix
+//    instructions align them as they are: 2.0e-7 of sum |a b| off in the mean
+//    against 1.8e-9.)
+//  * q is split into two f16 halves (22 bits) after a power-of-two scaling of
+//    its row, and so is p * d_v, the probability times the value block's
+//    scale, under a power of two that follows the largest d_v seen (what is
+//    below 2^-39 of that largest product is lost).
+//  * The key blocks' scales multiply the 32-dim partial products in f32.
+typedef float float2_t __attribute__((ext_vector_type(2)));
+
+__device__ inline half8_t join(half2_t a, half2_t b, half2_t c, half2_t d) {
+    return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+constexpr unsigned kNib0 = 0x000f000fu, kNib1 = 0x00f000f0u;
+// The eight quants of a dword, times 2^-9.
+__device__ inline half8_t quants(unsigned w) {
+    const half2_t s0 = {(_Float16)0x1p15f, (_Float16)0x1p15f};
+    const half2_t s1 = {(_Float16)0x1p11f, (_Float16)0x1p11f};
+    const half2_t m8 = {(_Float16)-0x1p-6f, (_Float16)-0x1p-6f};
     const unsigned w8 = w >> 8;
-    const half2_t lo = {(_Float16)1032.0f, (_Float16)1032.0f};
-    const half2_t m16 = {(_Float16)0.0625f, (_Float16)0.0625f};
-    const half2_t c72 = {(_Float16)-72.0f, (_Float16)-72.0f};
-    const half2_t a0 = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | 0x64006400u) - lo;
-    const half2_t a1 = __builtin_elementwise_fma(
-        __builtin_bit_cast(half2_t, (w & 0x00f000f0u) | 0x64006400u), m16, c72);
-    const half2_t a2 = __builtin_bit_cast(half2_t, (w8 & 0x000f000fu) | 0x64006400u) - lo;
-    const half2_t a3 = __builtin_elementwise_fma(
-        __builtin_bit_cast(half2_t, (w8 & 0x00f000f0u) | 0x64006400u), m16, c72);
-    return half8_t{a0.x, a0.y, a1.x, a1.y, a2.x, a2.y, a3.x, a3.y};
+    return join(__builtin_elementwise_fma(__builtin_bit_cast(half2_t, w & kNib0), s0, m8),
+                __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w & kNib1), s1, m8),
+                __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w8 & kNib0), s0, m8),
+                __builtin_elementwise_fma(__builtin_bit_cast(half2_t, w8 & kNib1), s1, m8));
 }
 
-// x in two f16: hi + lo, off by 2^-22 of x at most where lo is not subnormal.
+// x in two f16, hi + lo: off by 2^-23 of x where lo is not subnormal.  (The
+// -1 is hidden from the compiler, which then takes the mixed-precision FMA
+// that rounds to f16 by itself: one instruction a value instead of three.)
+__device__ inline float minus_one() {
+    float v = -1.0f;
+    asm("" : "+s"(v));
+    return v;
+}
+__device__ inline void split2(float x0, float x1, half2_t *hi, half2_t *lo) {
+    const half2_t h = __builtin_convertvector((float2_t{x0, x1}), half2_t);
+    *hi = h;
+    const float m = minus_one();
+    *lo = half2_t{(_Float16)fmaf((float)h.x, m, x0), (_Float16)fmaf((float)h.y, m, x1)};
+}
 __device__ inline void split8(const float *x, half8_t *hi, half8_t *lo) {
+    half2_t h[4], l[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const _Float16 h = (_Float16)x[j];
-        (*hi)[j] = h;
-        (*lo)[j] = (_Float16)(x[j] - (float)h);
-    }
+    for (int u = 0; u < 4; ++u) split2(x[2 * u], x[2 * u + 1], &h[u], &l[u]);
+    *hi = join(h[0], h[1], h[2], h[3]);
+    *lo = join(l[0], l[1], l[2], l[3]);
+}
+
+// Sum and maximum over the four lanes of a column (lanes r, r + 16, ..).
+__device__ inline float col_max(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float col_sum(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // The query operand of a 16-column tile: column r of lane (g, r).
@@ -279,10 +313,9 @@ struct QTile {
                 x[b][j] = src ? src[32 * b + 8 * g + j] : 0.0f;
                 mx = fmaxf(mx, fabsf(x[b][j]));
             }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-        // the row's largest magnitude to [2^10, 2^11)
-        const int e = mx > 0.0f && mx < INFINITY ? min(10 - ilogbf(mx), 120) : 0;
+        mx = col_max(mx);
+        // the row's largest magnitude to [2^14, 2^15)
+        const int e = mx > 0.0f && mx < INFINITY ? min(14 - ilogbf(mx), 120) : 0;
         const float up = ldexpf(1.0f, e);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -290,98 +323,137 @@ struct QTile {
             for (int j = 0; j < 8; ++j) x[b][j] = x[b][j] * up;
             split8(x[b], &hi[b], &lo[b]);
         }
-        // log2(e) / sqrt(HD), rounded once
+        // 2^9 log2(e) / sqrt(HD), rounded once
         constexpr float c = HD == 64 ? 0.18033688011112042592f : 0.12751743021347021697f;
-        inv = ldexpf(c, -e);
+        inv = ldexpf(c, 9 - e);
     }
 };
 
-// Scores (log2 units) of the 16 keys of tile t of a page: keys 4 g + i of
-// column r in lane (g, r).
+// A page on its way through a wave: every byte is loaded once, in whole lines,
+// before the first is used (a wave that loads as it goes touches its page's
+// lines up to sixteen times, and sixteen such waves a CU are more than its
+// caches hold: 138 us for 196 MB of pages).  The scales go on through LDS, from
+// where each lane group takes those of its keys.
 template <int HD>
-__device__ inline float4_t score_tile(const uint8_t *pb, int t, int lane, const QTile<HD> &q) {
-    using P = Page<HD>;
-    constexpr int NB = P::NB;
-    unsigned w[NB];
-    const uint8_t *kp = pb + t * 8 * HD + lane * 4 * NB;
-    const uint8_t *sp = pb + P::kKs + (t * 4 + (lane >> 4)) * NB * 8;
-    uint2 d[NB];
-    if constexpr (NB == 4) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(kp);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else {
-        const uint2 v = *reinterpret_cast<const uint2 *>(kp);
-        w[0] = v.x, w[1] = v.y;
-    }
+struct PageLoad {
+    static constexpr int NB = HD / 32;
+    unsigned k[4][NB];          // tile, block
+    unsigned v[HD / 16][2];     // dim tile, key half
+    unsigned ks[NB / 2], vs[NB / 2];  // scales, in order over the lanes
+    __device__ void load(const uint8_t *pb, int lane) {
+        load_k(pb, lane);
 #pragma unroll
-    for (int b = 0; b < NB; b += 2) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(sp + 8 * b);
-        d[b] = uint2{v.x, v.y};
-        d[b + 1] = uint2{v.z, v.w};
+        for (int c = 0; c < HD / 32; ++c) {
+            const uint4 x =
+                *reinterpret_cast<const uint4 *>(pb + Page<HD>::kV + c * 1024 + lane * 16);
+            v[2 * c][0] = x.x, v[2 * c][1] = x.y, v[2 * c + 1][0] = x.z, v[2 * c + 1][1] = x.w;
+        }
+        load_scales(pb + Page<HD>::kVs, lane, vs);
     }
+    __device__ void load_k(const uint8_t *pb, int lane) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint8_t *kp = pb + t * 8 * HD + lane * (HD / 8);
+            if constexpr (HD == 128) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(kp);
+                k[t][0] = x.x, k[t][1] = x.y, k[t][2] = x.z, k[t][3] = x.w;
+            } else {
+                const uint2 x = *reinterpret_cast<const uint2 *>(kp);
+                k[t][0] = x.x, k[t][1] = x.y;
+            }
+        }
+        load_scales(pb + Page<HD>::kKs, lane, ks);
+    }
+    static __device__ void load_scales(const uint8_t *sp, int lane, unsigned *d) {
+        if constexpr (HD == 128) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(sp + 8 * lane);
+            d[0] = x.x, d[1] = x.y;
+        } else {
+            d[0] = *reinterpret_cast<const unsigned *>(sp + 4 * lane);
+        }
+    }
+    static __device__ void stage(const unsigned *d, int lane, unsigned *lds) {
+#pragma unroll
+        for (int u = 0; u < NB / 2; ++u) lds[lane * (NB / 2) + u] = d[u];
+    }
+};
+template <int HD>
+constexpr int kScaleWords = 64 * HD / 64;  // of the keys or the values of a page
+
+// A tile's raw scores (times q.inv: log2 units), of the keys 4 g + i of column r
+// in lane (g, r).  w: the K dwords; sp: the tile's staged scales of this lane
+// group, two dwords a block.
+template <int HD>
+__device__ inline float4_t score_tile(const unsigned *w, const unsigned *sp, const QTile<HD> &q) {
+    constexpr int NB = HD / 32;
+    unsigned d[2 * NB];
+#pragma unroll
+    for (int u = 0; u < NB / 2; ++u)
+        *reinterpret_cast<uint4 *>(d + 4 * u) = reinterpret_cast<const uint4 *>(sp)[u];
     float4_t s = {0, 0, 0, 0};
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        const half8_t kq = unpack8(w[b]);
+        const half8_t kn = quants(w[b]);
         float4_t c = {0, 0, 0, 0};
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q.lo[b], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q.hi[b], c, 0, 0, 0);
-        const half2_t d01 = __builtin_bit_cast(half2_t, d[b].x),
-                      d23 = __builtin_bit_cast(half2_t, d[b].y);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kn, q.lo[b], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kn, q.hi[b], c, 0, 0, 0);
+        const half2_t d01 = __builtin_bit_cast(half2_t, d[2 * b]),
+                      d23 = __builtin_bit_cast(half2_t, d[2 * b + 1]);
         s[0] = fmaf(c[0], (float)d01.x, s[0]);
         s[1] = fmaf(c[1], (float)d01.y, s[1]);
         s[2] = fmaf(c[2], (float)d23.x, s[2]);
         s[3] = fmaf(c[3], (float)d23.y, s[3]);
     }
-    return s * q.inv;
+    return s;
 }
 
 // The running softmax of a wave's 16 columns.
 template <int HD>
 struct Softmax {
-    float m = -INFINITY, l = 0.0f;  // per column; l of this lane's keys only
-    int ve = -100;                  // 2^ve <= the largest d_v seen; o is in units of 2^(ve - 14)
+    float m = -INFINITY;  // per column, log2 units
+    float l = 0.0f;       // of this lane's keys; l and o in units of 2^(ve - 14)
+    int ve = -100;        // 2^ve <= the largest d_v seen < 2^(ve + 1)
     float4_t o[HD / 16];
     __device__ Softmax() {
 #pragma unroll
         for (int e = 0; e < HD / 16; ++e) o[e] = float4_t{0, 0, 0, 0};
     }
+    __device__ void scale(float f) {
+        l = l * f;
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) o[e] = o[e] * f;
+    }
 };
 
-// Adds one page: keys [0, lim) of it are seen by this lane's column (lim <= 0:
-// none), the first n_keys by any; `whole`: all 64 by every column.
-template <int HD>
-__device__ inline void attend_page(const uint8_t *pb, int lane, const QTile<HD> &q, int lim,
-                                   int n_keys, bool whole, Softmax<HD> &st) {
-    using P = Page<HD>;
-    constexpr int NB = P::NB;
+// Adds one page.  WHOLE: every column sees its 64 keys; else keys [0, lim) of it
+// are seen by this lane's column (lim <= 0: none), the first n_keys by any.
+// s_ks, s_vs: its staged scales.
+template <int HD, bool WHOLE>
+__device__ inline void attend_page(const PageLoad<HD> &pl, const unsigned *s_ks,
+                                   const unsigned *s_vs, int lane, const QTile<HD> &q, int lim,
+                                   int n_keys, Softmax<HD> &st) {
+    constexpr int NB = HD / 32;
     const int g = lane >> 4;
-    // the page's V scales: their largest sets the power of two
+    // the page's largest V scale; it seldom grows past the power of two in use
     float dmax = 0.0f;
-    {
-        const unsigned *sp = reinterpret_cast<const unsigned *>(pb + P::kVs);
 #pragma unroll
-        for (int u = 0; u < NB / 2; ++u) {
-            const int w = u * 64 + lane;
-            half2_t d = __builtin_bit_cast(half2_t, sp[w]);
-            if (!whole) {  // what lies past the end counts for nothing
-                const int key = w / (2 * NB) * 4 + 2 * (w & 1);
-                if (key >= n_keys) d.x = (_Float16)0.0f;
-                if (key + 1 >= n_keys) d.y = (_Float16)0.0f;
-            }
-            dmax = fmaxf(dmax, fmaxf(fabsf((float)d.x), fabsf((float)d.y)));
+    for (int u = 0; u < NB / 2; ++u) {
+        half2_t d = __builtin_bit_cast(half2_t, pl.vs[u] & 0x7fff7fffu);
+        if (!WHOLE) {  // what lies past the end counts for nothing
+            const int w = lane * (NB / 2) + u, key = w / (2 * NB) * 4 + 2 * (w & 1);
+            if (key >= n_keys) d.x = (_Float16)0.0f;
+            if (key + 1 >= n_keys) d.y = (_Float16)0.0f;
         }
-#pragma unroll
-        for (int x = 1; x < kWave; x <<= 1) dmax = fmaxf(dmax, __shfl_xor(dmax, x, kWave));
+        dmax = fmaxf(dmax, fmaxf((float)d.x, (float)d.y));
     }
     float s[16];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        const float4_t v = score_tile<HD>(pb, t, lane, q);
+        const float4_t v = score_tile<HD>(pl.k[t], s_ks + (t * 4 + g) * 2 * NB, q);
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[4 * t + i] = v[i];
     }
-    if (!whole) {
+    if (!WHOLE) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -391,69 +463,66 @@ __device__ inline void attend_page(const uint8_t *pb, int lane, const QTile<HD> 
     float pm = s[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[i]);
-    pm = fmaxf(pm, __shfl_xor(pm, 16, kWave));
-    pm = fmaxf(pm, __shfl_xor(pm, 32, kWave));
-    // f16 exponent of the largest scale, 2^ve <= d < 2^(ve + 1)
-    int ve = dmax > 0.0f && dmax < INFINITY ? ilogbf(dmax) : -24;
-    ve = max(ve, st.ve);
-    const float m_new = fmaxf(st.m, pm);
-    if (__any(m_new > st.m || ve > st.ve)) {
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f(st.m - m_use);
-        st.l = st.l * alpha;
-        const float f = ldexpf(alpha, st.ve - ve);
+    const float m_new = fmaxf(st.m, col_max(pm) * q.inv);
+    if (__any(m_new > st.m || dmax >= ldexpf(1.0f, st.ve + 1))) {
 #pragma unroll
-        for (int e = 0; e < HD / 16; ++e) st.o[e] = st.o[e] * f;
+        for (int x = 1; x < kWave; x <<= 1) dmax = fmaxf(dmax, __shfl_xor(dmax, x, kWave));
+        const int ve = max(dmax > 0.0f ? ilogbf(dmax) : -24, st.ve);
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+        st.scale(ldexpf(__builtin_amdgcn_exp2f(st.m - m_use), st.ve - ve));
         st.m = m_new;
         st.ve = ve;
     }
-    const float m_use = st.m == -INFINITY ? 0.0f : st.m;
-    const float up = ldexpf(1.0f, 14 - st.ve);  // p * d_v to below 2^15
+    // p 2^(14 - ve)
+    const float m0 = (st.m == -INFINITY ? 0.0f : st.m) - (float)(14 - st.ve);
     float p[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
+        p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], q.inv, -m0));
         st.l = st.l + p[i];
-        p[i] = p[i] * up;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        half8_t ph[NB], pl[NB];
+        half8_t ph[NB], pl8[NB];
+        unsigned dv[2][2 * NB];  // the scales of tiles 2 h and 2 h + 1
+#pragma unroll
+        for (int u = 0; u < NB; ++u)
+            *reinterpret_cast<uint4 *>(&dv[u / (NB / 2)][u % (NB / 2) * 4]) =
+                reinterpret_cast<const uint4 *>(s_vs + ((2 * h + u / (NB / 2)) * 4 + g) * 2 * NB)
+                    [u % (NB / 2)];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            float x[8];
+            half2_t hh[4], ll[4];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint2 d = *reinterpret_cast<const uint2 *>(
-                    pb + P::kVs + (((2 * h + u) * 4 + g) * NB + b) * 8);
-                const half2_t d01 = __builtin_bit_cast(half2_t, d.x),
-                              d23 = __builtin_bit_cast(half2_t, d.y);
-                const float dv[4] = {(float)d01.x, (float)d01.y, (float)d23.x, (float)d23.y};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = 4 * (2 * h + u) + i;
-                    x[4 * u + i] = p[n] * dv[i];
-                    // a key past the end may hold anything, NaN too
-                    if (!whole && 16 * (2 * h + u) + 4 * g + i >= lim) x[4 * u + i] = 0.0f;
+            for (int u = 0; u < 4; ++u) {  // keys 16 t + 4 g + 2 (u % 2) + {0, 1}
+                const int t = 2 * h + (u >> 1), n = 4 * t + 2 * (u & 1);
+                half2_t d = __builtin_bit_cast(half2_t, dv[u >> 1][2 * b + (u & 1)]);
+                if (!WHOLE) {  // a key past the end may hold anything, NaN too
+                    const int key = 16 * t + 4 * g + 2 * (u & 1);
+                    if (key >= lim) d.x = (_Float16)0.0f;
+                    if (key + 1 >= lim) d.y = (_Float16)0.0f;
                 }
+                split2(fmaf(p[n], (float)d.x, 0.0f), fmaf(p[n + 1], (float)d.y, 0.0f), &hh[u],
+                       &ll[u]);
             }
-            split8(x, &ph[b], &pl[b]);
+            ph[b] = join(hh[0], hh[1], hh[2], hh[3]);
+            pl8[b] = join(ll[0], ll[1], ll[2], ll[3]);
         }
 #pragma unroll
         for (int e = 0; e < HD / 16; ++e) {
-            const unsigned w = *reinterpret_cast<const unsigned *>(
-                pb + P::kV + (e >> 1) * 1024 + lane * 16 + (e & 1) * 8 + 4 * h);
-            const half8_t vq = unpack8(w);
-            st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, pl[e >> 1], st.o[e], 0, 0, 0);
+            const half8_t vq = quants(pl.v[e][h]);
+            st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, pl8[e >> 1], st.o[e], 0, 0, 0);
             st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, ph[e >> 1], st.o[e], 0, 0, 0);
         }
     }
 }
 
-// How the pages of a call's sequences are dealt to `slots` runs of at most
-// `chunk` pages: sequence b takes ceil(pages_b / chunk) runs.  chunk is the
-// least for which the runs suffice (every wave computes the same).
-constexpr int kMinChunk = 4;
+// How the pages of a call's sequences are dealt to at most `slots` runs (slots
+// >= 2 n_seqs) of at most `chunk` pages: sequence b takes ceil(pages_b / chunk)
+// of them, in order.  chunk = ceil(total / slots) where the sequences' last, short
+// runs leave room for that, else ceil(total / (slots - n_seqs)), which always
+// suffices.  Every wave computes the same, a sequence a lane.
+constexpr unsigned kMinChunk = 4;
 __device__ inline unsigned seq_pages(const Kv4Rows &a, int b) {
     unsigned p0;
     const unsigned cnt = rows_of(a, b, &p0);
@@ -464,74 +533,97 @@ __device__ inline unsigned wave_sum_u(unsigned v) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
     return v;
 }
-__device__ inline unsigned run_chunk(const Kv4Rows &a, unsigned slots) {
+struct Run {
+    int b;                // the sequence, -1: no such run
+    unsigned first, n;    // its runs
+    unsigned pg0, pg1;    // the run's pages
+};
+__device__ inline Run find_run(const Kv4Rows &a, unsigned slots, unsigned slot) {
     const int lane = threadIdx.x & 63;
-    unsigned total = 0;
-    for (int b = lane; b < a.n_seqs; b += kWave) total += seq_pages(a, b);
-    total = wave_sum_u(total);
-    unsigned chunk = max((total + slots - 1) / slots, (unsigned)kMinChunk);
-    for (;;) {
-        unsigned runs = 0;
-        for (int b = lane; b < a.n_seqs; b += kWave) runs += (seq_pages(a, b) + chunk - 1) / chunk;
-        runs = wave_sum_u(runs);
-        if (runs <= slots) return chunk;
-        chunk += max(chunk / 16, 1u);
+    const unsigned n_seqs = a.n_seqs;
+    if (n_seqs == 1) {
+        const unsigned np = seq_pages(a, 0), chunk = max((np + slots - 1) / slots, kMinChunk);
+        const unsigned n = (np + chunk - 1) / chunk;
+        return Run{slot < n ? 0 : -1, 0, n, slot * chunk, min(slot * chunk + chunk, np)};
     }
+    const unsigned mine = lane < (int)n_seqs ? seq_pages(a, lane) : 0;  // of the first 64
+    unsigned total = mine;
+    for (unsigned b = lane + kWave; b < n_seqs; b += kWave) total += seq_pages(a, b);
+    total = wave_sum_u(total);
+    unsigned chunk = max((total + slots - 1) / slots, kMinChunk);
+    unsigned runs = (mine + chunk - 1) / chunk;
+    for (unsigned b = lane + kWave; b < n_seqs; b += kWave)
+        runs += (seq_pages(a, b) + chunk - 1) / chunk;
+    if (wave_sum_u(runs) > slots)
+        chunk = max((total + slots - n_seqs - 1) / (slots - n_seqs), kMinChunk);
+    unsigned before = 0;
+    for (unsigned b0 = 0; b0 < n_seqs; b0 += kWave) {
+        const unsigned np = b0 == 0 ? mine : b0 + lane < n_seqs ? seq_pages(a, b0 + lane) : 0;
+        const unsigned n = (np + chunk - 1) / chunk;
+        unsigned inc = n;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const unsigned y = __shfl_up(inc, o, kWave);
+            if (lane >= o) inc += y;
+        }
+        const unsigned long long over = __ballot(before + inc > slot);
+        if (over) {
+            const int l = __ffsll((long long)over) - 1;
+            Run r;
+            r.b = (int)b0 + l;
+            r.n = __shfl(n, l, kWave);
+            r.first = before + __shfl(inc, l, kWave) - r.n;
+            r.pg0 = (slot - r.first) * chunk;
+            r.pg1 = min(r.pg0 + chunk, (unsigned)__shfl(np, l, kWave));
+            return r;
+        }
+        before += __shfl(inc, kWave - 1, kWave);
+    }
+    return Run{-1, 0, 0, 0, 0};
 }
 
-// (the runs of one sequence never need more than max_seq / 64 pages, and with
-// slots >= n_seqs the loop above ends)
-
-// The first run and the number of runs of sequence b.
-__device__ inline void runs_of(const Kv4Rows &a, unsigned chunk, int b, unsigned *first,
-                               unsigned *n) {
-    const int lane = threadIdx.x & 63;
-    unsigned before = 0;
-    for (int i = lane; i < b; i += kWave) before += (seq_pages(a, i) + chunk - 1) / chunk;
-    *first = wave_sum_u(before);
-    *n = (seq_pages(a, b) + chunk - 1) / chunk;
+__device__ inline void part_store(float *p, float v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline float part_load(const float *p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 constexpr int kFewWaves = 4;
 
 // Grid: slots x (KV heads x query tiles).  SPLIT: a slot is a run of pages of
-// one sequence, whose partial results go to `part`; else it is a sequence.
-// The four waves take every fourth page and meet in LDS.
+// one sequence; else it is a sequence.  The four waves take every fourth page
+// and meet in LDS.  Where a sequence has several runs, each publishes its columns'
+// (m, l, o) in `part` by device-scope stores that are complete before it counts
+// itself on the tile's counter; the one that counts last joins them in the order
+// of the runs and leaves the counter zero, so none waits for another.
 template <int HD, bool SPLIT>
 __global__ __launch_bounds__(kFewWaves *kWave) void k_kv4_attend(
     Kv4Rows a, const float *__restrict__ q, size_t qs, int groups, int n_qt, unsigned slots,
-    float *__restrict__ out, size_t os, float *__restrict__ part, float *__restrict__ lse) {
+    float *__restrict__ out, size_t os, float *__restrict__ part, int *__restrict__ cnts,
+    float *__restrict__ lse) {
     using P = Page<HD>;
     __shared__ float s_m[kFewWaves][16], s_l[kFewWaves][16];
     __shared__ __attribute__((aligned(16))) float s_o[kFewWaves][16][HD + 4];
+    __shared__ __attribute__((aligned(16))) unsigned s_d[kFewWaves][2][kScaleWords<HD>];
+    __shared__ int s_last;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
     const int qt = blockIdx.x % n_qt, head = blockIdx.x / n_qt % a.n_kv;
     const unsigned slot = blockIdx.x / (n_qt * a.n_kv);
-    int b = (int)slot;
-    unsigned pg0 = 0, pg1 = 0;
+    Run run{(int)slot, 0, 1, 0, 0};
     if constexpr (SPLIT) {
-        const unsigned chunk = run_chunk(a, slots);
-        // the sequence of this run
-        unsigned first = 0;
-        for (b = 0; b < a.n_seqs; ++b) {
-            const unsigned np = seq_pages(a, b), n = (np + chunk - 1) / chunk;
-            if (slot < first + n) {
-                pg0 = (slot - first) * chunk;
-                pg1 = min(pg0 + chunk, np);
-                break;
-            }
-            first += n;
-        }
-        if (b == a.n_seqs) return;
+        run = find_run(a, slots, slot);
+        if (run.b < 0) return;
     }
+    const int b = run.b;
     unsigned p0;
     const int cnt = (int)rows_of(a, b, &p0);
     const int n_q = cnt * groups;       // real queries of the KV head
     if (qt * 16 >= n_q) return;
     const int last_row = (min(qt * 16 + 16, n_q) - 1) / groups;
     const unsigned end = p0 + last_row + 1;  // keys that the tile's last row sees
-    if constexpr (!SPLIT) pg1 = (end + kPageKeys - 1) / kPageKeys;
-    pg1 = min(pg1, (end + kPageKeys - 1) / kPageKeys);
+    const unsigned end_pg = (end + kPageKeys - 1) / kPageKeys;
+    const unsigned pg1 = SPLIT ? min(run.pg1, end_pg) : end_pg;
     const int qi = qt * 16 + r, row = qi / groups;
     const bool real = qi < n_q;
     const size_t qrow = row_index(a, b, row);
@@ -543,28 +635,55 @@ __global__ __launch_bounds__(kFewWaves *kWave) void k_kv4_attend(
     Softmax<HD> st;
     const uint8_t *base =
         a.pages + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages * P::kBytes;
-    for (unsigned pg = pg0 + wv; pg < pg1; pg += kFewWaves) {
+    // a page's loads are in flight while the one before it is computed
+    PageLoad<HD> next;
+    unsigned pg = run.pg0 + wv;
+    if (pg < pg1) next.load(base + (size_t)pg * P::kBytes, lane);
+    for (; pg < pg1; pg += kFewWaves) {
+        const PageLoad<HD> now = next;
+        __builtin_amdgcn_wave_barrier();  // the last page's scales are read (LDS is in order)
+        PageLoad<HD>::stage(now.ks, lane, s_d[wv][0]);
+        PageLoad<HD>::stage(now.vs, lane, s_d[wv][1]);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (pg + kFewWaves < pg1) next.load(base + (size_t)(pg + kFewWaves) * P::kBytes, lane);
         const bool whole = (pg + 1) * kPageKeys <= all;
         const long lim = see - (long)pg * kPageKeys;
-        attend_page<HD>(base + (size_t)pg * P::kBytes, lane, qtile, (int)min(lim, 64l),
-                        (int)min(end - pg * kPageKeys, 64u), whole, st);
+        if (whole)
+            attend_page<HD, true>(now, s_d[wv][0], s_d[wv][1], lane, qtile, 64, 64, st);
+        else
+            attend_page<HD, false>(now, s_d[wv][0], s_d[wv][1], lane, qtile, (int)min(lim, 64l),
+                                   (int)min(end - pg * kPageKeys, 64u), st);
     }
-    // the column's sum over its four lane groups, then the waves
-    st.l = st.l + __shfl_xor(st.l, 16, kWave);
-    st.l = st.l + __shfl_xor(st.l, 32, kWave);
+    // o holds 2^-9 of the quants; l and o back to their own units, the
+    // column's sum over its four lane groups, then the waves
+    const float down = ldexpf(1.0f, st.ve - 14);
+    st.l = col_sum(st.l) * down;
     if (g == 0) {
         s_m[wv][r] = st.m;
         s_l[wv][r] = st.l;
     }
-    const float down = ldexpf(1.0f, st.ve - 14);
 #pragma unroll
     for (int e = 0; e < HD / 16; ++e)
-        *reinterpret_cast<float4_t *>(&s_o[wv][r][16 * e + 4 * g]) = st.o[e] * down;
+        *reinterpret_cast<float4_t *>(&s_o[wv][r][16 * e + 4 * g]) =
+            st.o[e] * (down * 0x1p9f);
     __syncthreads();
-    for (int it = threadIdx.x; it < 16 * HD; it += kFewWaves * kWave) {
+    const int cols = min(16, n_q - qt * 16);
+    const size_t z0 = ((size_t)b * a.rows) * (a.n_kv * groups);
+    auto store = [&](int c, int d, float m, float l, float o) {
+        const int ci = qt * 16 + c, oh = head * groups + ci % groups;
+        out[row_index(a, b, ci / groups) * os + oh * HD + d] = o / l;
+        if (lse && d == 0)
+            lse[z0 + (size_t)(ci / groups) * (a.n_kv * groups) + oh] = m + __log2f(l);
+    };
+    const bool alone = !SPLIT || run.n == 1;
+    // partial results of run i, column c
+    auto part_of = [&](unsigned i, int c) {
+        return part + ((((size_t)(run.first + i) * a.n_kv + head) * n_qt + qt) * 16 + c) * (HD + 2);
+    };
+    for (int it = threadIdx.x; it < cols * HD; it += kFewWaves * kWave) {
         const int c = it / HD, d = it % HD;
-        const int ci = qt * 16 + c;
-        if (ci >= n_q) break;
         float m = s_m[0][c];
 #pragma unroll
         for (int w = 1; w < kFewWaves; ++w) m = fmaxf(m, s_m[w][c]);
@@ -576,57 +695,58 @@ __global__ __launch_bounds__(kFewWaves *kWave) void k_kv4_attend(
             l = l + s_l[w][c] * f;
             o = o + s_o[w][c][d] * f;
         }
-        if constexpr (SPLIT) {
-            float *pc = part + ((size_t)blockIdx.x * 16 + c) * (HD + 2);
-            pc[2 + d] = o;
-            if (d == 0) {
-                pc[0] = m;
-                pc[1] = l;
-            }
+        if (alone) {
+            store(c, d, m_use, l, o);
         } else {
-            const size_t orow = row_index(a, b, ci / groups);
-            const int oh = head * groups + ci % groups;
-            out[orow * os + oh * HD + d] = o / l;
-            if (lse && d == 0) lse[((size_t)b * a.rows + ci / groups) * (a.n_kv * groups) + oh] = m_use + __log2f(l);
+            float *pc = part_of(slot - run.first, c);
+            part_store(pc + 2 + d, o);
+            if (d == 0) {
+                part_store(pc, m);
+                part_store(pc + 1, l);
+            }
         }
     }
-}
-
-// Joins the runs of one (sequence, KV head, query tile, column).
-template <int HD>
-__global__ __launch_bounds__(HD) void k_kv4_join(Kv4Rows a, int groups, int n_qt, unsigned slots,
-                                                 const float *__restrict__ part,
-                                                 float *__restrict__ out, size_t os,
-                                                 float *__restrict__ lse) {
-    const int d = threadIdx.x;
-    const int c = blockIdx.x % 16;
-    const int qt = blockIdx.x / 16 % n_qt, head = blockIdx.x / (16 * n_qt) % a.n_kv;
-    const int b = blockIdx.x / (16 * n_qt * a.n_kv);
-    unsigned p0;
-    const int cnt = (int)rows_of(a, b, &p0);
-    const int ci = qt * 16 + c;
-    if (ci >= cnt * groups) return;
-    const unsigned chunk = run_chunk(a, slots);
-    unsigned first, n;
-    runs_of(a, chunk, b, &first, &n);
-    // runs past the tile's last row wrote nothing useful but m = -inf, l = 0
-    auto at = [&](unsigned i) {
-        return part + ((((size_t)(first + i) * a.n_kv + head) * n_qt + qt) * 16 + c) * (HD + 2);
-    };
-    float m = -INFINITY;
-    for (unsigned i = 0; i < n; ++i) m = fmaxf(m, at(i)[0]);
-    const float m_use = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o = 0.0f;
-    for (unsigned i = 0; i < n; ++i) {
-        const float *pc = at(i);
-        const float f = __builtin_amdgcn_exp2f(pc[0] - m_use);
-        l = l + pc[1] * f;
-        o = o + pc[2 + d] * f;
+    if (alone) return;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's partials are at the device
+    __syncthreads();
+    int *cn = cnts + ((size_t)b * a.n_kv + head) * n_qt + qt;
+    if (threadIdx.x == 0)
+        s_last = __hip_atomic_fetch_add(cn, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                 (int)run.n - 1;
+    __syncthreads();
+    if (!s_last) return;
+    if (threadIdx.x == 0) __hip_atomic_store(cn, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int it = threadIdx.x; it < cols * HD; it += kFewWaves * kWave) {
+        const int c = it / HD, d = it % HD;
+        constexpr unsigned B = 8;
+        float m = -INFINITY, l = 0.0f, o = 0.0f;
+        for (unsigned i0 = 0; i0 < run.n; i0 += B) {  // B runs' loads in flight
+            float pm[B], pl[B], po[B];
+#pragma unroll
+            for (unsigned u = 0; u < B; ++u) {
+                const float *pc = part_of(min(i0 + u, run.n - 1), c);
+                pm[u] = part_load(pc);
+                pl[u] = part_load(pc + 1);
+                po[u] = part_load(pc + 2 + d);
+            }
+            float mn = m;
+#pragma unroll
+            for (unsigned u = 0; u < B; ++u) mn = fmaxf(mn, pm[u]);
+            const float m_use = mn == -INFINITY ? 0.0f : mn, f0 = __builtin_amdgcn_exp2f(m - m_use);
+            l = l * f0;
+            o = o * f0;
+            m = mn;
+#pragma unroll
+            for (unsigned u = 0; u < B; ++u) {
+                if (i0 + u < run.n) {
+                    const float f = __builtin_amdgcn_exp2f(pm[u] - m_use);
+                    l = l + pl[u] * f;
+                    o = o + po[u] * f;
+                }
+            }
+        }
+        store(c, d, m, l, o);
     }
-    const size_t orow = row_index(a, b, ci / groups);
-    const int oh = head * groups + ci % groups;
-    out[orow * os + oh * HD + d] = o / l;
-    if (lse && d == 0) lse[((size_t)b * a.rows + ci / groups) * (a.n_kv * groups) + oh] = m_use + __log2f(l);
 }
 
 // The keys' attention weights: one wave a page of a KV head goes over all the
@@ -650,6 +770,11 @@ __global__ __launch_bounds__(kWave) void k_kv4_weights(Kv4Rows a, const float *_
     const int n_q = cnt * groups;
     const uint8_t *pb = a.pages + (((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages + pg) *
                                       P::kBytes;
+    __shared__ __attribute__((aligned(16))) unsigned s_d[kScaleWords<HD>];
+    PageLoad<HD> page;
+    page.load_k(pb, lane);
+    PageLoad<HD>::stage(page.ks, lane, s_d);
+    __syncthreads();
     float w[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = 0.0f;
@@ -665,11 +790,13 @@ __global__ __launch_bounds__(kWave) void k_kv4_weights(Kv4Rows a, const float *_
         const long lim = real ? (long)p0 + row + 1 - (long)key0 : 0;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const float4_t s = score_tile<HD>(pb, t, lane, qtile);
+            const float4_t s =
+                score_tile<HD>(page.k[t], s_d + (t * 4 + g) * 2 * P::NB, qtile);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (16 * t + 4 * g + i < lim)
-                    w[4 * t + i] = w[4 * t + i] + __builtin_amdgcn_exp2f(s[i] - z);
+                    w[4 * t + i] =
+                        w[4 * t + i] + __builtin_amdgcn_exp2f(fmaf(s[i], qtile.inv, -z));
         }
     }
 #pragma unroll
@@ -950,33 +1077,28 @@ namespace {
 // asked for.
 template <int HD>
 mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_heads, float *out,
-                       size_t os, float *weights, float *part, float *lse, hipStream_t s) {
+                       size_t os, float *weights, float *part, int *cnts, float *lse,
+                       hipStream_t s) {
     const int groups = (int)(n_heads / a.n_kv);
     const size_t n_qt = ((size_t)a.rows * groups + 15) / 16;
     const size_t tiles = n_qt * a.n_kv;
     float *z = weights ? lse : nullptr;
-    // two workgroups of four waves fit a CU: a call with fewer tiles than that
-    // many splits its keys
-    const size_t fill = std::min<size_t>(2 * (size_t)std::max(device_cus(), 1), kKv4PartTiles);
+    // four workgroups of four waves fit a CU: a call that fills less than half of
+    // them splits its keys
+    const size_t fill = std::min<size_t>(4 * (size_t)std::max(device_cus(), 1), kKv4PartTiles);
     if (tiles * a.n_seqs * 2 <= fill) {
         const size_t slots = fill / tiles;
-        const size_t blocks = slots * tiles;
-        if (const mri_status st = grid_ok(blocks)) return st;
-        hipLaunchKernelGGL((k_kv4_attend<HD, true>), dim3((unsigned)blocks),
+        hipLaunchKernelGGL((k_kv4_attend<HD, true>), dim3((unsigned)(slots * tiles)),
                            dim3(kFewWaves * kWave), 0, s, a, q, qs, groups, (int)n_qt,
-                           (unsigned)slots, out, os, part, z);
-        MRI_LAUNCHED("k_kv4_attend");
-        hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)(a.n_seqs * tiles * 16)), dim3(HD), 0,
-                           s, a, groups, (int)n_qt, (unsigned)slots, part, out, os, z);
-        MRI_LAUNCHED("k_kv4_join");
+                           (unsigned)slots, out, os, part, cnts, z);
     } else {
         const size_t blocks = tiles * a.n_seqs;
         if (const mri_status st = grid_ok(blocks)) return st;
         hipLaunchKernelGGL((k_kv4_attend<HD, false>), dim3((unsigned)blocks),
                            dim3(kFewWaves * kWave), 0, s, a, q, qs, groups, (int)n_qt, 0u, out, os,
-                           part, z);
-        MRI_LAUNCHED("k_kv4_attend");
+                           part, cnts, z);
     }
+    MRI_LAUNCHED("k_kv4_attend");
     if (weights) {
         const size_t n_pg = a.pos ? a.n_pages : (a.start + (size_t)a.row0 + a.rows - 1) / kPageKeys + 1;
         const size_t blocks = n_pg * a.n_kv * a.n_seqs;
@@ -992,13 +1114,14 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
 
 mri_status launch_kv4_attend(const Kv4Rows &a, size_t hd, const float *q, size_t q_stride,
                              size_t n_heads, float *out, size_t out_stride, float *weights,
-                             float *part, float *lse, hipStream_t s) {
+                             float *part, int *cnts, float *lse, hipStream_t s) {
     if (!a.rows || !a.n_seqs || !n_heads) return MRI_OK;
     mri_status st = MRI_OK;
     auto go = [&](const Kv4Rows &c, const float *cq, float *co) {
         by_head(hd, [&](auto h) {
             constexpr int HD = decltype(h)::value;
-            st = attend_rows<HD>(c, cq, q_stride, n_heads, co, out_stride, weights, part, lse, s);
+            st = attend_rows<HD>(c, cq, q_stride, n_heads, co, out_stride, weights, part, cnts, lse,
+                                 s);
         });
     };
     if (!weights || (size_t)a.n_seqs * a.rows * n_heads <= kKv4LseFloats) {

@@ -45,8 +45,8 @@ struct Kv4Rows {
 };
 
 // Workspace of the attention, owned by the cache: partial results of split
-// rows and the rows' log-sum-exps.
-constexpr size_t kKv4PartTiles = 1536;   // 16-query tiles of partials
+// rows, a counter a split tile (zero between calls) and the rows' log-sum-exps.
+constexpr size_t kKv4PartTiles = 1024;   // 16-query tiles of partials, and counters
 constexpr size_t kKv4LseFloats = 1 << 20;
 inline size_t kv4_part_floats(size_t hd) { return kKv4PartTiles * 16 * (hd + 2); }
 
@@ -58,7 +58,7 @@ mri_status launch_kv4_read(const Kv4Rows &a, size_t hd, size_t n_layers, size_t 
 // weights (nullable): [sequence slots][n_kv][max_seq] of the layer.
 mri_status launch_kv4_attend(const Kv4Rows &a, size_t hd, const float *q, size_t q_stride,
                              size_t n_heads, float *out, size_t out_stride, float *weights,
-                             float *part, float *lse, hipStream_t s);
+                             float *part, int *cnts, float *lse, hipStream_t s);
 
 struct Kv4Evict {
     const uint8_t *src = nullptr;

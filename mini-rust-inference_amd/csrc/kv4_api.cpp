@@ -103,6 +103,8 @@ mri_status mri_kv4_cache_create(size_t n_layers, size_t n_seqs, size_t max_seq, 
     if ((e = hipMalloc(&c->pages, bytes)) || (e = hipMemset(c->pages, 0, bytes)) ||
         (e = hipMalloc(&c->part, part)) ||
         (e = hipMalloc(&c->lse, kKv4LseFloats * sizeof(float))) ||
+        (e = hipMalloc(&c->cnts, kKv4PartTiles * sizeof(int))) ||
+        (e = hipMemset(c->cnts, 0, kKv4PartTiles * sizeof(int))) ||
         (e = hipStreamSynchronize(nullptr))) {
         mri_kv4_cache_destroy(c);
         return hip_error(e, "kv4_cache_create");
@@ -114,7 +116,7 @@ mri_status mri_kv4_cache_create(size_t n_layers, size_t n_seqs, size_t max_seq, 
 size_t mri_kv4_cache_device_bytes(const mri_kv4_cache *c) {
     if (!c) return 0;
     return c->n_layers * c->layer_bytes() +
-           (kv4_part_floats(c->hd) + kKv4LseFloats) * sizeof(float);
+           (kv4_part_floats(c->hd) + kKv4LseFloats + kKv4PartTiles) * sizeof(float);
 }
 
 void mri_kv4_cache_destroy(mri_kv4_cache *c) {
@@ -122,6 +124,7 @@ void mri_kv4_cache_destroy(mri_kv4_cache *c) {
     if (c->pages) (void)hipFree(c->pages);
     if (c->part) (void)hipFree(c->part);
     if (c->lse) (void)hipFree(c->lse);
+    if (c->cnts) (void)hipFree(c->cnts);
     delete c;
 }
 
@@ -172,7 +175,7 @@ mri_status mri_kv4_attend(mri_kv4_cache *c, size_t layer, const mri_kv4_rows *ro
         return bad_arg("kv4_attend: unaligned rows");
     TRY(kv4_on_device(c));
     return launch_kv4_attend(a, c->hd, q, q_stride, n_heads, out, out_stride, weights, c->part,
-                             c->lse, static_cast<hipStream_t>(stream));
+                             c->cnts, c->lse, static_cast<hipStream_t>(stream));
 }
 
 mri_status mri_kv4_evict(const mri_kv4_cache *src, mri_kv4_cache *dst, const float *weights,

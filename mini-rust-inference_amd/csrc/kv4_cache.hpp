@@ -10,6 +10,7 @@ struct mri_kv4_cache {
     size_t n_layers = 0, n_seqs = 0, max_seq = 0, n_kv = 0, hd = 0, n_pages = 0;
     uint8_t *pages = nullptr;
     float *part = nullptr, *lse = nullptr;
+    int *cnts = nullptr;
     int device = 0;
     size_t layer_bytes() const { return n_seqs * n_kv * n_pages * mri::kv4_page_bytes(hd); }
 };

@@ -343,8 +343,8 @@ mri_status attend_kv4(mri_llama *m, size_t li, size_t rows, const KvTarget &kv, 
     TRY(kv4_rows(c, li, &r, &a));
     TRY(launch_kv4_append(a, c->hd, k, v, m->kvd, s));
     float *w = kv.weights ? kv.weights + li * c->n_seqs * c->n_kv * c->max_seq : nullptr;
-    return launch_kv4_attend(a, c->hd, q, qs, m->cfg.n_heads, m->attn, m->qd, w, c->part, c->lse,
-                             s);
+    return launch_kv4_attend(a, c->hd, q, qs, m->cfg.n_heads, m->attn, m->qd, w, c->part, c->cnts,
+                             c->lse, s);
 }
 
 // TransformerBlockInt8::forward_cached (forward_int8.rs:207-216): attention
