@@ -296,32 +296,78 @@ __device__ inline float col_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The query operand of a 16-column tile: column r of lane (g, r).
-template <int HD>
+// Sum and maximum over a column's blocks (FEW, below): lanes r + k * 16 / NB.
+template <int N>
+__device__ inline float ror(float v) {  // of lane r + N of the row of 16
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x120 + N, 0xf, 0xf,
+                                                       true));
+}
+template <int NB>
+__device__ inline float block_sum(float v) {
+    v = v + ror<8>(v);
+    if constexpr (NB == 4) v = v + ror<4>(v);
+    return v;
+}
+template <int NB>
+__device__ inline float block_max(float v) {
+    v = fmaxf(v, ror<8>(v));
+    if constexpr (NB == 4) v = fmaxf(v, ror<4>(v));
+    return v;
+}
+
+// A tile's columns are 16 queries; with FEW they are 16 / NB queries times the NB
+// blocks of the head dim, column b * 16 / NB + query.  Such a column holds its own
+// block of the query only, so the products with all of K's blocks leave its block's
+// dot; one scale a key multiplies it and the blocks' columns are added.  A column's
+// probabilities need the scales of its own block only, a quarter of the work at head
+// dim 128, and its sums count for that block's dims.
+template <int HD, bool FEW>
 struct QTile {
-    static constexpr int NB = HD / 32;
+    static constexpr int NB = HD / 32, NQ = FEW ? 16 / NB : 16;
     half8_t hi[NB], lo[NB];
     float inv;  // what the raw products are multiplied by (log2 units)
-    // src null: an empty column
-    __device__ void load(const float *src, int g) {
-        float x[NB][8];
+    // src null: an empty column; vec: 16-byte loads are aligned
+    __device__ void load(const float *src, int lane, bool vec) {
+        constexpr int N = FEW ? 1 : NB;
+        const int g = lane >> 4, own = (lane & 15) / NQ;
+        float x[N][8];
         float mx = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < N; ++b) {
+            const float *p = src + 32 * (FEW ? own : b) + 8 * g;
+            if (!src) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[b][j] = src ? src[32 * b + 8 * g + j] : 0.0f;
-                mx = fmaxf(mx, fabsf(x[b][j]));
+                for (int j = 0; j < 8; ++j) x[b][j] = 0.0f;
+            } else if (vec) {
+                *reinterpret_cast<float4 *>(x[b]) = *reinterpret_cast<const float4 *>(p);
+                *reinterpret_cast<float4 *>(x[b] + 4) = *reinterpret_cast<const float4 *>(p + 4);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[b][j] = p[j];
             }
+        }
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(x[b][j]));
         mx = col_max(mx);
+        if constexpr (FEW) mx = block_max<NB>(mx);
         // the row's largest magnitude to [2^14, 2^15)
         const int e = mx > 0.0f && mx < INFINITY ? min(14 - ilogbf(mx), 120) : 0;
         const float up = ldexpf(1.0f, e);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        for (int b = 0; b < N; ++b) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[b][j] = x[b][j] * up;
             split8(x[b], &hi[b], &lo[b]);
+        }
+        if constexpr (FEW) {
+            const half8_t h = hi[0], l = lo[0], z = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                hi[b] = b == own ? h : z;
+                lo[b] = b == own ? l : z;
+            }
         }
         // 2^9 log2(e) / sqrt(HD), rounded once
         constexpr float c = HD == 64 ? 0.18033688011112042592f : 0.12751743021347021697f;
@@ -330,10 +376,10 @@ struct QTile {
 };
 
 // A page on its way through a wave: every byte is loaded once, in whole lines,
-// before the first is used (a wave that loads as it goes touches its page's
-// lines up to sixteen times, and sixteen such waves a CU are more than its
-// caches hold: 138 us for 196 MB of pages).  The scales go on through LDS, from
-// where each lane group takes those of its keys.
+// while the page before it is computed (a wave that takes the scales where it
+// needs them touches its page's lines up to sixteen times, and the waves of a CU
+// are more than its caches hold: 138 us for 196 MB of pages).  The scales go on
+// through LDS, from where each lane group takes those of its keys.
 template <int HD>
 struct PageLoad {
     static constexpr int NB = HD / 32;
@@ -380,58 +426,83 @@ struct PageLoad {
 template <int HD>
 constexpr int kScaleWords = 64 * HD / 64;  // of the keys or the values of a page
 
-// A tile's raw scores (times q.inv: log2 units), of the keys 4 g + i of column r
-// in lane (g, r).  w: the K dwords; sp: the tile's staged scales of this lane
-// group, two dwords a block.
-template <int HD>
-__device__ inline float4_t score_tile(const unsigned *w, const unsigned *sp, const QTile<HD> &q) {
+// Raw scores (times q.inv: log2 units) of a page's 16 keys of tile t, for QT
+// query tiles: keys 4 g + i of column r in lane (g, r).  kw: the K dwords; s_ks:
+// the page's staged K scales, two dwords a block and four keys.
+template <int HD, int QT, bool FEW>
+__device__ inline void score_tile(const unsigned *kw, const unsigned *s_ks, int t, int lane,
+                                  const QTile<HD, FEW> *q, float4_t *s) {
     constexpr int NB = HD / 32;
-    unsigned d[2 * NB];
-#pragma unroll
-    for (int u = 0; u < NB / 2; ++u)
-        *reinterpret_cast<uint4 *>(d + 4 * u) = reinterpret_cast<const uint4 *>(sp)[u];
-    float4_t s = {0, 0, 0, 0};
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const half8_t kn = quants(w[b]);
+    const unsigned *sp = s_ks + (t * 4 + (lane >> 4)) * 2 * NB;
+    if constexpr (FEW) {
+        const uint2 d = reinterpret_cast<const uint2 *>(sp)[(lane & 15) / (16 / NB)];
+        const half2_t d01 = __builtin_bit_cast(half2_t, d.x),
+                      d23 = __builtin_bit_cast(half2_t, d.y);
         float4_t c = {0, 0, 0, 0};
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kn, q.lo[b], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kn, q.hi[b], c, 0, 0, 0);
-        const half2_t d01 = __builtin_bit_cast(half2_t, d[2 * b]),
-                      d23 = __builtin_bit_cast(half2_t, d[2 * b + 1]);
-        s[0] = fmaf(c[0], (float)d01.x, s[0]);
-        s[1] = fmaf(c[1], (float)d01.y, s[1]);
-        s[2] = fmaf(c[2], (float)d23.x, s[2]);
-        s[3] = fmaf(c[3], (float)d23.y, s[3]);
+        half8_t kq[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            kq[b] = quants(kw[b]);
+            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[b], q[0].lo[b], c, 0, 0, 0);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[b], q[0].hi[b], c, 0, 0, 0);
+        s[0][0] = block_sum<NB>(c[0] * (float)d01.x);
+        s[0][1] = block_sum<NB>(c[1] * (float)d01.y);
+        s[0][2] = block_sum<NB>(c[2] * (float)d23.x);
+        s[0][3] = block_sum<NB>(c[3] * (float)d23.y);
+    } else {
+        unsigned d[2 * NB];
+#pragma unroll
+        for (int u = 0; u < NB / 2; ++u)
+            *reinterpret_cast<uint4 *>(d + 4 * u) = reinterpret_cast<const uint4 *>(sp)[u];
+#pragma unroll
+        for (int k = 0; k < QT; ++k) s[k] = float4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const half8_t kq = quants(kw[b]);
+            const half2_t d01 = __builtin_bit_cast(half2_t, d[2 * b]),
+                          d23 = __builtin_bit_cast(half2_t, d[2 * b + 1]);
+#pragma unroll
+            for (int k = 0; k < QT; ++k) {
+                float4_t c = {0, 0, 0, 0};
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q[k].lo[b], c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q[k].hi[b], c, 0, 0, 0);
+                s[k][0] = fmaf(c[0], (float)d01.x, s[k][0]);
+                s[k][1] = fmaf(c[1], (float)d01.y, s[k][1]);
+                s[k][2] = fmaf(c[2], (float)d23.x, s[k][2]);
+                s[k][3] = fmaf(c[3], (float)d23.y, s[k][3]);
+            }
+        }
     }
-    return s;
 }
 
-// The running softmax of a wave's 16 columns.
-template <int HD>
+// The running softmax of a wave's columns.
+template <int HD, int QT>
 struct Softmax {
-    float m = -INFINITY;  // per column, log2 units
-    float l = 0.0f;       // of this lane's keys; l and o in units of 2^(ve - 14)
-    int ve = -100;        // 2^ve <= the largest d_v seen < 2^(ve + 1)
-    float4_t o[HD / 16];
+    float m[QT];    // per column, log2 units
+    float l[QT];    // of this lane's keys; l and o in units of 2^(ve - 14)
+    int ve = -100;  // 2^ve <= the largest d_v seen < 2^(ve + 1)
+    float4_t o[QT][HD / 16];
     __device__ Softmax() {
 #pragma unroll
-        for (int e = 0; e < HD / 16; ++e) o[e] = float4_t{0, 0, 0, 0};
-    }
-    __device__ void scale(float f) {
-        l = l * f;
+        for (int k = 0; k < QT; ++k) {
+            m[k] = -INFINITY;
+            l[k] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < HD / 16; ++e) o[e] = o[e] * f;
+            for (int e = 0; e < HD / 16; ++e) o[k][e] = float4_t{0, 0, 0, 0};
+        }
     }
 };
 
-// Adds one page.  WHOLE: every column sees its 64 keys; else keys [0, lim) of it
-// are seen by this lane's column (lim <= 0: none), the first n_keys by any.
+// Adds one page.  WHOLE: every column sees its 64 keys; else keys [0, lim[k]) of it
+// are seen by this lane's column of tile k (none if <= 0), the first n_keys by any.
 // s_ks, s_vs: its staged scales.
-template <int HD, bool WHOLE>
+template <int HD, int QT, bool FEW, bool WHOLE>
 __device__ inline void attend_page(const PageLoad<HD> &pl, const unsigned *s_ks,
-                                   const unsigned *s_vs, int lane, const QTile<HD> &q, int lim,
-                                   int n_keys, Softmax<HD> &st) {
+                                   const unsigned *s_vs, int lane, const QTile<HD, FEW> *q,
+                                   const int *lim, int n_keys, Softmax<HD, QT> &st) {
     constexpr int NB = HD / 32;
     const int g = lane >> 4;
     // the page's largest V scale; it seldom grows past the power of two in use
@@ -446,103 +517,158 @@ __device__ inline void attend_page(const PageLoad<HD> &pl, const unsigned *s_ks,
         }
         dmax = fmaxf(dmax, fmaxf((float)d.x, (float)d.y));
     }
-    float s[16];
+    float s[QT][16];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        const float4_t v = score_tile<HD>(pl.k[t], s_ks + (t * 4 + g) * 2 * NB, q);
+        float4_t v[QT];
+        score_tile<HD, QT, FEW>(pl.k[t], s_ks, t, lane, q, v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * t + i] = v[i];
-    }
-    if (!WHOLE) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int k = 0; k < QT; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (16 * t + 4 * g + i >= lim) s[4 * t + i] = -INFINITY;
+                s[k][4 * t + i] = WHOLE || 16 * t + 4 * g + i < lim[k] ? v[k][i] : -INFINITY;
     }
-    float pm = s[0];
+    float m_new[QT];
+    bool grows = dmax >= ldexpf(1.0f, st.ve + 1);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[i]);
-    const float m_new = fmaxf(st.m, col_max(pm) * q.inv);
-    if (__any(m_new > st.m || dmax >= ldexpf(1.0f, st.ve + 1))) {
+    for (int k = 0; k < QT; ++k) {
+        float pm = s[k][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[k][i]);
+        m_new[k] = fmaxf(st.m[k], col_max(pm) * q[k].inv);
+        grows = grows || m_new[k] > st.m[k];
+    }
+    if (__any(grows)) {
 #pragma unroll
         for (int x = 1; x < kWave; x <<= 1) dmax = fmaxf(dmax, __shfl_xor(dmax, x, kWave));
         const int ve = max(dmax > 0.0f ? ilogbf(dmax) : -24, st.ve);
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-        st.scale(ldexpf(__builtin_amdgcn_exp2f(st.m - m_use), st.ve - ve));
-        st.m = m_new;
+#pragma unroll
+        for (int k = 0; k < QT; ++k) {
+            const float m_use = m_new[k] == -INFINITY ? 0.0f : m_new[k];
+            const float f = ldexpf(__builtin_amdgcn_exp2f(st.m[k] - m_use), st.ve - ve);
+            st.l[k] = st.l[k] * f;
+#pragma unroll
+            for (int e = 0; e < HD / 16; ++e) st.o[k][e] = st.o[k][e] * f;
+            st.m[k] = m_new[k];
+        }
         st.ve = ve;
     }
     // p 2^(14 - ve)
-    const float m0 = (st.m == -INFINITY ? 0.0f : st.m) - (float)(14 - st.ve);
-    float p[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], q.inv, -m0));
-        st.l = st.l + p[i];
+    for (int k = 0; k < QT; ++k) {
+        const float m0 = (st.m[k] == -INFINITY ? 0.0f : st.m[k]) - (float)(14 - st.ve);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[k][i] = __builtin_amdgcn_exp2f(fmaf(s[k][i], q[k].inv, -m0));
+            st.l[k] = st.l[k] + s[k][i];
+        }
     }
+    // p d_v of the keys of half h under the scales d: two dwords a tile
+    auto weigh = [&](int k, int h, const unsigned (*d)[2], half8_t *hi, half8_t *lo)
+                     __attribute__((always_inline)) {
+        half2_t hh[4], ll[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {  // keys 16 t + 4 g + 2 (u % 2) + {0, 1}
+            const int t = 2 * h + (u >> 1), n = 4 * t + 2 * (u & 1);
+            half2_t x = __builtin_bit_cast(half2_t, d[u >> 1][u & 1]);
+            if (!WHOLE) {  // a key past the end may hold anything, NaN too
+                const int key = 16 * t + 4 * g + 2 * (u & 1);
+                if (key >= lim[k]) x.x = (_Float16)0.0f;
+                if (key + 1 >= lim[k]) x.y = (_Float16)0.0f;
+            }
+            split2(fmaf(s[k][n], (float)x.x, 0.0f), fmaf(s[k][n + 1], (float)x.y, 0.0f), &hh[u],
+                   &ll[u]);
+        }
+        *hi = join(hh[0], hh[1], hh[2], hh[3]);
+        *lo = join(ll[0], ll[1], ll[2], ll[3]);
+    };
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        half8_t ph[NB], pl8[NB];
-        unsigned dv[2][2 * NB];  // the scales of tiles 2 h and 2 h + 1
+        if constexpr (FEW) {
+            unsigned d[2][2];
 #pragma unroll
-        for (int u = 0; u < NB; ++u)
-            *reinterpret_cast<uint4 *>(&dv[u / (NB / 2)][u % (NB / 2) * 4]) =
-                reinterpret_cast<const uint4 *>(s_vs + ((2 * h + u / (NB / 2)) * 4 + g) * 2 * NB)
-                    [u % (NB / 2)];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            half2_t hh[4], ll[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {  // keys 16 t + 4 g + 2 (u % 2) + {0, 1}
-                const int t = 2 * h + (u >> 1), n = 4 * t + 2 * (u & 1);
-                half2_t d = __builtin_bit_cast(half2_t, dv[u >> 1][2 * b + (u & 1)]);
-                if (!WHOLE) {  // a key past the end may hold anything, NaN too
-                    const int key = 16 * t + 4 * g + 2 * (u & 1);
-                    if (key >= lim) d.x = (_Float16)0.0f;
-                    if (key + 1 >= lim) d.y = (_Float16)0.0f;
-                }
-                split2(fmaf(p[n], (float)d.x, 0.0f), fmaf(p[n + 1], (float)d.y, 0.0f), &hh[u],
-                       &ll[u]);
+            for (int u = 0; u < 2; ++u) {
+                const uint2 x = reinterpret_cast<const uint2 *>(
+                    s_vs + ((2 * h + u) * 4 + g) * 2 * NB)[(lane & 15) / (16 / NB)];
+                d[u][0] = x.x, d[u][1] = x.y;
             }
-            ph[b] = join(hh[0], hh[1], hh[2], hh[3]);
-            pl8[b] = join(ll[0], ll[1], ll[2], ll[3]);
-        }
+            half8_t hi, lo;
+            weigh(0, h, d, &hi, &lo);
 #pragma unroll
-        for (int e = 0; e < HD / 16; ++e) {
-            const half8_t vq = quants(pl.v[e][h]);
-            st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, pl8[e >> 1], st.o[e], 0, 0, 0);
-            st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, ph[e >> 1], st.o[e], 0, 0, 0);
+            for (int e = 0; e < HD / 16; ++e) {
+                const half8_t vq = quants(pl.v[e][h]);
+                st.o[0][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, lo, st.o[0][e], 0, 0, 0);
+                st.o[0][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, hi, st.o[0][e], 0, 0, 0);
+            }
+        } else {
+            unsigned dv[2][2 * NB];  // the scales of tiles 2 h and 2 h + 1
+#pragma unroll
+            for (int u = 0; u < NB; ++u)
+                *reinterpret_cast<uint4 *>(&dv[u / (NB / 2)][u % (NB / 2) * 4]) =
+                    reinterpret_cast<const uint4 *>(
+                        s_vs + ((2 * h + u / (NB / 2)) * 4 + g) * 2 * NB)[u % (NB / 2)];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const unsigned d[2][2] = {{dv[0][2 * b], dv[0][2 * b + 1]},
+                                          {dv[1][2 * b], dv[1][2 * b + 1]}};
+                half8_t hi[QT], lo[QT];
+#pragma unroll
+                for (int k = 0; k < QT; ++k) weigh(k, h, d, &hi[k], &lo[k]);
+#pragma unroll
+                for (int e = 2 * b; e < 2 * b + 2; ++e) {
+                    const half8_t vq = quants(pl.v[e][h]);
+#pragma unroll
+                    for (int k = 0; k < QT; ++k) {
+                        float4_t o = st.o[k][e];
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, lo[k], o, 0, 0, 0);
+                        st.o[k][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, hi[k], o, 0, 0, 0);
+                    }
+                }
+            }
         }
     }
 }
 
 // How the pages of a call's sequences are dealt to at most `slots` runs (slots
-// >= 2 n_seqs) of at most `chunk` pages: sequence b takes ceil(pages_b / chunk)
-// of them, in order.  chunk = ceil(total / slots) where the sequences' last, short
-// runs leave room for that, else ceil(total / (slots - n_seqs)), which always
-// suffices.  Every wave computes the same, a sequence a lane.
-constexpr unsigned kMinChunk = 4;
+// >= 2 n_seqs) of at most `chunk` pages, chunk the least that suffices: sequence b
+// takes ceil(pages_b / chunk) runs, in order.  Every wave computes the same, a
+// sequence a lane.  A run has at least min_chunk pages.
 __device__ inline unsigned seq_pages(const Kv4Rows &a, int b) {
     unsigned p0;
     const unsigned cnt = rows_of(a, b, &p0);
     return cnt ? (p0 + cnt + kPageKeys - 1) / kPageKeys : 0;
 }
-__device__ inline unsigned wave_sum_u(unsigned v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+// Inclusive sums over the lanes.
+__device__ inline unsigned wave_scan_u(unsigned v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0's last to row 1, 2's to 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row 1's last to rows 2, 3
     return v;
+}
+__device__ inline unsigned wave_sum_u(unsigned v) {
+    return __builtin_amdgcn_readlane(wave_scan_u(v), kWave - 1);
+}
+// ceil(n / d) of n, d < 2^24: the f32 quotient is off by less than one.
+__device__ inline unsigned ceil_div(unsigned n, unsigned d, float inv) {
+    unsigned q = (unsigned)((float)n * inv);
+    q -= q * d > n;
+    q += (q + 1) * d <= n;
+    return q + (q * d < n);
 }
 struct Run {
     int b;                // the sequence, -1: no such run
     unsigned first, n;    // its runs
     unsigned pg0, pg1;    // the run's pages
 };
-__device__ inline Run find_run(const Kv4Rows &a, unsigned slots, unsigned slot) {
+__device__ inline Run find_run(const Kv4Rows &a, unsigned slots, unsigned slot,
+                               unsigned min_chunk) {
     const int lane = threadIdx.x & 63;
     const unsigned n_seqs = a.n_seqs;
     if (n_seqs == 1) {
-        const unsigned np = seq_pages(a, 0), chunk = max((np + slots - 1) / slots, kMinChunk);
+        const unsigned np = seq_pages(a, 0), chunk = max((np + slots - 1) / slots, min_chunk);
         const unsigned n = (np + chunk - 1) / chunk;
         return Run{slot < n ? 0 : -1, 0, n, slot * chunk, min(slot * chunk + chunk, np)};
     }
@@ -550,96 +676,114 @@ __device__ inline Run find_run(const Kv4Rows &a, unsigned slots, unsigned slot) 
     unsigned total = mine;
     for (unsigned b = lane + kWave; b < n_seqs; b += kWave) total += seq_pages(a, b);
     total = wave_sum_u(total);
-    unsigned chunk = max((total + slots - 1) / slots, kMinChunk);
-    unsigned runs = (mine + chunk - 1) / chunk;
-    for (unsigned b = lane + kWave; b < n_seqs; b += kWave)
-        runs += (seq_pages(a, b) + chunk - 1) / chunk;
-    if (wave_sum_u(runs) > slots)
-        chunk = max((total + slots - n_seqs - 1) / (slots - n_seqs), kMinChunk);
+    // ceil(total / slots) is too few pages, or just enough; ceil(total / (slots -
+    // n_seqs)) suffices, for each sequence has one short run at most
+    unsigned lo = max((total + slots - 1) / slots, min_chunk);
+    unsigned hi = max((total + slots - n_seqs - 1) / (slots - n_seqs), min_chunk);
+    while (lo < hi) {
+        const unsigned mid = (lo + hi) >> 1;
+        const float inv = 1.0f / (float)mid;
+        unsigned runs = ceil_div(mine, mid, inv);
+        for (unsigned b = lane + kWave; b < n_seqs; b += kWave)
+            runs += ceil_div(seq_pages(a, b), mid, inv);
+        if (wave_sum_u(runs) <= slots) hi = mid;
+        else lo = mid + 1;
+    }
+    const float inv = 1.0f / (float)lo;
     unsigned before = 0;
     for (unsigned b0 = 0; b0 < n_seqs; b0 += kWave) {
         const unsigned np = b0 == 0 ? mine : b0 + lane < n_seqs ? seq_pages(a, b0 + lane) : 0;
-        const unsigned n = (np + chunk - 1) / chunk;
-        unsigned inc = n;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const unsigned y = __shfl_up(inc, o, kWave);
-            if (lane >= o) inc += y;
-        }
+        const unsigned n = ceil_div(np, lo, inv), inc = wave_scan_u(n);
         const unsigned long long over = __ballot(before + inc > slot);
         if (over) {
             const int l = __ffsll((long long)over) - 1;
             Run r;
             r.b = (int)b0 + l;
-            r.n = __shfl(n, l, kWave);
-            r.first = before + __shfl(inc, l, kWave) - r.n;
-            r.pg0 = (slot - r.first) * chunk;
-            r.pg1 = min(r.pg0 + chunk, (unsigned)__shfl(np, l, kWave));
+            r.n = __builtin_amdgcn_readlane(n, l);
+            r.first = before + __builtin_amdgcn_readlane(inc, l) - r.n;
+            r.pg0 = (slot - r.first) * lo;
+            r.pg1 = min(r.pg0 + lo, (unsigned)__builtin_amdgcn_readlane(np, l));
             return r;
         }
-        before += __shfl(inc, kWave - 1, kWave);
+        before += __builtin_amdgcn_readlane(inc, kWave - 1);
     }
     return Run{-1, 0, 0, 0, 0};
 }
 
-__device__ inline void part_store(float *p, float v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Partial results go through the memory that all XCDs see, two floats an access.
+__device__ inline void part_store(float *p, float a, float b) {
+    const unsigned long long v =
+        (unsigned long long)__float_as_uint(b) << 32 | __float_as_uint(a);
+    __hip_atomic_store(reinterpret_cast<unsigned long long *>(p), v, __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ inline float part_load(const float *p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ inline float2 part_load(const float *p) {
+    const unsigned long long v =
+        __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p), __ATOMIC_RELAXED,
+                          __HIP_MEMORY_SCOPE_AGENT);
+    return float2{__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))};
 }
 
-constexpr int kFewWaves = 4;
+// Waves of a workgroup, and workgroups of a CU where keys are split (registers
+// leave two waves a SIMD at head dim 128, three at 64).
+constexpr int waves_of(int hd, bool split) { return split && hd == 128 ? 8 : 4; }
+constexpr int wgs_of(int hd) { return hd == 128 ? 1 : 3; }
 
 // Grid: slots x (KV heads x query tiles).  SPLIT: a slot is a run of pages of
-// one sequence; else it is a sequence.  The four waves take every fourth page
-// and meet in LDS.  Where a sequence has several runs, each publishes its columns'
+// one sequence; else it is a sequence.  The waves take its pages in turn and meet
+// in LDS.  Where a sequence has several runs, each publishes its columns'
 // (m, l, o) in `part` by device-scope stores that are complete before it counts
 // itself on the tile's counter; the one that counts last joins them in the order
 // of the runs and leaves the counter zero, so none waits for another.
-template <int HD, bool SPLIT>
-__global__ __launch_bounds__(kFewWaves *kWave) void k_kv4_attend(
-    Kv4Rows a, const float *__restrict__ q, size_t qs, int groups, int n_qt, unsigned slots,
-    float *__restrict__ out, size_t os, float *__restrict__ part, int *__restrict__ cnts,
-    float *__restrict__ lse) {
+template <int HD, int QT, bool FEW, bool SPLIT>
+__global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
+    Kv4Rows a, const float *__restrict__ q, size_t qs, bool vec, int groups, int n_qt,
+    unsigned slots, float *__restrict__ out, size_t os, float *__restrict__ part,
+    int *__restrict__ cnts, float *__restrict__ lse) {
     using P = Page<HD>;
-    __shared__ float s_m[kFewWaves][16], s_l[kFewWaves][16];
-    __shared__ __attribute__((aligned(16))) float s_o[kFewWaves][16][HD + 4];
-    __shared__ __attribute__((aligned(16))) unsigned s_d[kFewWaves][2][kScaleWords<HD>];
+    constexpr int NQ = QTile<HD, FEW>::NQ, TW = QT * NQ;  // queries of a tile
+    constexpr int kWaves = waves_of(HD, SPLIT);
+    __shared__ float s_m[kWaves][TW], s_l[kWaves][TW];
+    __shared__ __attribute__((aligned(16))) float s_o[kWaves][TW][HD + 4];
+    __shared__ __attribute__((aligned(16))) unsigned s_d[kWaves][2][kScaleWords<HD>];
     __shared__ int s_last;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
     const int qt = blockIdx.x % n_qt, head = blockIdx.x / n_qt % a.n_kv;
     const unsigned slot = blockIdx.x / (n_qt * a.n_kv);
     Run run{(int)slot, 0, 1, 0, 0};
     if constexpr (SPLIT) {
-        run = find_run(a, slots, slot);
+        // two pages a wave cost less than another workgroup's partial results
+        run = find_run(a, slots, slot, 2 * kWaves);
         if (run.b < 0) return;
     }
     const int b = run.b;
     unsigned p0;
     const int cnt = (int)rows_of(a, b, &p0);
     const int n_q = cnt * groups;       // real queries of the KV head
-    if (qt * 16 >= n_q) return;
-    const int last_row = (min(qt * 16 + 16, n_q) - 1) / groups;
+    if (qt * TW >= n_q) return;
+    const int last_row = (min(qt * TW + TW, n_q) - 1) / groups;
     const unsigned end = p0 + last_row + 1;  // keys that the tile's last row sees
     const unsigned end_pg = (end + kPageKeys - 1) / kPageKeys;
     const unsigned pg1 = SPLIT ? min(run.pg1, end_pg) : end_pg;
-    const int qi = qt * 16 + r, row = qi / groups;
-    const bool real = qi < n_q;
-    const size_t qrow = row_index(a, b, row);
-    const int qh = head * groups + qi % groups;
-    QTile<HD> qtile;
-    qtile.load(real ? q + qrow * qs + qh * HD : nullptr, g);
-    const long see = real ? (long)p0 + row + 1 : 0;          // keys this column sees
-    const unsigned all = p0 + (qt * 16) / groups + 1;        // keys every real column sees
-    Softmax<HD> st;
+    // a page's loads are in flight while the one before it is computed
     const uint8_t *base =
         a.pages + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages * P::kBytes;
-    // a page's loads are in flight while the one before it is computed
     PageLoad<HD> next;
     unsigned pg = run.pg0 + wv;
     if (pg < pg1) next.load(base + (size_t)pg * P::kBytes, lane);
-    for (; pg < pg1; pg += kFewWaves) {
+    QTile<HD, FEW> qtile[QT];
+    long see[QT];  // keys this column sees
+#pragma unroll
+    for (int k = 0; k < QT; ++k) {
+        const int qi = qt * TW + k * NQ + r % NQ, row = qi / groups;
+        const bool real = qi < n_q;
+        const int qh = head * groups + qi % groups;
+        qtile[k].load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, lane, vec);
+        see[k] = real ? (long)p0 + row + 1 : 0;
+    }
+    const unsigned all = p0 + (qt * TW) / groups + 1;        // keys every real column sees
+    Softmax<HD, QT> st;
+    for (; pg < pg1; pg += kWaves) {
         const PageLoad<HD> now = next;
         __builtin_amdgcn_wave_barrier();  // the last page's scales are read (LDS is in order)
         PageLoad<HD>::stage(now.ks, lane, s_d[wv][0]);
@@ -647,63 +791,72 @@ __global__ __launch_bounds__(kFewWaves *kWave) void k_kv4_attend(
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (pg + kFewWaves < pg1) next.load(base + (size_t)(pg + kFewWaves) * P::kBytes, lane);
-        const bool whole = (pg + 1) * kPageKeys <= all;
-        const long lim = see - (long)pg * kPageKeys;
-        if (whole)
-            attend_page<HD, true>(now, s_d[wv][0], s_d[wv][1], lane, qtile, 64, 64, st);
+        if (pg + kWaves < pg1) next.load(base + (size_t)(pg + kWaves) * P::kBytes, lane);
+        int lim[QT];
+#pragma unroll
+        for (int k = 0; k < QT; ++k) lim[k] = (int)min(see[k] - (long)pg * kPageKeys, 64l);
+        if ((pg + 1) * kPageKeys <= all)
+            attend_page<HD, QT, FEW, true>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim, 64, st);
         else
-            attend_page<HD, false>(now, s_d[wv][0], s_d[wv][1], lane, qtile, (int)min(lim, 64l),
-                                   (int)min(end - pg * kPageKeys, 64u), st);
+            attend_page<HD, QT, FEW, false>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim,
+                                            (int)min(end - pg * kPageKeys, 64u), st);
     }
     // o holds 2^-9 of the quants; l and o back to their own units, the
     // column's sum over its four lane groups, then the waves
     const float down = ldexpf(1.0f, st.ve - 14);
-    st.l = col_sum(st.l) * down;
-    if (g == 0) {
-        s_m[wv][r] = st.m;
-        s_l[wv][r] = st.l;
-    }
 #pragma unroll
-    for (int e = 0; e < HD / 16; ++e)
-        *reinterpret_cast<float4_t *>(&s_o[wv][r][16 * e + 4 * g]) =
-            st.o[e] * (down * 0x1p9f);
+    for (int k = 0; k < QT; ++k) {
+        const float l = col_sum(st.l[k]) * down;
+        const int c = k * NQ + r % NQ;
+        if (g == 0 && r < NQ) {
+            s_m[wv][c] = st.m[k];
+            s_l[wv][c] = l;
+        }
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e)
+            if (!FEW || e / 2 == r / NQ)
+                *reinterpret_cast<float4_t *>(&s_o[wv][c][16 * e + 4 * g]) =
+                    st.o[k][e] * (down * 0x1p9f);
+    }
     __syncthreads();
-    const int cols = min(16, n_q - qt * 16);
+    const int cols = min(TW, n_q - qt * TW);
     const size_t z0 = ((size_t)b * a.rows) * (a.n_kv * groups);
-    auto store = [&](int c, int d, float m, float l, float o) {
-        const int ci = qt * 16 + c, oh = head * groups + ci % groups;
-        out[row_index(a, b, ci / groups) * os + oh * HD + d] = o / l;
+    // four dims of a column from d on
+    auto store = [&](int c, int d, float m, float l, const float *o) {
+        const int ci = qt * TW + c, oh = head * groups + ci % groups;
+        float *to = out + row_index(a, b, ci / groups) * os + oh * HD + d;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[j] = o[j] / l;
         if (lse && d == 0)
             lse[z0 + (size_t)(ci / groups) * (a.n_kv * groups) + oh] = m + __log2f(l);
     };
     const bool alone = !SPLIT || run.n == 1;
     // partial results of run i, column c
     auto part_of = [&](unsigned i, int c) {
-        return part + ((((size_t)(run.first + i) * a.n_kv + head) * n_qt + qt) * 16 + c) * (HD + 2);
+        return part + ((((size_t)(run.first + i) * a.n_kv + head) * n_qt + qt) * TW + c) * (HD + 2);
     };
-    for (int it = threadIdx.x; it < cols * HD; it += kFewWaves * kWave) {
-        const int c = it / HD, d = it % HD;
+    for (int it = threadIdx.x; it < cols * (HD / 4); it += kWaves * kWave) {
+        const int c = it / (HD / 4), d = it % (HD / 4) * 4;
         float m = s_m[0][c];
 #pragma unroll
-        for (int w = 1; w < kFewWaves; ++w) m = fmaxf(m, s_m[w][c]);
+        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][c]);
         const float m_use = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, o = 0.0f;
+        float l = 0.0f, o[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < kFewWaves; ++w) {
+        for (int w = 0; w < kWaves; ++w) {
             const float f = __builtin_amdgcn_exp2f(s_m[w][c] - m_use);
+            const float4_t x = *reinterpret_cast<const float4_t *>(&s_o[w][c][d]);
             l = l + s_l[w][c] * f;
-            o = o + s_o[w][c][d] * f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = o[j] + x[j] * f;
         }
         if (alone) {
             store(c, d, m_use, l, o);
         } else {
             float *pc = part_of(slot - run.first, c);
-            part_store(pc + 2 + d, o);
-            if (d == 0) {
-                part_store(pc, m);
-                part_store(pc + 1, l);
-            }
+            part_store(pc + 2 + d, o[0], o[1]);
+            part_store(pc + 4 + d, o[2], o[3]);
+            if (d == 0) part_store(pc, m, l);
         }
     }
     if (alone) return;
@@ -716,32 +869,36 @@ __global__ __launch_bounds__(kFewWaves *kWave) void k_kv4_attend(
     __syncthreads();
     if (!s_last) return;
     if (threadIdx.x == 0) __hip_atomic_store(cn, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int it = threadIdx.x; it < cols * HD; it += kFewWaves * kWave) {
-        const int c = it / HD, d = it % HD;
+    for (int it = threadIdx.x; it < cols * (HD / 4); it += kWaves * kWave) {
+        const int c = it / (HD / 4), d = it % (HD / 4) * 4;
         constexpr unsigned B = 8;
-        float m = -INFINITY, l = 0.0f, o = 0.0f;
+        float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
         for (unsigned i0 = 0; i0 < run.n; i0 += B) {  // B runs' loads in flight
-            float pm[B], pl[B], po[B];
+            float2 ml[B], x[B][2];
 #pragma unroll
             for (unsigned u = 0; u < B; ++u) {
                 const float *pc = part_of(min(i0 + u, run.n - 1), c);
-                pm[u] = part_load(pc);
-                pl[u] = part_load(pc + 1);
-                po[u] = part_load(pc + 2 + d);
+                ml[u] = part_load(pc);
+                x[u][0] = part_load(pc + 2 + d);
+                x[u][1] = part_load(pc + 4 + d);
             }
             float mn = m;
 #pragma unroll
-            for (unsigned u = 0; u < B; ++u) mn = fmaxf(mn, pm[u]);
+            for (unsigned u = 0; u < B; ++u) mn = fmaxf(mn, ml[u].x);
             const float m_use = mn == -INFINITY ? 0.0f : mn, f0 = __builtin_amdgcn_exp2f(m - m_use);
             l = l * f0;
-            o = o * f0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = o[j] * f0;
             m = mn;
 #pragma unroll
             for (unsigned u = 0; u < B; ++u) {
                 if (i0 + u < run.n) {
-                    const float f = __builtin_amdgcn_exp2f(pm[u] - m_use);
-                    l = l + pl[u] * f;
-                    o = o + po[u] * f;
+                    const float f = __builtin_amdgcn_exp2f(ml[u].x - m_use);
+                    l = l + ml[u].y * f;
+                    o[0] = o[0] + x[u][0].x * f;
+                    o[1] = o[1] + x[u][0].y * f;
+                    o[2] = o[2] + x[u][1].x * f;
+                    o[3] = o[3] + x[u][1].y * f;
                 }
             }
         }
@@ -754,7 +911,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void k_kv4_attend(
 // rows' log-sum-exps, so each key has one writer and one order of sums.
 template <int HD>
 __global__ __launch_bounds__(kWave) void k_kv4_weights(Kv4Rows a, const float *__restrict__ q,
-                                                       size_t qs, int groups, int n_pages,
+                                                       size_t qs, bool vec, int groups, int n_pages,
                                                        const float *__restrict__ lse,
                                                        float *__restrict__ weights) {
     using P = Page<HD>;
@@ -784,14 +941,14 @@ __global__ __launch_bounds__(kWave) void k_kv4_weights(Kv4Rows a, const float *_
         const bool real = qi < n_q;
         const size_t qrow = row_index(a, b, row);
         const int qh = head * groups + qi % groups;
-        QTile<HD> qtile;
-        qtile.load(real ? q + qrow * qs + qh * HD : nullptr, g);
+        QTile<HD, false> qtile;
+        qtile.load(real ? q + qrow * qs + qh * HD : nullptr, lane, vec);
         const float z = real ? lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] : 0.0f;
         const long lim = real ? (long)p0 + row + 1 - (long)key0 : 0;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const float4_t s =
-                score_tile<HD>(page.k[t], s_d + (t * 4 + g) * 2 * P::NB, qtile);
+            float4_t s;
+            score_tile<HD, 1, false>(page.k[t], s_d, t, lane, &qtile, &s);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (16 * t + 4 * g + i < lim)
@@ -1080,31 +1237,44 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
                        size_t os, float *weights, float *part, int *cnts, float *lse,
                        hipStream_t s) {
     const int groups = (int)(n_heads / a.n_kv);
-    const size_t n_qt = ((size_t)a.rows * groups + 15) / 16;
-    const size_t tiles = n_qt * a.n_kv;
+    const size_t n_q = (size_t)a.rows * groups;
+    const bool vec = qs % 4 == 0 && al16(q);
     float *z = weights ? lse : nullptr;
-    // four workgroups of four waves fit a CU: a call that fills less than half of
-    // them splits its keys
-    const size_t fill = std::min<size_t>(4 * (size_t)std::max(device_cus(), 1), kKv4PartTiles);
-    if (tiles * a.n_seqs * 2 <= fill) {
-        const size_t slots = fill / tiles;
-        hipLaunchKernelGGL((k_kv4_attend<HD, true>), dim3((unsigned)(slots * tiles)),
-                           dim3(kFewWaves * kWave), 0, s, a, q, qs, groups, (int)n_qt,
-                           (unsigned)slots, out, os, part, cnts, z);
-    } else {
-        const size_t blocks = tiles * a.n_seqs;
-        if (const mri_status st = grid_ok(blocks)) return st;
-        hipLaunchKernelGGL((k_kv4_attend<HD, false>), dim3((unsigned)blocks),
-                           dim3(kFewWaves * kWave), 0, s, a, q, qs, groups, (int)n_qt, 0u, out, os,
-                           part, cnts, z);
-    }
-    MRI_LAUNCHED("k_kv4_attend");
+    auto go = [&](auto qt_, auto few_) -> mri_status {
+        constexpr int QT = decltype(qt_)::value;
+        constexpr bool FEW = decltype(few_)::value;
+        constexpr int TW = QT * QTile<HD, FEW>::NQ;
+        const size_t n_qt = (n_q + TW - 1) / TW, tiles = n_qt * a.n_kv;
+        // a call with tiles for less than half of the CUs splits its keys
+        const size_t fill =
+            std::min<size_t>(wgs_of(HD) * (size_t)std::max(device_cus(), 1), kKv4PartTiles / QT);
+        if (tiles * a.n_seqs * 2 <= fill) {
+            const size_t slots = fill / tiles;
+            hipLaunchKernelGGL((k_kv4_attend<HD, QT, FEW, true>), dim3((unsigned)(slots * tiles)),
+                               dim3(waves_of(HD, true) * kWave), 0, s, a, q, qs, vec, groups, (int)n_qt,
+                               (unsigned)slots, out, os, part, cnts, z);
+        } else {
+            const size_t blocks = tiles * a.n_seqs;
+            if (const mri_status st = grid_ok(blocks)) return st;
+            hipLaunchKernelGGL((k_kv4_attend<HD, QT, FEW, false>), dim3((unsigned)blocks),
+                               dim3(waves_of(HD, false) * kWave), 0, s, a, q, qs, vec, groups, (int)n_qt, 0u, out, os, part, cnts, z);
+        }
+        MRI_LAUNCHED("k_kv4_attend");
+        return MRI_OK;
+    };
+    using T = std::true_type;
+    using F = std::false_type;
+    mri_status st;
+    if (n_q <= QTile<HD, true>::NQ) st = go(std::integral_constant<int, 1>{}, T{});
+    else if (n_q <= 16) st = go(std::integral_constant<int, 1>{}, F{});
+    else st = go(std::integral_constant<int, 1>{}, F{});
+    if (st) return st;
     if (weights) {
         const size_t n_pg = a.pos ? a.n_pages : (a.start + (size_t)a.row0 + a.rows - 1) / kPageKeys + 1;
         const size_t blocks = n_pg * a.n_kv * a.n_seqs;
         if (const mri_status st = grid_ok(blocks)) return st;
         hipLaunchKernelGGL((k_kv4_weights<HD>), dim3((unsigned)blocks), dim3(kWave), 0, s, a, q,
-                           qs, groups, (int)n_pg, lse, weights);
+                           qs, vec, groups, (int)n_pg, lse, weights);
         MRI_LAUNCHED("k_kv4_weights");
     }
     return MRI_OK;
