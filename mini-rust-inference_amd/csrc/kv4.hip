@@ -321,17 +321,15 @@ __device__ inline float block_max(float v) {
 // dot; one scale a key multiplies it and the blocks' columns are added.  A column's
 // probabilities need the scales of its own block only, a quarter of the work at head
 // dim 128, and its sums count for that block's dims.
+//
+// What lane (g, r) loads of a tile: dims 8 g .. of the blocks of column r.
 template <int HD, bool FEW>
-struct QTile {
-    static constexpr int NB = HD / 32, NQ = FEW ? 16 / NB : 16;
-    half8_t hi[NB], lo[NB];
-    float inv;  // what the raw products are multiplied by (log2 units)
+struct QRaw {
+    static constexpr int NB = HD / 32, NQ = FEW ? 16 / NB : 16, N = FEW ? 1 : NB;
+    float x[N][8];
     // src null: an empty column; vec: 16-byte loads are aligned
     __device__ void load(const float *src, int lane, bool vec) {
-        constexpr int N = FEW ? 1 : NB;
         const int g = lane >> 4, own = (lane & 15) / NQ;
-        float x[N][8];
-        float mx = 0.0f;
 #pragma unroll
         for (int b = 0; b < N; ++b) {
             const float *p = src + 32 * (FEW ? own : b) + 8 * g;
@@ -346,10 +344,20 @@ struct QTile {
                 for (int j = 0; j < 8; ++j) x[b][j] = p[j];
             }
         }
+    }
+};
+template <int HD, bool FEW>
+struct QTile {
+    using R = QRaw<HD, FEW>;
+    static constexpr int NB = HD / 32, NQ = R::NQ, N = R::N;
+    half8_t hi[NB], lo[NB];
+    float inv;  // what the raw products are multiplied by (log2 units)
+    __device__ void make(const R &raw, int lane) {
+        float mx = 0.0f;
 #pragma unroll
         for (int b = 0; b < N; ++b)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(x[b][j]));
+            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(raw.x[b][j]));
         mx = col_max(mx);
         if constexpr (FEW) mx = block_max<NB>(mx);
         // the row's largest magnitude to [2^14, 2^15)
@@ -357,11 +365,13 @@ struct QTile {
         const float up = ldexpf(1.0f, e);
 #pragma unroll
         for (int b = 0; b < N; ++b) {
+            float x[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[b][j] = x[b][j] * up;
-            split8(x[b], &hi[b], &lo[b]);
+            for (int j = 0; j < 8; ++j) x[j] = raw.x[b][j] * up;
+            split8(x, &hi[b], &lo[b]);
         }
         if constexpr (FEW) {
+            const int own = (lane & 15) / NQ;
             const half8_t h = hi[0], l = lo[0], z = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -422,94 +432,86 @@ struct PageLoad {
 #pragma unroll
         for (int u = 0; u < NB / 2; ++u) lds[lane * (NB / 2) + u] = d[u];
     }
+    // the operands of a key tile's block and of a dim tile's key half
+    __device__ half8_t kop(int t, int b) const { return quants(k[t][b]); }
+    __device__ half8_t vop(int e, int h) const { return quants(v[e][h]); }
+    __device__ unsigned vscale(int u) const { return vs[u]; }
 };
 template <int HD>
 constexpr int kScaleWords = 64 * HD / 64;  // of the keys or the values of a page
 
-// Raw scores (times q.inv: log2 units) of a page's 16 keys of tile t, for QT
-// query tiles: keys 4 g + i of column r in lane (g, r).  kw: the K dwords; s_ks:
-// the page's staged K scales, two dwords a block and four keys.
-template <int HD, int QT, bool FEW>
-__device__ inline void score_tile(const unsigned *kw, const unsigned *s_ks, int t, int lane,
-                                  const QTile<HD, FEW> *q, float4_t *s) {
+// Raw scores (times q.inv: log2 units) of a page's 16 keys of tile t: keys 4 g + i
+// of column r in lane (g, r).  s_ks: the page's staged K scales, two dwords a block
+// and four keys.
+template <int HD, bool FEW, class Src>
+__device__ inline float4_t score_tile(const Src &pl, const unsigned *s_ks, int t, int lane,
+                                      const QTile<HD, FEW> &q) {
     constexpr int NB = HD / 32;
     const unsigned *sp = s_ks + (t * 4 + (lane >> 4)) * 2 * NB;
+    float4_t s = {0, 0, 0, 0};
     if constexpr (FEW) {
         const uint2 d = reinterpret_cast<const uint2 *>(sp)[(lane & 15) / (16 / NB)];
         const half2_t d01 = __builtin_bit_cast(half2_t, d.x),
                       d23 = __builtin_bit_cast(half2_t, d.y);
-        float4_t c = {0, 0, 0, 0};
         half8_t kq[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            kq[b] = quants(kw[b]);
-            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[b], q[0].lo[b], c, 0, 0, 0);
+            kq[b] = pl.kop(t, b);
+            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[b], q.lo[b], s, 0, 0, 0);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b)
-            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[b], q[0].hi[b], c, 0, 0, 0);
-        s[0][0] = block_sum<NB>(c[0] * (float)d01.x);
-        s[0][1] = block_sum<NB>(c[1] * (float)d01.y);
-        s[0][2] = block_sum<NB>(c[2] * (float)d23.x);
-        s[0][3] = block_sum<NB>(c[3] * (float)d23.y);
-    } else {
-        unsigned d[2 * NB];
-#pragma unroll
-        for (int u = 0; u < NB / 2; ++u)
-            *reinterpret_cast<uint4 *>(d + 4 * u) = reinterpret_cast<const uint4 *>(sp)[u];
-#pragma unroll
-        for (int k = 0; k < QT; ++k) s[k] = float4_t{0, 0, 0, 0};
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const half8_t kq = quants(kw[b]);
-            const half2_t d01 = __builtin_bit_cast(half2_t, d[2 * b]),
-                          d23 = __builtin_bit_cast(half2_t, d[2 * b + 1]);
-#pragma unroll
-            for (int k = 0; k < QT; ++k) {
-                float4_t c = {0, 0, 0, 0};
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q[k].lo[b], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q[k].hi[b], c, 0, 0, 0);
-                s[k][0] = fmaf(c[0], (float)d01.x, s[k][0]);
-                s[k][1] = fmaf(c[1], (float)d01.y, s[k][1]);
-                s[k][2] = fmaf(c[2], (float)d23.x, s[k][2]);
-                s[k][3] = fmaf(c[3], (float)d23.y, s[k][3]);
-            }
-        }
+            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[b], q.hi[b], s, 0, 0, 0);
+        return float4_t{block_sum<NB>(s[0] * (float)d01.x), block_sum<NB>(s[1] * (float)d01.y),
+                        block_sum<NB>(s[2] * (float)d23.x), block_sum<NB>(s[3] * (float)d23.y)};
     }
+    unsigned d[2 * NB];
+#pragma unroll
+    for (int u = 0; u < NB / 2; ++u)
+        *reinterpret_cast<uint4 *>(d + 4 * u) = reinterpret_cast<const uint4 *>(sp)[u];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const half8_t kq = pl.kop(t, b);
+        const half2_t d01 = __builtin_bit_cast(half2_t, d[2 * b]),
+                      d23 = __builtin_bit_cast(half2_t, d[2 * b + 1]);
+        float4_t c = {0, 0, 0, 0};
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q.lo[b], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq, q.hi[b], c, 0, 0, 0);
+        s[0] = fmaf(c[0], (float)d01.x, s[0]);
+        s[1] = fmaf(c[1], (float)d01.y, s[1]);
+        s[2] = fmaf(c[2], (float)d23.x, s[2]);
+        s[3] = fmaf(c[3], (float)d23.y, s[3]);
+    }
+    return s;
 }
 
-// The running softmax of a wave's columns.
-template <int HD, int QT>
+// The running softmax of a wave's 16 columns.
+template <int HD>
 struct Softmax {
-    float m[QT];    // per column, log2 units
-    float l[QT];    // of this lane's keys; l and o in units of 2^(ve - 14)
-    int ve = -100;  // 2^ve <= the largest d_v seen < 2^(ve + 1)
-    float4_t o[QT][HD / 16];
+    float m = -INFINITY;  // per column, log2 units
+    float l = 0.0f;       // of this lane's keys; l and o in units of 2^(ve - 14)
+    int ve = -100;        // 2^ve <= the largest d_v seen < 2^(ve + 1)
+    float4_t o[HD / 16];
     __device__ Softmax() {
 #pragma unroll
-        for (int k = 0; k < QT; ++k) {
-            m[k] = -INFINITY;
-            l[k] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < HD / 16; ++e) o[k][e] = float4_t{0, 0, 0, 0};
-        }
+        for (int e = 0; e < HD / 16; ++e) o[e] = float4_t{0, 0, 0, 0};
     }
 };
 
-// Adds one page.  WHOLE: every column sees its 64 keys; else keys [0, lim[k]) of it
-// are seen by this lane's column of tile k (none if <= 0), the first n_keys by any.
+// Adds one page.  WHOLE: every column sees its 64 keys; else keys [0, lim) of it
+// are seen by this lane's column (none if <= 0), the first n_keys by any.
 // s_ks, s_vs: its staged scales.
-template <int HD, int QT, bool FEW, bool WHOLE>
-__device__ inline void attend_page(const PageLoad<HD> &pl, const unsigned *s_ks,
-                                   const unsigned *s_vs, int lane, const QTile<HD, FEW> *q,
-                                   const int *lim, int n_keys, Softmax<HD, QT> &st) {
+template <int HD, bool FEW, bool WHOLE, class Src>
+__device__ inline void attend_page(const Src &pl, const unsigned *s_ks, const unsigned *s_vs,
+                                   int lane, const QTile<HD, FEW> &q, int lim, int n_keys,
+                                   Softmax<HD> &st) {
     constexpr int NB = HD / 32;
     const int g = lane >> 4;
     // the page's largest V scale; it seldom grows past the power of two in use
     float dmax = 0.0f;
 #pragma unroll
     for (int u = 0; u < NB / 2; ++u) {
-        half2_t d = __builtin_bit_cast(half2_t, pl.vs[u] & 0x7fff7fffu);
+        half2_t d = __builtin_bit_cast(half2_t, pl.vscale(u) & 0x7fff7fffu);
         if (!WHOLE) {  // what lies past the end counts for nothing
             const int w = lane * (NB / 2) + u, key = w / (2 * NB) * 4 + 2 * (w & 1);
             if (key >= n_keys) d.x = (_Float16)0.0f;
@@ -517,54 +519,39 @@ __device__ inline void attend_page(const PageLoad<HD> &pl, const unsigned *s_ks,
         }
         dmax = fmaxf(dmax, fmaxf((float)d.x, (float)d.y));
     }
-    float s[QT][16];
+    float s[16];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        float4_t v[QT];
-        score_tile<HD, QT, FEW>(pl.k[t], s_ks, t, lane, q, v);
+        const float4_t v = score_tile<HD, FEW>(pl, s_ks, t, lane, q);
 #pragma unroll
-        for (int k = 0; k < QT; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                s[k][4 * t + i] = WHOLE || 16 * t + 4 * g + i < lim[k] ? v[k][i] : -INFINITY;
+        for (int i = 0; i < 4; ++i)
+            s[4 * t + i] = WHOLE || 16 * t + 4 * g + i < lim ? v[i] : -INFINITY;
     }
-    float m_new[QT];
-    bool grows = dmax >= ldexpf(1.0f, st.ve + 1);
+    float pm = s[0];
 #pragma unroll
-    for (int k = 0; k < QT; ++k) {
-        float pm = s[k][0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[k][i]);
-        m_new[k] = fmaxf(st.m[k], col_max(pm) * q[k].inv);
-        grows = grows || m_new[k] > st.m[k];
-    }
-    if (__any(grows)) {
+    for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[i]);
+    const float m_new = fmaxf(st.m, col_max(pm) * q.inv);
+    if (__any(m_new > st.m || dmax >= ldexpf(1.0f, st.ve + 1))) {
 #pragma unroll
         for (int x = 1; x < kWave; x <<= 1) dmax = fmaxf(dmax, __shfl_xor(dmax, x, kWave));
         const int ve = max(dmax > 0.0f ? ilogbf(dmax) : -24, st.ve);
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+        const float f = ldexpf(__builtin_amdgcn_exp2f(st.m - m_use), st.ve - ve);
+        st.l = st.l * f;
 #pragma unroll
-        for (int k = 0; k < QT; ++k) {
-            const float m_use = m_new[k] == -INFINITY ? 0.0f : m_new[k];
-            const float f = ldexpf(__builtin_amdgcn_exp2f(st.m[k] - m_use), st.ve - ve);
-            st.l[k] = st.l[k] * f;
-#pragma unroll
-            for (int e = 0; e < HD / 16; ++e) st.o[k][e] = st.o[k][e] * f;
-            st.m[k] = m_new[k];
-        }
+        for (int e = 0; e < HD / 16; ++e) st.o[e] = st.o[e] * f;
+        st.m = m_new;
         st.ve = ve;
     }
     // p 2^(14 - ve)
+    const float m0 = (st.m == -INFINITY ? 0.0f : st.m) - (float)(14 - st.ve);
 #pragma unroll
-    for (int k = 0; k < QT; ++k) {
-        const float m0 = (st.m[k] == -INFINITY ? 0.0f : st.m[k]) - (float)(14 - st.ve);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[k][i] = __builtin_amdgcn_exp2f(fmaf(s[k][i], q[k].inv, -m0));
-            st.l[k] = st.l[k] + s[k][i];
-        }
+    for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], q.inv, -m0));
+        st.l = st.l + s[i];
     }
     // p d_v of the keys of half h under the scales d: two dwords a tile
-    auto weigh = [&](int k, int h, const unsigned (*d)[2], half8_t *hi, half8_t *lo)
+    auto weigh = [&](int h, const unsigned (*d)[2], half8_t *hi, half8_t *lo)
                      __attribute__((always_inline)) {
         half2_t hh[4], ll[4];
 #pragma unroll
@@ -573,14 +560,18 @@ __device__ inline void attend_page(const PageLoad<HD> &pl, const unsigned *s_ks,
             half2_t x = __builtin_bit_cast(half2_t, d[u >> 1][u & 1]);
             if (!WHOLE) {  // a key past the end may hold anything, NaN too
                 const int key = 16 * t + 4 * g + 2 * (u & 1);
-                if (key >= lim[k]) x.x = (_Float16)0.0f;
-                if (key + 1 >= lim[k]) x.y = (_Float16)0.0f;
+                if (key >= lim) x.x = (_Float16)0.0f;
+                if (key + 1 >= lim) x.y = (_Float16)0.0f;
             }
-            split2(fmaf(s[k][n], (float)x.x, 0.0f), fmaf(s[k][n + 1], (float)x.y, 0.0f), &hh[u],
-                   &ll[u]);
+            split2(fmaf(s[n], (float)x.x, 0.0f), fmaf(s[n + 1], (float)x.y, 0.0f), &hh[u], &ll[u]);
         }
         *hi = join(hh[0], hh[1], hh[2], hh[3]);
         *lo = join(ll[0], ll[1], ll[2], ll[3]);
+    };
+    auto sum = [&](int e, int h, half8_t hi, half8_t lo) __attribute__((always_inline)) {
+        const half8_t vq = pl.vop(e, h);
+        st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, lo, st.o[e], 0, 0, 0);
+        st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, hi, st.o[e], 0, 0, 0);
     };
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -593,13 +584,9 @@ __device__ inline void attend_page(const PageLoad<HD> &pl, const unsigned *s_ks,
                 d[u][0] = x.x, d[u][1] = x.y;
             }
             half8_t hi, lo;
-            weigh(0, h, d, &hi, &lo);
+            weigh(h, d, &hi, &lo);
 #pragma unroll
-            for (int e = 0; e < HD / 16; ++e) {
-                const half8_t vq = quants(pl.v[e][h]);
-                st.o[0][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, lo, st.o[0][e], 0, 0, 0);
-                st.o[0][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, hi, st.o[0][e], 0, 0, 0);
-            }
+            for (int e = 0; e < HD / 16; ++e) sum(e, h, hi, lo);
         } else {
             unsigned dv[2][2 * NB];  // the scales of tiles 2 h and 2 h + 1
 #pragma unroll
@@ -611,19 +598,10 @@ __device__ inline void attend_page(const PageLoad<HD> &pl, const unsigned *s_ks,
             for (int b = 0; b < NB; ++b) {
                 const unsigned d[2][2] = {{dv[0][2 * b], dv[0][2 * b + 1]},
                                           {dv[1][2 * b], dv[1][2 * b + 1]}};
-                half8_t hi[QT], lo[QT];
-#pragma unroll
-                for (int k = 0; k < QT; ++k) weigh(k, h, d, &hi[k], &lo[k]);
-#pragma unroll
-                for (int e = 2 * b; e < 2 * b + 2; ++e) {
-                    const half8_t vq = quants(pl.v[e][h]);
-#pragma unroll
-                    for (int k = 0; k < QT; ++k) {
-                        float4_t o = st.o[k][e];
-                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, lo[k], o, 0, 0, 0);
-                        st.o[k][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, hi[k], o, 0, 0, 0);
-                    }
-                }
+                half8_t hi, lo;
+                weigh(h, d, &hi, &lo);
+                sum(2 * b, h, hi, lo);
+                sum(2 * b + 1, h, hi, lo);
             }
         }
     }
@@ -735,16 +713,16 @@ constexpr int wgs_of(int hd) { return hd == 128 ? 1 : 3; }
 // (m, l, o) in `part` by device-scope stores that are complete before it counts
 // itself on the tile's counter; the one that counts last joins them in the order
 // of the runs and leaves the counter zero, so none waits for another.
-template <int HD, int QT, bool FEW, bool SPLIT>
+template <int HD, bool FEW, bool SPLIT>
 __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     Kv4Rows a, const float *__restrict__ q, size_t qs, bool vec, int groups, int n_qt,
     unsigned slots, float *__restrict__ out, size_t os, float *__restrict__ part,
     int *__restrict__ cnts, float *__restrict__ lse) {
     using P = Page<HD>;
-    constexpr int NQ = QTile<HD, FEW>::NQ, TW = QT * NQ;  // queries of a tile
+    constexpr int NQ = QTile<HD, FEW>::NQ;  // queries of a tile
     constexpr int kWaves = waves_of(HD, SPLIT);
-    __shared__ float s_m[kWaves][TW], s_l[kWaves][TW];
-    __shared__ __attribute__((aligned(16))) float s_o[kWaves][TW][HD + 4];
+    __shared__ float s_m[kWaves][NQ], s_l[kWaves][NQ];
+    __shared__ __attribute__((aligned(16))) float s_o[kWaves][NQ][HD + 4];
     __shared__ __attribute__((aligned(16))) unsigned s_d[kWaves][2][kScaleWords<HD>];
     __shared__ int s_last;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
@@ -760,8 +738,8 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     unsigned p0;
     const int cnt = (int)rows_of(a, b, &p0);
     const int n_q = cnt * groups;       // real queries of the KV head
-    if (qt * TW >= n_q) return;
-    const int last_row = (min(qt * TW + TW, n_q) - 1) / groups;
+    if (qt * NQ >= n_q) return;
+    const int last_row = (min(qt * NQ + NQ, n_q) - 1) / groups;
     const unsigned end = p0 + last_row + 1;  // keys that the tile's last row sees
     const unsigned end_pg = (end + kPageKeys - 1) / kPageKeys;
     const unsigned pg1 = SPLIT ? min(run.pg1, end_pg) : end_pg;
@@ -771,18 +749,16 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     PageLoad<HD> next;
     unsigned pg = run.pg0 + wv;
     if (pg < pg1) next.load(base + (size_t)pg * P::kBytes, lane);
-    QTile<HD, FEW> qtile[QT];
-    long see[QT];  // keys this column sees
-#pragma unroll
-    for (int k = 0; k < QT; ++k) {
-        const int qi = qt * TW + k * NQ + r % NQ, row = qi / groups;
-        const bool real = qi < n_q;
-        const int qh = head * groups + qi % groups;
-        qtile[k].load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, lane, vec);
-        see[k] = real ? (long)p0 + row + 1 : 0;
-    }
-    const unsigned all = p0 + (qt * TW) / groups + 1;        // keys every real column sees
-    Softmax<HD, QT> st;
+    const int qi = qt * NQ + r % NQ, row = qi / groups;
+    const bool real = qi < n_q;
+    QRaw<HD, FEW> raw;
+    raw.load(real ? q + row_index(a, b, row) * qs + (head * groups + qi % groups) * HD : nullptr,
+             lane, vec);
+    QTile<HD, FEW> qtile;
+    qtile.make(raw, lane);
+    const long see = real ? (long)p0 + row + 1 : 0;      // keys this column sees
+    const unsigned all = p0 + (qt * NQ) / groups + 1;    // keys every real column sees
+    Softmax<HD> st;
     for (; pg < pg1; pg += kWaves) {
         const PageLoad<HD> now = next;
         __builtin_amdgcn_wave_barrier();  // the last page's scales are read (LDS is in order)
@@ -792,38 +768,32 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         if (pg + kWaves < pg1) next.load(base + (size_t)(pg + kWaves) * P::kBytes, lane);
-        int lim[QT];
-#pragma unroll
-        for (int k = 0; k < QT; ++k) lim[k] = (int)min(see[k] - (long)pg * kPageKeys, 64l);
+        const int lim = (int)min(see - (long)pg * kPageKeys, 64l);
         if ((pg + 1) * kPageKeys <= all)
-            attend_page<HD, QT, FEW, true>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim, 64, st);
+            attend_page<HD, FEW, true>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim, 64, st);
         else
-            attend_page<HD, QT, FEW, false>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim,
-                                            (int)min(end - pg * kPageKeys, 64u), st);
+            attend_page<HD, FEW, false>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim,
+                                        (int)min(end - pg * kPageKeys, 64u), st);
     }
     // o holds 2^-9 of the quants; l and o back to their own units, the
     // column's sum over its four lane groups, then the waves
     const float down = ldexpf(1.0f, st.ve - 14);
-#pragma unroll
-    for (int k = 0; k < QT; ++k) {
-        const float l = col_sum(st.l[k]) * down;
-        const int c = k * NQ + r % NQ;
-        if (g == 0 && r < NQ) {
-            s_m[wv][c] = st.m[k];
-            s_l[wv][c] = l;
-        }
-#pragma unroll
-        for (int e = 0; e < HD / 16; ++e)
-            if (!FEW || e / 2 == r / NQ)
-                *reinterpret_cast<float4_t *>(&s_o[wv][c][16 * e + 4 * g]) =
-                    st.o[k][e] * (down * 0x1p9f);
+    st.l = col_sum(st.l) * down;
+    if (g == 0 && r < NQ) {
+        s_m[wv][r] = st.m;
+        s_l[wv][r] = st.l;
     }
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e)
+        if (!FEW || e / 2 == r / NQ)
+            *reinterpret_cast<float4_t *>(&s_o[wv][r % NQ][16 * e + 4 * g]) =
+                st.o[e] * (down * 0x1p9f);
     __syncthreads();
-    const int cols = min(TW, n_q - qt * TW);
+    const int cols = min(NQ, n_q - qt * NQ);
     const size_t z0 = ((size_t)b * a.rows) * (a.n_kv * groups);
     // four dims of a column from d on
     auto store = [&](int c, int d, float m, float l, const float *o) {
-        const int ci = qt * TW + c, oh = head * groups + ci % groups;
+        const int ci = qt * NQ + c, oh = head * groups + ci % groups;
         float *to = out + row_index(a, b, ci / groups) * os + oh * HD + d;
 #pragma unroll
         for (int j = 0; j < 4; ++j) to[j] = o[j] / l;
@@ -833,7 +803,7 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     const bool alone = !SPLIT || run.n == 1;
     // partial results of run i, column c
     auto part_of = [&](unsigned i, int c) {
-        return part + ((((size_t)(run.first + i) * a.n_kv + head) * n_qt + qt) * TW + c) * (HD + 2);
+        return part + ((((size_t)(run.first + i) * a.n_kv + head) * n_qt + qt) * NQ + c) * (HD + 2);
     };
     for (int it = threadIdx.x; it < cols * (HD / 4); it += kWaves * kWave) {
         const int c = it / (HD / 4), d = it % (HD / 4) * 4;
@@ -906,67 +876,290 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     }
 }
 
-// The keys' attention weights: one wave a page of a KV head goes over all the
-// queries that see it, with the scores of the attention itself and the
-// rows' log-sum-exps, so each key has one writer and one order of sums.
+// Prompts: a workgroup takes 64 queries of a KV head over all the pages they see,
+// a tile of 16 a wave.  The waves turn each page's quants into f16 operands once,
+// a quarter each, and read them from LDS in the operands' order; the next page
+// comes in while this one is computed, into a second buffer (one barrier a page).
+// The workgroups with the most pages start first.
+constexpr int kPromptWaves = 4;
 template <int HD>
-__global__ __launch_bounds__(kWave) void k_kv4_weights(Kv4Rows a, const float *__restrict__ q,
-                                                       size_t qs, bool vec, int groups, int n_pages,
-                                                       const float *__restrict__ lse,
-                                                       float *__restrict__ weights) {
+struct LdsPage {
+    static constexpr int NB = HD / 32;
+    half8_t k[4][NB][kWave];
+    half8_t v[HD / 16][2][kWave];
+    unsigned d[2][kScaleWords<HD>];
+};
+template <int HD>
+struct LdsSrc {
+    const LdsPage<HD> &p;
+    int lane;
+    __device__ half8_t kop(int t, int b) const { return p.k[t][b][lane]; }
+    __device__ half8_t vop(int e, int h) const { return p.v[e][h][lane]; }
+    __device__ unsigned vscale(int u) const { return p.d[1][lane * (HD / 64) + u]; }
+};
+// What a thread holds of a page on its way to LDS: K tile `wave`, V chunk `wave`
+// (head dim 64: the first two waves), and the first wave K's scales, the second V's.
+template <int HD>
+struct PagePart {
     using P = Page<HD>;
-    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    static constexpr int NB = HD / 32;
+    unsigned k[NB], v[4], d[NB / 2];
+    __device__ void load(const uint8_t *pb, int wv, int lane) {
+        const uint8_t *kp = pb + wv * 8 * HD + lane * 4 * NB;
+        if constexpr (HD == 128) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(kp);
+            k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2 *>(kp);
+            k[0] = x.x, k[1] = x.y;
+        }
+        if (wv < NB) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(pb + P::kV + wv * 1024 + lane * 16);
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        }
+        if (wv < 2) PageLoad<HD>::load_scales(pb + (wv ? P::kVs : P::kKs), lane, d);
+    }
+    __device__ void store(LdsPage<HD> &p, int wv, int lane) const {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) p.k[wv][b][lane] = quants(k[b]);
+        if (wv < NB) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p.v[2 * wv + (i >> 1)][i & 1][lane] = quants(v[i]);
+        }
+        if (wv < 2) PageLoad<HD>::stage(d, lane, p.d[wv]);
+    }
+};
+
+template <int HD>
+__global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
+    Kv4Rows a, const float *__restrict__ q, size_t qs, bool vec, int groups, int n_qg,
+    float *__restrict__ out, size_t os, float *__restrict__ lse) {
+    using P = Page<HD>;
+    constexpr int QW = kPromptWaves * 16;  // queries of a workgroup
+    __shared__ LdsPage<HD> s_p[2];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
     unsigned x = blockIdx.x;
-    const unsigned pg = x % n_pages;
-    x /= n_pages;
-    const int head = x % a.n_kv, b = x / a.n_kv;
+    const int head = x % a.n_kv;
+    x /= a.n_kv;
+    const int b = x % a.n_seqs, qg = n_qg - 1 - (int)(x / a.n_seqs);
     unsigned p0;
     const int cnt = (int)rows_of(a, b, &p0);
-    const unsigned key0 = pg * kPageKeys;
-    if (cnt == 0 || key0 >= p0 + cnt) return;
     const int n_q = cnt * groups;
-    const uint8_t *pb = a.pages + (((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages + pg) *
-                                      P::kBytes;
-    __shared__ __attribute__((aligned(16))) unsigned s_d[kScaleWords<HD>];
-    PageLoad<HD> page;
-    page.load_k(pb, lane);
-    PageLoad<HD>::stage(page.ks, lane, s_d);
+    if (qg * QW >= n_q) return;
+    const unsigned n_pg = (p0 + (min(qg * QW + QW, n_q) - 1) / groups) / kPageKeys + 1;
+    const uint8_t *base =
+        a.pages + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages * P::kBytes;
+    PagePart<HD> next;
+    next.load(base, wv, lane);
+    const int q0 = qg * QW + wv * 16, qi = q0 + r, row = qi / groups;
+    const bool real = qi < n_q;
+    const int qh = head * groups + qi % groups;
+    QTile<HD, false> qtile;
+    {
+        QRaw<HD, false> raw;
+        raw.load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, lane, vec);
+        qtile.make(raw, lane);
+    }
+    const long see = real ? (long)p0 + row + 1 : 0;  // keys this column sees
+    const unsigned all = p0 + q0 / groups + 1;       // keys every real column of the wave sees
+    // pages that the wave's last row sees
+    const unsigned my_pg =
+        q0 < n_q ? (p0 + (min(q0 + 16, n_q) - 1) / groups) / kPageKeys + 1 : 0;
+    const unsigned end = q0 < n_q ? p0 + (min(q0 + 16, n_q) - 1) / groups + 1 : 0;
+    Softmax<HD> st;
+    next.store(s_p[0], wv, lane);
     __syncthreads();
+    for (unsigned pg = 0; pg < n_pg; ++pg) {
+        const LdsSrc<HD> src{s_p[pg & 1], lane};
+        if (pg + 1 < n_pg) next.load(base + (size_t)(pg + 1) * P::kBytes, wv, lane);
+        const int lim = (int)min(see - (long)pg * kPageKeys, 64l);
+        if ((pg + 1) * kPageKeys <= all)
+            attend_page<HD, false, true>(src, src.p.d[0], src.p.d[1], lane, qtile, lim, 64, st);
+        else if (pg < my_pg)
+            attend_page<HD, false, false>(src, src.p.d[0], src.p.d[1], lane, qtile, lim,
+                                          (int)min(end - pg * kPageKeys, 64u), st);
+        if (pg + 1 < n_pg) next.store(s_p[(pg + 1) & 1], wv, lane);
+        __syncthreads();
+    }
+    const float l = col_sum(st.l);
+    if (!real) return;
+    // l and o share their power of two; o holds 2^-9 of the quants
+    float *to = out + row_index(a, b, row) * os + qh * HD + 4 * g;
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[16 * e + i] = st.o[e][i] * 0x1p9f / l;
+    if (lse && g == 0)
+        lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] =
+            st.m + __log2f(l * ldexpf(1.0f, st.ve - 14));
+}
+
+// The keys' attention weights: a wave a page of a KV head goes over all the
+// queries that see it, with the scores of the attention itself and the rows'
+// log-sum-exps; the page's quants stay in its registers.  The four waves of a
+// workgroup (consecutive pages) prepare a query tile each and share the four
+// through LDS.  Where pages alone do not fill the CUs, n_parts workgroups take
+// every n_parts-th batch of four tiles, and the one that is done last adds their
+// sums in order: each key has one writer and one order of sums.
+constexpr int kWtWaves = 4;
+template <int HD>
+__global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
+    Kv4Rows a, const float *__restrict__ q, size_t qs, bool vec, int groups, int n_grp,
+    int n_parts, const float *__restrict__ lse, float *__restrict__ weights,
+    float *__restrict__ part, int *__restrict__ cnts) {
+    using P = Page<HD>;
+    constexpr int NB = P::NB;
+    __shared__ half8_t s_q[kWtWaves][NB][2][kWave];
+    __shared__ float s_inv[kWtWaves][16], s_z[kWtWaves][16];
+    __shared__ unsigned s_see[kWtWaves][16];
+    __shared__ __attribute__((aligned(16))) unsigned s_d[kWtWaves][kScaleWords<HD>];
+    __shared__ float s_w[kWtWaves][kPageKeys];
+    __shared__ int s_last;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    unsigned x = blockIdx.x;
+    const int mine = x % n_parts;
+    x /= n_parts;
+    const int head = x % a.n_kv;
+    x /= a.n_kv;
+    const int b = x % a.n_seqs, grp = x / a.n_seqs;  // (the first keys have the most queries)
+    unsigned p0;
+    const int cnt = (int)rows_of(a, b, &p0);
+    const unsigned end = p0 + cnt, key0 = grp * kWtWaves * kPageKeys;
+    if (cnt == 0 || key0 >= end) return;
+    const unsigned pg = grp * kWtWaves + wv, pkey = pg * kPageKeys;
+    const bool has = pkey < end;
+    const int n_q = cnt * groups;
     float w[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = 0.0f;
-    const int row0 = key0 > p0 ? (int)(key0 - p0) : 0;  // the first row that sees the page
-    for (int qt = row0 * groups / 16; qt * 16 < n_q; ++qt) {
-        const int qi = qt * 16 + r, row = qi / groups;
+    half8_t kq[4][NB];
+    if (has) {
+        PageLoad<HD> pl;
+        pl.load_k(a.pages + (((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages + pg) *
+                                P::kBytes,
+                  lane);
+        PageLoad<HD>::stage(pl.ks, lane, s_d[wv]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < NB; ++c) kq[t][c] = quants(pl.k[t][c]);
+    }
+    // from the first row that sees the group's first key on; a tile's queries are
+    // loaded while the batch before it is computed
+    const int qt0 = (key0 > p0 ? (int)(key0 - p0) : 0) * groups / 16;
+    const int n_qt = (n_q + 15) / 16, step = n_parts * kWtWaves;
+    QRaw<HD, false> raw;
+    float z_next = 0.0f;
+    unsigned see_next = 0;
+    auto fetch = [&](int t) {
+        const int qi = t * 16 + r, row = qi / groups;
         const bool real = qi < n_q;
-        const size_t qrow = row_index(a, b, row);
         const int qh = head * groups + qi % groups;
-        QTile<HD, false> qtile;
-        qtile.load(real ? q + qrow * qs + qh * HD : nullptr, lane, vec);
-        const float z = real ? lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] : 0.0f;
-        const long lim = real ? (long)p0 + row + 1 - (long)key0 : 0;
+        raw.load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, lane, vec);
+        see_next = real ? p0 + row + 1 : 0;
+        z_next = real ? lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] : 0.0f;
+    };
+    fetch(qt0 + mine * kWtWaves + wv);
+    for (int q0 = qt0 + mine * kWtWaves; q0 < n_qt; q0 += step) {
+        const int nt = min(kWtWaves, n_qt - q0);
+        {
+            QTile<HD, false> qt;
+            qt.make(raw, lane);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            float4_t s;
-            score_tile<HD, 1, false>(page.k[t], s_d, t, lane, &qtile, &s);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (16 * t + 4 * g + i < lim)
-                    w[4 * t + i] =
-                        w[4 * t + i] + __builtin_amdgcn_exp2f(fmaf(s[i], qtile.inv, -z));
+            for (int c = 0; c < NB; ++c) {
+                s_q[wv][c][0][lane] = qt.hi[c];
+                s_q[wv][c][1][lane] = qt.lo[c];
+            }
+            if (g == 0) {
+                s_inv[wv][r] = qt.inv;
+                s_z[wv][r] = z_next;
+                s_see[wv][r] = see_next;
+            }
         }
+        __syncthreads();
+        fetch(q0 + step + wv);
+        // the first of the tiles whose last row sees this wave's page
+        for (int u = 0; u < nt && has; ++u) {
+            const int c0 = (q0 + u) * 16, c1 = min(c0 + 16, n_q) - 1;
+            if (p0 + c1 / groups < pkey) continue;
+            const bool whole = c0 + 16 <= n_q && p0 + c0 / groups + 1 >= pkey + kPageKeys;
+            const float inv = s_inv[u][r], z = s_z[u][r];
+            const int lim = (int)(s_see[u][r] - min(pkey, s_see[u][r]));
+            half8_t hi[NB], lo[NB];
+#pragma unroll
+            for (int c = 0; c < NB; ++c) {
+                hi[c] = s_q[u][c][0][lane];
+                lo[c] = s_q[u][c][1][lane];
+            }
+            float s[16];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                unsigned kd[2 * NB];  // the scales of this lane's keys
+#pragma unroll
+                for (int c = 0; c < NB / 2; ++c)
+                    *reinterpret_cast<uint4 *>(kd + 4 * c) =
+                        reinterpret_cast<const uint4 *>(s_d[wv] + (t * 4 + g) * 2 * NB)[c];
+#pragma unroll
+                for (int c = 0; c < NB; ++c) {
+                    float4_t y = {0, 0, 0, 0};
+                    y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[t][c], lo[c], y, 0, 0, 0);
+                    y = __builtin_amdgcn_mfma_f32_16x16x32_f16(kq[t][c], hi[c], y, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const half2_t d = __builtin_bit_cast(half2_t, kd[2 * c + (i >> 1)]);
+                        const float x = (float)(i & 1 ? d.y : d.x);
+                        s[4 * t + i] = c == 0 ? y[i] * x : fmaf(y[i], x, s[4 * t + i]);
+                    }
+                }
+            }
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    w[i] = w[i] + __builtin_amdgcn_exp2f(fmaf(s[i], inv, -z));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (16 * (i >> 2) + 4 * g + (i & 3) < lim)
+                        w[i] = w[i] + __builtin_amdgcn_exp2f(fmaf(s[i], inv, -z));
+            }
+        }
+        __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) w[i] = w[i] + __shfl_xor(w[i], o, kWave);
-    if (r == 0) {
-        float *wr = weights + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.max_seq;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const unsigned key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
-            if (key < p0 + cnt) wr[key] = (key < p0 ? wr[key] : 0.0f) + w[i];
-        }
+    for (int i = 0; i < 16; ++i) {
+        float v = w[i];
+        v = v + ror<8>(v);
+        v = v + ror<4>(v);
+        v = v + ror<2>(v);
+        v = v + ror<1>(v);
+        if (r == 0) s_w[wv][16 * (i >> 2) + 4 * g + (i & 3)] = v;
+    }
+    __syncthreads();
+    float sum = s_w[wv][lane];
+    const size_t row = (size_t)b * a.n_kv + head;
+    if (n_parts > 1) {
+        float *pp = part + (row * n_grp + grp) * n_parts * (kWtWaves * kPageKeys) + threadIdx.x;
+        __hip_atomic_store(pp + mine * (kWtWaves * kPageKeys), sum, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the sums are at the device
+        __syncthreads();
+        int *cn = cnts + row * n_grp + grp;
+        if (threadIdx.x == 0)
+            s_last = __hip_atomic_fetch_add(cn, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                     n_parts - 1;
+        __syncthreads();
+        if (!s_last) return;
+        if (threadIdx.x == 0)
+            __hip_atomic_store(cn, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sum = 0.0f;
+        for (int i = 0; i < n_parts; ++i)
+            sum = sum + __hip_atomic_load(pp + i * (kWtWaves * kPageKeys), __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_AGENT);
+    }
+    const unsigned key = pkey + lane;
+    if (key < end) {
+        float *to = weights + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.max_seq + key;
+        *to = (key < p0 ? *to : 0.0f) + sum;
     }
 }
 
@@ -1240,41 +1433,57 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
     const size_t n_q = (size_t)a.rows * groups;
     const bool vec = qs % 4 == 0 && al16(q);
     float *z = weights ? lse : nullptr;
-    auto go = [&](auto qt_, auto few_) -> mri_status {
-        constexpr int QT = decltype(qt_)::value;
+    const size_t cus = (size_t)std::max(device_cus(), 1);
+    auto go = [&](auto few_) -> mri_status {
         constexpr bool FEW = decltype(few_)::value;
-        constexpr int TW = QT * QTile<HD, FEW>::NQ;
-        const size_t n_qt = (n_q + TW - 1) / TW, tiles = n_qt * a.n_kv;
+        constexpr int NQ = QTile<HD, FEW>::NQ;
+        const size_t n_qt = (n_q + NQ - 1) / NQ, tiles = n_qt * a.n_kv;
         // a call with tiles for less than half of the CUs splits its keys
-        const size_t fill =
-            std::min<size_t>(wgs_of(HD) * (size_t)std::max(device_cus(), 1), kKv4PartTiles / QT);
+        const size_t fill = std::min<size_t>(wgs_of(HD) * cus, kKv4PartTiles);
         if (tiles * a.n_seqs * 2 <= fill) {
             const size_t slots = fill / tiles;
-            hipLaunchKernelGGL((k_kv4_attend<HD, QT, FEW, true>), dim3((unsigned)(slots * tiles)),
-                               dim3(waves_of(HD, true) * kWave), 0, s, a, q, qs, vec, groups, (int)n_qt,
-                               (unsigned)slots, out, os, part, cnts, z);
+            hipLaunchKernelGGL((k_kv4_attend<HD, FEW, true>), dim3((unsigned)(slots * tiles)),
+                               dim3(waves_of(HD, true) * kWave), 0, s, a, q, qs, vec, groups,
+                               (int)n_qt, (unsigned)slots, out, os, part, cnts, z);
         } else {
             const size_t blocks = tiles * a.n_seqs;
             if (const mri_status st = grid_ok(blocks)) return st;
-            hipLaunchKernelGGL((k_kv4_attend<HD, QT, FEW, false>), dim3((unsigned)blocks),
-                               dim3(waves_of(HD, false) * kWave), 0, s, a, q, qs, vec, groups, (int)n_qt, 0u, out, os, part, cnts, z);
+            hipLaunchKernelGGL((k_kv4_attend<HD, FEW, false>), dim3((unsigned)blocks),
+                               dim3(waves_of(HD, false) * kWave), 0, s, a, q, qs, vec, groups,
+                               (int)n_qt, 0u, out, os, part, cnts, z);
         }
         MRI_LAUNCHED("k_kv4_attend");
         return MRI_OK;
     };
-    using T = std::true_type;
-    using F = std::false_type;
-    mri_status st;
-    if (n_q <= QTile<HD, true>::NQ) st = go(std::integral_constant<int, 1>{}, T{});
-    else if (n_q <= 16) st = go(std::integral_constant<int, 1>{}, F{});
-    else st = go(std::integral_constant<int, 1>{}, F{});
-    if (st) return st;
+    const size_t n_qg = (n_q + kPromptWaves * 16 - 1) / (kPromptWaves * 16);
+    const size_t prompt_wgs = n_qg * a.n_kv * a.n_seqs;
+    if (n_q > 32 && prompt_wgs >= cus) {
+        if (const mri_status st = grid_ok(prompt_wgs)) return st;
+        hipLaunchKernelGGL((k_kv4_prompt<HD>), dim3((unsigned)prompt_wgs),
+                           dim3(kPromptWaves * kWave), 0, s, a, q, qs, vec, groups, (int)n_qg, out,
+                           os, z);
+        MRI_LAUNCHED("k_kv4_prompt");
+    } else {
+        const mri_status st =
+            n_q <= QTile<HD, true>::NQ ? go(std::true_type{}) : go(std::false_type{});
+        if (st) return st;
+    }
     if (weights) {
-        const size_t n_pg = a.pos ? a.n_pages : (a.start + (size_t)a.row0 + a.rows - 1) / kPageKeys + 1;
-        const size_t blocks = n_pg * a.n_kv * a.n_seqs;
-        if (const mri_status st = grid_ok(blocks)) return st;
-        hipLaunchKernelGGL((k_kv4_weights<HD>), dim3((unsigned)blocks), dim3(kWave), 0, s, a, q,
-                           qs, vec, groups, (int)n_pg, lse, weights);
+        const size_t n_pg =
+            a.pos ? a.n_pages : (a.start + (size_t)a.row0 + a.rows - 1) / kPageKeys + 1;
+        const size_t n_grp = (n_pg + kWtWaves - 1) / kWtWaves;
+        const size_t groups_all = n_grp * a.n_kv * a.n_seqs;
+        // parts of the queries: three workgroups a CU, four query tiles a part at least
+        size_t parts = 3 * cus / groups_all;
+        parts = std::min(parts, ((n_q + 15) / 16 + kWtWaves - 1) / kWtWaves);
+        parts = std::max<size_t>(1, std::min<size_t>(parts, 16));
+        if (groups_all > kKv4PartTiles ||
+            groups_all * parts * kWtWaves * kPageKeys > kv4_part_floats(HD))
+            parts = 1;
+        if (const mri_status e = grid_ok(groups_all * parts)) return e;
+        hipLaunchKernelGGL((k_kv4_weights<HD>), dim3((unsigned)(groups_all * parts)),
+                           dim3(kWtWaves * kWave), 0, s, a, q, qs, vec, groups, (int)n_grp,
+                           (int)parts, lse, weights, part, cnts);
         MRI_LAUNCHED("k_kv4_weights");
     }
     return MRI_OK;
