@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "common.hpp"
+#include "kv4.hpp"
 
 struct mri_qmatrix {
     mri::QMatrixDev d;
@@ -120,7 +121,7 @@ mri_status scratch_get(hipStream_t stream, size_t bytes, void **ptr) {
 // The Q4_0 GEMM has its own: it uses it in no captured call, so it may grow
 // beside recorded graphs, whose INT8 and Q8_0 GEMMs replay with g_ws.
 static std::mutex g_ws_mu;
-static std::map<std::pair<int, hipStream_t>, Scratch> g_ws, g_q4ws, g_aws;
+static std::map<std::pair<int, hipStream_t>, Scratch> g_ws, g_q4ws, g_aws, g_sws;
 
 static mri_status zeroed_ws_get(std::map<std::pair<int, hipStream_t>, Scratch> &map,
                                 hipStream_t stream, size_t bytes, void **ptr) {
@@ -182,6 +183,22 @@ mri_status q4_ws_get(hipStream_t stream, size_t bytes, void **ptr) {
         if (old) {
             MRI_HIP(hipStreamSynchronize(stream));
             MRI_HIP(hipFree(old));
+        }
+    }
+    *ptr = sc.ptr;
+    return MRI_OK;
+}
+
+mri_status softmax_ws_get(hipStream_t stream, void **ptr) {
+    int dev = 0;
+    MRI_HIP(hipGetDevice(&dev));
+    std::lock_guard<std::mutex> lk(g_ws_mu);
+    Scratch &sc = g_sws[{dev, stream}];
+    if (!sc.ptr) {
+        const RelaxedCapture relaxed;
+        if (hipMalloc(&sc.ptr, kSoftmaxWsBytes) != hipSuccess) {
+            (void)hipGetLastError();
+            sc.ptr = nullptr;
         }
     }
     *ptr = sc.ptr;

@@ -1172,13 +1172,16 @@ __device__ inline unsigned weight_key(float w) {
 }
 
 // The kept positions of one (layer, sequence, KV head) a workgroup: the k-th
-// largest weight by four passes over its bytes (counts in LDS), then the
-// positions above it and the first of those equal to it, in order: each wave
-// counts and writes a contiguous sixteenth.
-constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / kWave;
+// largest weight by three passes over its bits (11, 11 and 10, counts in LDS: an
+// exponent alone would put most weights on a few counters), then the positions
+// above it and the first of those equal to it, in order: each wave counts and
+// writes contiguous positions.  Up to 32768 weights are read once, into registers.
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / kWave, kSelBins = 2048;
+constexpr int kSelRegs = 32;
+template <bool REGS>
 __global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
-    __shared__ unsigned s_hist[256];
-    __shared__ unsigned s_digit, s_left;
+    __shared__ unsigned s_hist[kSelBins];
+    __shared__ unsigned s_wave[kSelWaves], s_digit, s_left;
     __shared__ unsigned s_gt[kSelWaves], s_eq[kSelWaves];
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
     const size_t rowi = blockIdx.x;
@@ -1193,51 +1196,69 @@ __global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
     const unsigned old = n - e.recent, take = e.keep - e.recent;
     for (unsigned i = t; i < e.recent; i += kSelThreads) kept[take + i] = old + i;
     if (take == 0) return;
-    unsigned prefix = 0, left = take;  // the digits so far; how many to take below them
-    for (int pass = 0; pass < 4; ++pass) {
-        const int sh = 24 - 8 * pass;
-        if (t < 256) s_hist[t] = 0;
+    // wave wv has positions [wv seg, (wv + 1) seg), 64 at a time
+    const unsigned seg = ((old + kSelWaves - 1) / kSelWaves + kWave - 1) / kWave * kWave;
+    const unsigned i0 = min(wv * seg, old), i1 = min(i0 + seg, old);
+    unsigned reg[REGS ? kSelRegs : 1];
+    if constexpr (REGS) {
+#pragma unroll
+        for (int u = 0; u < kSelRegs; ++u) {
+            const unsigned i = i0 + u * kWave + lane;
+            reg[u] = i < i1 ? __float_as_uint(w[i]) : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < kSelRegs; ++u) reg[u] = weight_key(__uint_as_float(reg[u]));
+    }
+    // f(key, position) of each of the wave's positions, 64 at a time; ok: a real one
+    auto each = [&](auto &&f) __attribute__((always_inline)) {
+        if constexpr (REGS) {
+#pragma unroll
+            for (int u = 0; u < kSelRegs; ++u) {
+                const unsigned i = i0 + u * kWave;
+                if (i < i1) f(reg[u], i + lane, i + lane < i1);
+            }
+        } else {
+            for (unsigned i = i0; i < i1; i += kWave)
+                f(i + lane < i1 ? weight_key(w[i + lane]) : 0u, i + lane, i + lane < i1);
+        }
+    };
+    unsigned prefix = 0, left = take;  // the bits so far; how many to take below them
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        s_hist[t] = 0;
+        s_hist[t + kSelThreads] = 0;
         __syncthreads();
-        for (unsigned i = t; i < old; i += kSelThreads) {
-            const unsigned key = weight_key(w[i]);
-            if (pass == 0 || (key >> (sh + 8)) == prefix) atomicAdd(&s_hist[key >> sh & 255], 1u);
+        each([&](unsigned key, unsigned, bool ok) {
+            if (ok && (pass == 0 || (key >> (sh + bits)) == prefix))
+                atomicAdd(&s_hist[key >> sh & ((1u << bits) - 1)], 1u);
+        });
+        __syncthreads();
+        // thread t holds digits 2047 - 2 t and 2046 - 2 t, from the largest down
+        const unsigned c0 = s_hist[kSelBins - 1 - 2 * t], c1 = s_hist[kSelBins - 2 - 2 * t];
+        const unsigned inc = wave_scan_u(c0 + c1);
+        if (lane == kWave - 1) s_wave[wv] = inc;
+        __syncthreads();
+        unsigned above = inc - c0 - c1;
+        for (int u = 0; u < wv; ++u) above += s_wave[u];
+        if (above < left && left <= above + c0) {
+            s_digit = kSelBins - 1 - 2 * t;
+            s_left = left - above;
+        } else if (above + c0 < left && left <= above + c0 + c1) {
+            s_digit = kSelBins - 2 - 2 * t;
+            s_left = left - above - c0;
         }
         __syncthreads();
-        if (wv == 0) {
-            // lane l holds digits 255 - 4 l .. 252 - 4 l, from the largest down
-            unsigned c[4], sum = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum += c[i] = s_hist[255 - 4 * lane - i];
-            unsigned inc = sum;
-#pragma unroll
-            for (int o = 1; o < kWave; o <<= 1) {
-                const unsigned y = __shfl_up(inc, o, kWave);
-                if (lane >= o) inc += y;
-            }
-            unsigned above = inc - sum;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (above < left && left <= above + c[i]) {
-                    s_digit = 255 - 4 * lane - i;
-                    s_left = left - above;
-                }
-                above += c[i];
-            }
-        }
-        __syncthreads();
-        prefix = prefix << 8 | s_digit;
+        prefix = prefix << bits | s_digit;
         left = s_left;
         __syncthreads();
     }
     // keys > prefix are taken, and the first `left` of those equal to it
-    const unsigned seg = ((old + kSelWaves - 1) / kSelWaves + kWave - 1) / kWave * kWave;
-    const unsigned i0 = min(wv * seg, old), i1 = min(i0 + seg, old);
     unsigned gt = 0, eq = 0;
-    for (unsigned i = i0; i < i1; i += kWave) {
-        const unsigned key = i + lane < i1 ? weight_key(w[i + lane]) : 0;
-        gt += __popcll(__ballot(i + lane < i1 && key > prefix));
-        eq += __popcll(__ballot(i + lane < i1 && key == prefix));
-    }
+    each([&](unsigned key, unsigned, bool ok) {
+        gt += __popcll(__ballot(ok && key > prefix));
+        eq += __popcll(__ballot(ok && key == prefix));
+    });
     if (lane == 0) {
         s_gt[wv] = gt;
         s_eq[wv] = eq;
@@ -1249,17 +1270,15 @@ __global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
         eq += s_eq[u];
     }
     const unsigned long long below = (1ull << lane) - 1;
-    for (unsigned i = i0; i < i1; i += kWave) {
-        const bool in = i + lane < i1;
-        const unsigned key = in ? weight_key(w[i + lane]) : 0;
-        const unsigned long long bg = __ballot(in && key > prefix),
-                                 be = __ballot(in && key == prefix);
-        const unsigned g_at = gt + __popcll(bg & below), e_at = eq + __popcll(be & below);
-        const unsigned at = g_at + min(e_at, left);
-        if (in && (key > prefix || (key == prefix && e_at < left))) kept[at] = i + lane;
+    each([&](unsigned key, unsigned i, bool ok) {
+        const unsigned long long bg = __ballot(ok && key > prefix),
+                                 be = __ballot(ok && key == prefix);
+        const unsigned e_at = eq + __popcll(be & below);
+        const unsigned at = gt + __popcll(bg & below) + min(e_at, left);
+        if (ok && (key > prefix || (key == prefix && e_at < left))) kept[at] = i;
         gt += __popcll(bg);
         eq += __popcll(be);
-    }
+    });
 }
 
 // Moves the kept keys of one (layer, sequence, KV head) to their new places,
@@ -1527,7 +1546,10 @@ mri_status launch_kv4_attend(const Kv4Rows &a, size_t hd, const float *q, size_t
 mri_status launch_kv4_evict(const Kv4Evict &e, size_t hd, hipStream_t s) {
     const size_t rows = (size_t)e.n_layers * e.n_seqs * e.n_kv;
     if (const mri_status st = grid_ok(rows * 4)) return st;
-    hipLaunchKernelGGL(k_kv4_select, dim3((unsigned)rows), dim3(kSelThreads), 0, s, e);
+    if (e.src_max <= kSelRegs * kSelThreads)
+        hipLaunchKernelGGL(k_kv4_select<true>, dim3((unsigned)rows), dim3(kSelThreads), 0, s, e);
+    else
+        hipLaunchKernelGGL(k_kv4_select<false>, dim3((unsigned)rows), dim3(kSelThreads), 0, s, e);
     MRI_LAUNCHED("k_kv4_select");
     const size_t per_row = e.src == e.dst ? 1 : (e.keep + kPageKeys - 1) / kPageKeys;
     if (const mri_status st = grid_ok(rows * per_row)) return st;

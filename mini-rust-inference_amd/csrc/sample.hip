@@ -2,6 +2,7 @@
 // tokens against them.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 
 #include "kv4.hpp"
@@ -11,97 +12,212 @@ namespace {
 
 constexpr int kWave = 64;
 
+// Four floats at any float's address (global loads and stores of four words need
+// no more than a word's alignment).
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+
 // ---- softmax with a temperature ----------------------------------------------
-// p_i = exp((x_i - max x) / T) / sum: one workgroup a row, which is read
-// twice (the second time from cache) and written once.  Each thread keeps a
-// running maximum and the sum of exponentials under it.
+// p_i = exp((x_i - max x) / T) / sum.  A row is cut into `parts` parts of `len`
+// values (a multiple of four); 256 threads take a part's (max, sum of
+// exponentials under it), sixteen values a thread at a time.  Few rows: a
+// workgroup a part, then a second launch that joins a row's parts and writes; the
+// values come from the device's cache then.  Else a workgroup of 1024 a row does
+// the same steps, four parts at a time, to the same bits.
 __device__ inline float exp_scaled(float d, float c) {
     return __builtin_amdgcn_exp2f(d * c);  // c = log2(e) / T
 }
+struct MaxSum {
+    float m, l;  // l = sum of exp of what is not -inf; NaN stays in it
+};
+__device__ inline MaxSum join(MaxSum a, MaxSum b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    return MaxSum{m, (a.m == m ? a.l : a.l * exp_scaled(a.m - m, c)) +
+                         (b.m == m ? b.l : b.l * exp_scaled(b.m - m, c))};
+}
 
-template <int NT>
-__global__ __launch_bounds__(NT) void k_softmax(const float *x, size_t n, size_t xs, float c,
-                                                float *out, size_t os) {
-    __shared__ float s_m[NT / kWave], s_l[NT / kWave];
-    const float *row = x + (size_t)blockIdx.x * xs;
-    float *orow = out + (size_t)blockIdx.x * os;
-    float m = -INFINITY, l = 0.0f;
-    for (size_t i = threadIdx.x; i < n; i += NT) {
-        const float v = row[i];
-        if (v > m) {
-            l = l * exp_scaled(m - v, c) + 1.0f;
-            m = v;
-        } else if (!(v == -INFINITY)) {
-            l = l + exp_scaled(v - m, c);  // NaN stays in the sum
+constexpr int kPartThreads = 256;
+// (max, sum) of x[lo, hi) over 256 threads, t of them this one; s_ms: four entries.
+__device__ inline MaxSum part_stats(const float *x, size_t lo, size_t hi, int t, float c,
+                                    MaxSum *s_ms) {
+    MaxSum a{-INFINITY, 0.0f};
+    for (size_t i0 = lo; i0 < hi; i0 += 16 * kPartThreads) {
+        float v[16];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const size_t i = i0 + 4 * ((size_t)u * kPartThreads + t);
+            if (i + 4 <= hi) {
+                const float4u w = *reinterpret_cast<const float4u *>(x + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * u + j] = w[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * u + j] = i + j < hi ? x[i + j] : -INFINITY;
+            }
         }
+        float m = a.m;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) m = fmaxf(m, v[j]);
+        float l = a.m == m ? a.l : a.l * exp_scaled(a.m - m, c);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            l = l + (v[j] == -INFINITY ? 0.0f : exp_scaled(v[j] - m, c));
+        a = MaxSum{m, l};
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor(m, o, kWave), l2 = __shfl_xor(l, o, kWave);
-        const float mm = fmaxf(m, m2);
-        l = (m == mm ? l : l * exp_scaled(m - mm, c)) + (m2 == mm ? l2 : l2 * exp_scaled(m2 - mm, c));
-        m = mm;
+    for (int o = 32; o > 0; o >>= 1)
+        a = join(a, MaxSum{__shfl_xor(a.m, o, kWave), __shfl_xor(a.l, o, kWave)}, c);
+    if (t % kWave == 0) s_ms[t / kWave] = a;
+    __syncthreads();
+    a = join(join(s_ms[0], s_ms[1], c), join(s_ms[2], s_ms[3], c), c);
+    __syncthreads();
+    return a;
+}
+
+// A row's probabilities x[lo, hi) from its (max, sum), over n_t threads.
+__device__ inline void write_probs(const float *x, size_t lo, size_t hi, int t, int n_t, float c,
+                                   MaxSum a, float *out) {
+    const bool none = a.m == -INFINITY && a.l == 0.0f;  // every logit -inf
+    const float inv = a.m == INFINITY ? NAN : 1.0f / a.l;
+    for (size_t i = lo + 4 * (size_t)t; i < hi; i += 4 * (size_t)n_t) {
+        if (i + 4 <= hi) {
+            const float4u w = *reinterpret_cast<const float4u *>(x + i);
+            float4u p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = none ? 0.0f : exp_scaled(w[j] - a.m, c) * inv;
+            *reinterpret_cast<float4u *>(out + i) = p;
+        } else {
+            for (size_t j = i; j < hi; ++j)
+                out[j] = none ? 0.0f : exp_scaled(x[j] - a.m, c) * inv;
+        }
     }
-    if (threadIdx.x % kWave == 0) {
-        s_m[threadIdx.x / kWave] = m;
-        s_l[threadIdx.x / kWave] = l;
+}
+
+constexpr int kMaxParts = 64;
+__device__ inline MaxSum join_parts(const MaxSum *p, int parts, float c) {
+    MaxSum a = p[0];
+    for (int i = 1; i < parts; ++i) a = join(a, p[i], c);
+    return a;
+}
+
+__global__ __launch_bounds__(1024) void k_softmax_row(const float *x, size_t n, size_t xs, float c,
+                                                      size_t len, int parts, float *out,
+                                                      size_t os) {
+    __shared__ MaxSum s_ms[4][4], s_part[kMaxParts];
+    const float *row = x + (size_t)blockIdx.x * xs;
+    const int sub = threadIdx.x / kPartThreads, t = threadIdx.x % kPartThreads;
+    for (int i0 = 0; i0 < parts; i0 += 4) {
+        const int i = i0 + sub;
+        const size_t lo = min(n, i * len), hi = min(n, lo + len);
+        const MaxSum a = part_stats(row, lo, hi, t, c, s_ms[sub]);
+        if (t == 0 && i < parts) s_part[i] = a;
     }
     __syncthreads();
-    m = s_m[0];
-    for (int w = 1; w < NT / kWave; ++w) m = fmaxf(m, s_m[w]);
-    l = 0.0f;
-    for (int w = 0; w < NT / kWave; ++w)
-        l = l + (s_m[w] == m ? s_l[w] : s_l[w] * exp_scaled(s_m[w] - m, c));
-    const bool none = m == -INFINITY && l == 0.0f;  // every logit -inf
-    const float inv = m == INFINITY ? NAN : 1.0f / l;
-    for (size_t i = threadIdx.x; i < n; i += NT)
-        orow[i] = none ? 0.0f : exp_scaled(row[i] - m, c) * inv;
+    write_probs(row, 0, n, threadIdx.x, 1024, c, join_parts(s_part, parts, c),
+                out + (size_t)blockIdx.x * os);
+}
+
+__global__ __launch_bounds__(kPartThreads) void k_softmax_stats(const float *__restrict__ x,
+                                                                size_t n, size_t xs, float c,
+                                                                size_t len, int parts,
+                                                                MaxSum *__restrict__ ws) {
+    __shared__ MaxSum s_ms[4];
+    const size_t row = blockIdx.x / parts, lo = blockIdx.x % parts * len;
+    const MaxSum a = part_stats(x + row * xs, lo, min(n, lo + len), threadIdx.x, c, s_ms);
+    if (threadIdx.x == 0) ws[blockIdx.x] = a;
+}
+
+__global__ __launch_bounds__(kPartThreads) void k_softmax_write(const float *x, size_t n,
+                                                                size_t xs, float c, size_t len,
+                                                                int parts,
+                                                                const MaxSum *__restrict__ ws,
+                                                                float *out, size_t os) {
+    __shared__ MaxSum s_part[kMaxParts];
+    const size_t row = blockIdx.x / parts, lo = blockIdx.x % parts * len;
+    if ((int)threadIdx.x < parts) s_part[threadIdx.x] = ws[row * parts + threadIdx.x];
+    __syncthreads();
+    write_probs(x + row * xs, lo, min(n, lo + len), threadIdx.x, kPartThreads, c,
+                join_parts(s_part, parts, c), out + row * os);
 }
 
 // ---- verification of drafted tokens ----------------------------------------------
 // One workgroup a sequence.  The acceptance tests are products of two floats
-// in f64, which are exact.  The drawn token is found by halving: the waves sum
-// contiguous sixteenths of a range (f64), the one in which the cumulative
-// sum passes the target is the next range, down to one wave's width.
+// in f64, which are exact.  The row that the token is drawn from is summed in f64 by
+// chunks, a chunk a wave at a time, sixteen values a lane in flight; the chunk in
+// which the cumulative sum passes the target is read again, a value a thread, until
+// it is no longer than the workgroup.
 struct Residual {
     const float *p, *q;  // q null: nothing is taken away, or 1 at `hot`
     size_t hot;
+    __device__ static double pos(double r) { return r > 0.0 ? r : 0.0; }  // (NaN: 0)
     __device__ double operator()(size_t i) const {
         double r = (double)p[i];
         if (q) r = r - (double)q[i];
         else if (i == hot) r = r - 1.0;
-        return r > 0.0 ? r : 0.0;  // (NaN: 0)
+        return pos(r);
     }
 };
 
-constexpr int kVerWaves = 16;
+constexpr int kVerWaves = 16, kVerThreads = kVerWaves * kWave, kVerChunks = 128;
 
 __device__ inline double wave_sum_f64(double v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
     return v;
 }
-
-// The sums of the sixteen parts of [lo, hi), `part` elements each, in s_sum.
-__device__ inline void part_sums(const Residual &r, size_t lo, size_t hi, size_t part,
-                                 double *s_sum) {
-    const int lane = threadIdx.x % kWave, wv = threadIdx.x / kWave;
-    const size_t a = min(lo + (size_t)wv * part, hi), b = min(a + part, hi);
-    double s = 0.0;
-    for (size_t i = a + lane; i < b; i += kWave) s += r(i);
-    s = wave_sum_f64(s);
-    __syncthreads();
-    if (lane == 0) s_sum[wv] = s;
-    __syncthreads();
+// The first lane at which base and the lanes' values so far exceed the goal, or the
+// last one with a value; base becomes the sum before it.
+__device__ inline int find_lane(double v, double goal, double *base) {
+    const int lane = threadIdx.x % kWave;
+    double c = v;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const double y = __shfl_up(c, o, kWave);
+        if (lane >= o) c += y;
+    }
+    const unsigned long long mass = __ballot(v > 0.0),
+                             over = __ballot(v > 0.0 && *base + c > goal);
+    const int l = over ? __ffsll((long long)over) - 1 : mass ? 63 - __clzll((long long)mass) : 0;
+    const double before = __shfl(c, max(l - 1, 0), kWave);
+    if (l > 0) *base += before;
+    return l;
 }
 
-__global__ __launch_bounds__(kVerWaves *kWave) void k_verify(
+// A lane's share of the sum over [lo, hi), 4 values at 4 (lane + 64 u).
+template <bool Q>
+__device__ inline double lane_sum(const Residual &r, size_t lo, size_t hi, int lane) {
+    constexpr int U = 4;
+    double s = 0.0;
+    size_t i0 = lo;
+    for (; i0 + 4 * U * kWave <= hi; i0 += 4 * U * kWave) {
+        float4u p[U], q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t i = i0 + 4 * (u * kWave + lane);
+            p[u] = *reinterpret_cast<const float4u *>(r.p + i);
+            if (Q) q[u] = *reinterpret_cast<const float4u *>(r.q + i);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                double v = (double)p[u][j];
+                if (Q) v = v - (double)q[u][j];
+                else if (i0 + 4 * (u * kWave + lane) + j == r.hot) v = v - 1.0;
+                s += Residual::pos(v);
+            }
+    }
+    for (size_t i = i0 + lane; i < hi; i += kWave) s += r(i);
+    return s;
+}
+
+__global__ __launch_bounds__(kVerThreads) void k_verify(
     const uint32_t *__restrict__ drafts, const float *__restrict__ dp,
     const float *__restrict__ tp, const float *__restrict__ us,
     const uint32_t *__restrict__ n_drafts, unsigned k, size_t n, uint32_t *__restrict__ tokens,
     uint32_t *__restrict__ accepted) {
-    __shared__ double s_sum[kVerWaves];
+    __shared__ double s_sum[kVerChunks];
     __shared__ unsigned s_first, s_tok;
+    const int lane = threadIdx.x % kWave, wv = threadIdx.x / kWave;
     const size_t b = blockIdx.x;
     const unsigned count = n_drafts ? min(n_drafts[b], k) : k;
     const uint32_t *x = drafts + b * k;
@@ -111,7 +227,7 @@ __global__ __launch_bounds__(kVerWaves *kWave) void k_verify(
         s_tok = MRI_NO_TOKEN;
     }
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < count; i += kVerWaves * kWave) {
+    for (unsigned i = threadIdx.x; i < count; i += kVerThreads) {
         const size_t t = x[i];
         bool ok = t < n;
         if (ok) {
@@ -127,61 +243,59 @@ __global__ __launch_bounds__(kVerWaves *kWave) void k_verify(
         if (dp) r.q = dp + (b * k + a) * n;
         else r.hot = x[a];
     }
-    auto part_of = [](size_t len) {
-        return ((len + kVerWaves - 1) / kVerWaves + kWave - 1) / kWave * kWave;
+    // the sums of the chunks of [lo, hi), `len` values each (whole 1024s: a wave's
+    // loads of sixteen a lane), zeros past them; all waves return their total
+    size_t lo = 0, hi = n, len = 0;
+    auto sums = [&]() {
+        len = ((hi - lo + kVerChunks - 1) / kVerChunks + kVerThreads - 1) / kVerThreads *
+              kVerThreads;
+        __syncthreads();
+        for (int c = wv; c < kVerChunks; c += kVerWaves) {
+            const size_t l0 = min(lo + c * len, hi), l1 = min(l0 + len, hi);
+            double s = 0.0;
+            if (l0 < l1)
+                s = wave_sum_f64(r.q ? lane_sum<true>(r, l0, l1, lane)
+                                     : lane_sum<false>(r, l0, l1, lane));
+            if (lane == 0) s_sum[c] = s;
+        }
+        __syncthreads();
+        return wave_sum_f64(s_sum[2 * lane] + s_sum[2 * lane + 1]);
     };
-    size_t lo = 0, hi = n, part = part_of(n);
-    auto total_of = [&]() {
-        part_sums(r, lo, hi, part, s_sum);
-        double t = 0.0;
-        for (int w = 0; w < kVerWaves; ++w) t += s_sum[w];
-        return t;
-    };
-    double total = total_of();
+    double total = sums();
     if (a < count && !(total > 0.0)) {  // the draft covers the target: draw from the target
         r.q = nullptr;
         r.hot = n;
-        total = total_of();
+        total = sums();
     }
     if (total > 0.0) {
         const double goal = (double)u[k] * total;
         double base = 0.0;
         for (;;) {
-            // the first part in which the sum passes the goal, else the last with mass
-            int at = 0;
-            double before = base, run = base;
-            for (int w = 0; w < kVerWaves; ++w) {
-                if (s_sum[w] > 0.0) {
-                    at = w;
-                    before = run;
-                    run += s_sum[w];
-                    if (run > goal) break;
-                }
-            }
-            base = before;
-            lo = lo + (size_t)at * part;
-            hi = min(lo + part, hi);
-            if (hi - lo <= kWave) break;
-            part = part_of(hi - lo);
-            part_sums(r, lo, hi, part, s_sum);
+            const double c0 = s_sum[2 * lane], c1 = s_sum[2 * lane + 1];
+            const int l = find_lane(c0 + c1, goal, &base);
+            const double f0 = __shfl(c0, l, kWave), f1 = __shfl(c1, l, kWave);
+            const bool second = f1 > 0.0 && !(f0 > 0.0 && base + f0 > goal);
+            if (second) base += f0;
+            lo = lo + (size_t)(2 * l + second) * len;
+            hi = min(lo + len, hi);
+            if (hi - lo <= kVerThreads) break;
+            (void)sums();
         }
-        if (threadIdx.x < kWave) {
-            const size_t i = lo + threadIdx.x;
-            const double v = i < hi ? r(i) : 0.0;
-            double c = v;
-#pragma unroll
-            for (int o = 1; o < kWave; o <<= 1) {
-                const double y = __shfl_up(c, o, kWave);
-                if ((int)threadIdx.x >= o) c += y;
-            }
-            const unsigned long long mass = __ballot(v > 0.0),
-                                     over = __ballot(v > 0.0 && base + c > goal);
-            const int lane = over ? __ffsll((long long)over) - 1 : 63 - __clzll((long long)mass);
-            if (threadIdx.x == 0) s_tok = (unsigned)(lo + lane);
+        // a value a thread: the wave that passes the goal, then its lane
+        const size_t i = lo + threadIdx.x;
+        const double v = i < hi ? r(i) : 0.0;
+        const double w = wave_sum_f64(v);
+        __syncthreads();
+        if (lane == 0) s_sum[wv] = w;
+        __syncthreads();
+        const int at = find_lane(lane < kVerWaves ? s_sum[lane] : 0.0, goal, &base);
+        if (wv == at) {
+            const int l = find_lane(v, goal, &base);
+            if (lane == 0) s_tok = (unsigned)(lo + wv * kWave + l);
         }
     }
     __syncthreads();
-    for (unsigned i = threadIdx.x; i <= k; i += kVerWaves * kWave)
+    for (unsigned i = threadIdx.x; i <= k; i += kVerThreads)
         tokens[b * (k + 1) + i] = i < a ? x[i] : i == a ? s_tok : MRI_NO_TOKEN;
     if (threadIdx.x == 0) accepted[b] = a;
 }
@@ -192,9 +306,35 @@ mri_status launch_softmax(const float *x, size_t rows, size_t n, size_t x_stride
                           float temperature, float *out, size_t out_stride, hipStream_t s) {
     if (!rows) return MRI_OK;
     const float c = (float)fmin(1.4426950408889634074 / (double)temperature, (double)FLT_MAX);
-    hipLaunchKernelGGL(k_softmax<1024>, dim3((unsigned)rows), dim3(1024), 0, s, x, n, x_stride, c,
-                       out, out_stride);
-    MRI_LAUNCHED("k_softmax");
+    // parts of 4096 values at least, 64 of them at most
+    const size_t len = round_up(std::max<size_t>((n + kMaxParts - 1) / kMaxParts, 4096), 4);
+    const size_t parts = (n + len - 1) / len;
+    // Rows in parts where whole rows leave CUs idle.  The parts' workspace is the
+    // stream's: a call that is being captured uses none, so that graphs recorded on one
+    // stream may run side by side.
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (parts > 1 && rows < 4 * (size_t)std::max(device_cus(), 1)) {
+        MRI_HIP(hipStreamIsCapturing(s, &capture));
+        void *ws = nullptr;
+        if (capture == hipStreamCaptureStatusNone) {
+            const mri_status st = softmax_ws_get(s, &ws);
+            if (st) return st;
+        }
+        if (ws && rows * parts * sizeof(MaxSum) <= kSoftmaxWsBytes) {
+            hipLaunchKernelGGL(k_softmax_stats, dim3((unsigned)(rows * parts)),
+                               dim3(kPartThreads), 0, s, x, n, x_stride, c, len, (int)parts,
+                               static_cast<MaxSum *>(ws));
+            MRI_LAUNCHED("k_softmax_stats");
+            hipLaunchKernelGGL(k_softmax_write, dim3((unsigned)(rows * parts)),
+                               dim3(kPartThreads), 0, s, x, n, x_stride, c, len, (int)parts,
+                               static_cast<const MaxSum *>(ws), out, out_stride);
+            MRI_LAUNCHED("k_softmax_write");
+            return MRI_OK;
+        }
+    }
+    hipLaunchKernelGGL(k_softmax_row, dim3((unsigned)rows), dim3(1024), 0, s, x, n, x_stride, c,
+                       len, (int)parts, out, out_stride);
+    MRI_LAUNCHED("k_softmax_row");
     return MRI_OK;
 }
 
@@ -203,7 +343,7 @@ mri_status launch_verify(const uint32_t *drafts, const float *draft_probs,
                          const uint32_t *n_drafts, size_t n_seqs, size_t k, size_t n,
                          uint32_t *tokens, uint32_t *accepted, hipStream_t s) {
     if (!n_seqs) return MRI_OK;
-    hipLaunchKernelGGL(k_verify, dim3((unsigned)n_seqs), dim3(kVerWaves * kWave), 0, s, drafts,
+    hipLaunchKernelGGL(k_verify, dim3((unsigned)n_seqs), dim3(kVerThreads), 0, s, drafts,
                        draft_probs, target_probs, uniforms, n_drafts, (unsigned)k, n, tokens,
                        accepted);
     MRI_LAUNCHED("k_verify");
