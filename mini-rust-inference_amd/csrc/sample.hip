@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kPartThreads) void k_softmax_write(const float *x, 
 // ---- verification of drafted tokens ----------------------------------------------
 // One workgroup a sequence.  The acceptance tests are products of two floats
 // in f64, which are exact.  The row that the token is drawn from is summed in f64 by
-// chunks, a chunk a wave at a time, sixteen values a lane in flight; the chunk in
+// chunks, a chunk a wave at a time, eight values a lane in flight; the chunk in
 // which the cumulative sum passes the target is read again, a value a thread, until
 // it is no longer than the workgroup.
 struct Residual {
@@ -185,7 +185,7 @@ __device__ inline int find_lane(double v, double goal, double *base) {
 // A lane's share of the sum over [lo, hi), 4 values at 4 (lane + 64 u).
 template <bool Q>
 __device__ inline double lane_sum(const Residual &r, size_t lo, size_t hi, int lane) {
-    constexpr int U = 4;
+    constexpr int U = 2;  // (four: registers spill; 64 x 7 of 100003 take 21.3 us, not 20.1)
     double s = 0.0;
     size_t i0 = lo;
     for (; i0 + 4 * U * kWave <= hi; i0 += 4 * U * kWave) {
@@ -243,8 +243,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify(
         if (dp) r.q = dp + (b * k + a) * n;
         else r.hot = x[a];
     }
-    // the sums of the chunks of [lo, hi), `len` values each (whole 1024s: a wave's
-    // loads of sixteen a lane), zeros past them; all waves return their total
+    // the sums of the chunks of [lo, hi), `len` values each (whole 1024s), zeros past them; all waves return their total
     size_t lo = 0, hi = n, len = 0;
     auto sums = [&]() {
         len = ((hi - lo + kVerChunks - 1) / kVerChunks + kVerThreads - 1) / kVerThreads *

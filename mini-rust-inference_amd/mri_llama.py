@@ -110,29 +110,45 @@ def _bad(kind, msg):
     return Q.MriError({"InvalidShape": 1, "InvalidArgument": 3}[kind], msg)
 
 
-def _tensor(t, name, dtype, shape=None):
-    """A device pointer of t after its type, place and (contiguous) shape are checked."""
-    import torch
-    if t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+_torch = None
+
+
+def _device():
+    """The current device (and torch, loaded at the first call)."""
+    global _torch, _F32, _INTS, _raw_stream
+    if _torch is None:
+        import torch
+        _F32, _INTS = (torch.float32,), (torch.int32, torch.uint32)
+        # (3 us a call less than making a Stream object)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+        _torch = torch
+    return _torch.cuda.current_device()
+
+
+def _stream(stream, dev):
+    return _raw_stream(dev) if stream is None else stream
+
+
+def _tensor(t, name, dtypes, dev, shape=None):
+    """The address of t after its type, place and (contiguous) shape are checked."""
+    if t.dtype not in dtypes:
         raise _bad("InvalidArgument", f"{name}: dtype {t.dtype}")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != dev:
         raise _bad("InvalidArgument", f"{name}: on {t.device}, not on the current device")
     if shape is not None:
-        if tuple(t.shape) != tuple(shape):
-            raise _bad("InvalidShape", f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+        if t.shape != shape:
+            raise _bad("InvalidShape", f"{name}: shape {tuple(t.shape)}, expected {shape}")
         if not t.is_contiguous():
             raise _bad("InvalidArgument", f"{name}: not contiguous")
-    return C.c_void_p(t.data_ptr())
-
-
-def _ints():
-    import torch
-    return (torch.int32, torch.uint32)
+    return t.data_ptr()
 
 
 def _row_stride(t, name):
     """Floats between consecutive rows of t [..., rows, features]: the rows of all
     leading indices follow each other at one distance."""
+    if t.is_contiguous():
+        return t.shape[-1]
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise _bad("InvalidArgument", f"{name}: features are not contiguous")
     stride, n = None, 1
@@ -156,73 +172,70 @@ class Kv4Cache:
         h = C.c_void_p()
         Q.check(lib().mri_kv4_cache_create(n_layers, n_seqs, max_seq, n_kv_heads, head_dim,
                                            C.byref(h)))
-        self.h = h
+        self.h, self.lib = h, lib()
         self.n_layers, self.n_seqs, self.max_seq = n_layers, n_seqs, max_seq
         self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
 
     @property
     def device_bytes(self):
-        return lib().mri_kv4_cache_device_bytes(self.h)
+        return self.lib.mri_kv4_cache_device_bytes(self.h)
 
-    def _rows(self, t, start, count, first_seq):
+    def _rows(self, t, start, count, first_seq, dev):
         n_seqs, rows = (1, t.shape[-2]) if t.dim() == 2 else t.shape[-3:-1]
-        r = Kv4Rows(first_seq, n_seqs, rows, 0, None, None)
-        if isinstance(start, int):
-            if start < 0:
-                raise _bad("InvalidShape", f"start {start} is negative")
-            r.start = start
-        else:
-            r.pos = _tensor(start, "start", _ints(), (n_seqs,))
+        pos = None
+        if not isinstance(start, int):
+            pos, start = _tensor(start, "start", _INTS, dev, (n_seqs,)), 0
+        elif start < 0:
+            raise _bad("InvalidShape", f"start {start} is negative")
         if count is not None:
-            r.count = _tensor(count, "count", _ints(), (n_seqs,))
-        return r
+            count = _tensor(count, "count", _INTS, dev, (n_seqs,))
+        return C.byref(Kv4Rows(first_seq, n_seqs, rows, start, pos, count))
 
-    def _kv(self, k, v, dims):
-        import torch
+    def _kv(self, k, v, dims, dev):
         if k.dim() not in dims or k.shape != v.shape or \
                 k.shape[-1] != self.n_kv_heads * self.head_dim:
             raise _bad("InvalidShape", f"k {tuple(k.shape)}, v {tuple(v.shape)}")
         s = _row_stride(k, "k")
         if _row_stride(v, "v") != s:
             raise _bad("InvalidArgument", "k and v differ in their row stride")
-        return _tensor(k, "k", torch.float32), _tensor(v, "v", torch.float32), s
+        return _tensor(k, "k", _F32, dev), _tensor(v, "v", _F32, dev), s
 
     def append(self, layer, k, v, start, count=None, first_seq=0, stream=None):
-        kp, vp, s = self._kv(k, v, (2, 3))
-        r = self._rows(k, start, count, first_seq)
-        Q.check(lib().mri_kv4_append(self.h, layer, C.byref(r), kp, vp, s, Q._stream(stream)))
+        dev = _device()
+        kp, vp, s = self._kv(k, v, (2, 3), dev)
+        Q.check(self.lib.mri_kv4_append(self.h, layer, self._rows(k, start, count, first_seq, dev),
+                                        kp, vp, s, _stream(stream, dev)))
 
     def read(self, layer, k, v, start, count=None, first_seq=0, stream=None):
         """Into k and v; with a fourth leading axis, of that many layers."""
-        kp, vp, s = self._kv(k, v, (2, 3, 4))
-        r = self._rows(k, start, count, first_seq)
-        Q.check(lib().mri_kv4_read(self.h, layer, k.shape[0] if k.dim() == 4 else 1, C.byref(r),
-                                   kp, vp, s, Q._stream(stream)))
+        dev = _device()
+        kp, vp, s = self._kv(k, v, (2, 3, 4), dev)
+        Q.check(self.lib.mri_kv4_read(self.h, layer, k.shape[0] if k.dim() == 4 else 1,
+                                      self._rows(k, start, count, first_seq, dev), kp, vp, s,
+                                      _stream(stream, dev)))
 
     def attend(self, layer, q, out, start, count=None, first_seq=0, weights=None, stream=None):
         """weights: f32 [n_seqs of the cache, n_kv_heads, max_seq] of this layer."""
-        import torch
         if q.dim() not in (2, 3) or q.shape != out.shape or q.shape[-1] % self.head_dim:
             raise _bad("InvalidShape", f"q {tuple(q.shape)}, out {tuple(out.shape)}")
-        qp, op = _tensor(q, "q", torch.float32), _tensor(out, "out", torch.float32)
-        r = self._rows(q, start, count, first_seq)
-        wp = None if weights is None else _tensor(
-            weights, "weights", torch.float32, (self.n_seqs, self.n_kv_heads, self.max_seq))
-        Q.check(lib().mri_kv4_attend(self.h, layer, C.byref(r), qp, _row_stride(q, "q"),
-                                     q.shape[-1] // self.head_dim, op, _row_stride(out, "out"),
-                                     wp, Q._stream(stream)))
+        dev = _device()
+        qp, op = _tensor(q, "q", _F32, dev), _tensor(out, "out", _F32, dev)
+        if weights is not None:
+            weights = _tensor(weights, "weights", _F32, dev,
+                              (self.n_seqs, self.n_kv_heads, self.max_seq))
+        Q.check(self.lib.mri_kv4_attend(self.h, layer, self._rows(q, start, count, first_seq, dev),
+                                        qp, _row_stride(q, "q"), q.shape[-1] // self.head_dim, op,
+                                        _row_stride(out, "out"), weights, _stream(stream, dev)))
 
     def evict(self, dst, weights, weights_out, lens, lens_out, keep, recent, kept, stream=None):
         """Into dst (self: in place, with weights_out = weights)."""
-        import torch
-        lead = (self.n_layers, self.n_seqs, self.n_kv_heads)
-        f = torch.float32
-        Q.check(lib().mri_kv4_evict(
-            self.h, dst.h, _tensor(weights, "weights", f, lead + (self.max_seq,)),
-            _tensor(weights_out, "weights_out", f, lead + (dst.max_seq,)),
-            _tensor(lens, "lens", _ints(), (self.n_seqs,)),
-            _tensor(lens_out, "lens_out", _ints(), (self.n_seqs,)), keep, recent,
-            _tensor(kept, "kept", _ints(), lead + (keep,)), Q._stream(stream)))
+        lead, dev = (self.n_layers, self.n_seqs, self.n_kv_heads), _device()
+        Q.check(self.lib.mri_kv4_evict(
+            self.h, dst.h, _tensor(weights, "weights", _F32, dev, lead + (self.max_seq,)),
+            _tensor(weights_out, "weights_out", _F32, dev, lead + (dst.max_seq,)),
+            _tensor(lens, "lens", _INTS, dev, (self.n_seqs,)),
+            _tensor(lens_out, "lens_out", _INTS, dev, (self.n_seqs,)), keep, recent,
+            _tensor(kept, "kept", _INTS, dev, lead + (keep,)), _stream(stream, dev)))
 
     def close(self):
         if self.h:
@@ -282,10 +295,10 @@ class Llama:
         """cache_pos: start_pos unless keys were evicted.  weights: f32
         [n_layers, n_seqs, n_kv_heads, max_seq] of the cache."""
         import numpy as np
-        import torch
         t = np.ascontiguousarray(tokens, np.uint32)
+        dev = _device()
         wp = None if weights is None else _tensor(
-            weights, "weights", torch.float32,
+            weights, "weights", _F32, dev,
             (cache.n_layers, cache.n_seqs, cache.n_kv_heads, cache.max_seq))
         Q.check(lib().mri_llama_forward_kv4(
             self.h, t.ctypes.data_as(P), t.size, start_pos, cache.h, seq,
@@ -325,13 +338,13 @@ def argmax(v, idx, stream=None):
 
 def softmax(x, out, temperature=1.0, stream=None):
     """Probabilities of rows of logits x [rows, n] (or [n]) into out; may be x."""
-    import torch
     if x.shape != out.shape or x.dim() not in (1, 2):
         raise _bad("InvalidShape", f"x {tuple(x.shape)}, out {tuple(out.shape)}")
-    rows, n = (1, x.numel()) if x.dim() == 1 else tuple(x.shape)
-    xp, op = _tensor(x, "x", torch.float32), _tensor(out, "out", torch.float32)
-    Q.check(lib().mri_softmax(xp, rows, n, _row_stride(x, "x"), temperature, op,
-                              _row_stride(out, "out"), Q._stream(stream)))
+    dev = _device()
+    rows, n = (1, x.numel()) if x.dim() == 1 else x.shape
+    Q.check(lib().mri_softmax(_tensor(x, "x", _F32, dev), rows, n, _row_stride(x, "x"), temperature,
+                              _tensor(out, "out", _F32, dev), _row_stride(out, "out"),
+                              _stream(stream, dev)))
 
 
 def verify_drafts(drafts, target_probs, uniforms, tokens, accepted, draft_probs=None,
@@ -339,16 +352,17 @@ def verify_drafts(drafts, target_probs, uniforms, tokens, accepted, draft_probs=
     """drafts int32 [n_seqs, k], target_probs f32 [n_seqs, k + 1, n], uniforms f32
     [n_seqs, k + 1], draft_probs f32 [n_seqs, k, n], n_drafts int32 [n_seqs]; into
     tokens int32 [n_seqs, k + 1] and accepted int32 [n_seqs]."""
-    import torch
     if drafts.dim() != 2 or target_probs.dim() != 3:
         raise _bad("InvalidShape",
                    f"drafts {tuple(drafts.shape)}, target_probs {tuple(target_probs.shape)}")
-    (b, k), n, f = drafts.shape, target_probs.shape[2], torch.float32
-    dp = None if draft_probs is None else _tensor(draft_probs, "draft_probs", f, (b, k, n))
-    nd = None if n_drafts is None else _tensor(n_drafts, "n_drafts", _ints(), (b,))
+    (b, k), n, dev = drafts.shape, target_probs.shape[2], _device()
+    if draft_probs is not None:
+        draft_probs = _tensor(draft_probs, "draft_probs", _F32, dev, (b, k, n))
+    if n_drafts is not None:
+        n_drafts = _tensor(n_drafts, "n_drafts", _INTS, dev, (b,))
     Q.check(lib().mri_verify_drafts(
-        _tensor(drafts, "drafts", _ints(), (b, k)), dp,
-        _tensor(target_probs, "target_probs", f, (b, k + 1, n)),
-        _tensor(uniforms, "uniforms", f, (b, k + 1)), nd, b, k, n,
-        _tensor(tokens, "tokens", _ints(), (b, k + 1)),
-        _tensor(accepted, "accepted", _ints(), (b,)), Q._stream(stream)))
+        _tensor(drafts, "drafts", _INTS, dev, (b, k)), draft_probs,
+        _tensor(target_probs, "target_probs", _F32, dev, (b, k + 1, n)),
+        _tensor(uniforms, "uniforms", _F32, dev, (b, k + 1)), n_drafts, b, k, n,
+        _tensor(tokens, "tokens", _INTS, dev, (b, k + 1)),
+        _tensor(accepted, "accepted", _INTS, dev, (b,)), _stream(stream, dev)))
