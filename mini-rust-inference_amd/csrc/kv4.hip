@@ -11,9 +11,17 @@ namespace {
 
 constexpr int kWave = 64;
 
+// What all lanes of a wave agree on, in a scalar register.
+template <class T>
+__device__ inline T uniform(T v) {
+    return (T)__builtin_amdgcn_readfirstlane((int)v);
+}
+__device__ inline int wave_id() { return uniform((int)threadIdx.x >> 6); }
+
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
 
 template <int HD>
 struct Page {
@@ -732,6 +740,8 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     if constexpr (SPLIT) {
         // two pages a wave cost less than another workgroup's partial results
         run = find_run(a, slots, slot, 2 * kWaves);
+        run = Run{uniform(run.b), uniform(run.first), uniform(run.n), uniform(run.pg0),
+                  uniform(run.pg1)};
         if (run.b < 0) return;
     }
     const int b = run.b;
@@ -937,7 +947,7 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
     using P = Page<HD>;
     constexpr int QW = kPromptWaves * 16;  // queries of a workgroup
     __shared__ LdsPage<HD> s_p[2];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    const int lane = threadIdx.x & 63, wv = wave_id(), g = lane >> 4, r = lane & 15;
     unsigned x = blockIdx.x;
     const int head = x % a.n_kv;
     x /= a.n_kv;
@@ -1015,7 +1025,7 @@ __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
     __shared__ __attribute__((aligned(16))) unsigned s_d[kWtWaves][kScaleWords<HD>];
     __shared__ float s_w[kWtWaves][kPageKeys];
     __shared__ int s_last;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    const int lane = threadIdx.x & 63, wv = wave_id(), g = lane >> 4, r = lane & 15;
     unsigned x = blockIdx.x;
     const int mine = x % n_parts;
     x /= n_parts;
@@ -1183,7 +1193,7 @@ __global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
     __shared__ unsigned s_hist[kSelBins];
     __shared__ unsigned s_wave[kSelWaves], s_digit, s_left;
     __shared__ unsigned s_gt[kSelWaves], s_eq[kSelWaves];
-    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    const int t = threadIdx.x, lane = t & 63, wv = wave_id();
     const size_t rowi = blockIdx.x;
     const int b = (int)(rowi / e.n_kv % e.n_seqs);
     const unsigned n = min(e.lens[b], e.src_max);
@@ -1239,8 +1249,9 @@ __global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
         const unsigned inc = wave_scan_u(c0 + c1);
         if (lane == kWave - 1) s_wave[wv] = inc;
         __syncthreads();
-        unsigned above = inc - c0 - c1;
-        for (int u = 0; u < wv; ++u) above += s_wave[u];
+        const unsigned ends = wave_scan_u(lane < kSelWaves ? s_wave[lane] : 0);
+        const unsigned above =
+            inc - c0 - c1 + (wv ? __builtin_amdgcn_readlane(ends, wv - 1) : 0);
         if (above < left && left <= above + c0) {
             s_digit = kSelBins - 1 - 2 * t;
             s_left = left - above;
@@ -1264,11 +1275,10 @@ __global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
         s_eq[wv] = eq;
     }
     __syncthreads();
-    gt = eq = 0;
-    for (int u = 0; u < wv; ++u) {
-        gt += s_gt[u];
-        eq += s_eq[u];
-    }
+    gt = wave_scan_u(lane < kSelWaves ? s_gt[lane] : 0);
+    eq = wave_scan_u(lane < kSelWaves ? s_eq[lane] : 0);
+    gt = wv ? __builtin_amdgcn_readlane(gt, wv - 1) : 0;
+    eq = wv ? __builtin_amdgcn_readlane(eq, wv - 1) : 0;
     const unsigned long long below = (1ull << lane) - 1;
     each([&](unsigned key, unsigned i, bool ok) {
         const unsigned long long bg = __ballot(ok && key > prefix),
@@ -1285,12 +1295,20 @@ __global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
 // page by page.  In place one workgroup walks the pages in order: a page's
 // sources lie at it or behind it, so only a page's own loads have to end
 // before its stores begin.  Into another cache every page has a workgroup.
+// A thread makes the 16 bytes of one lane of a K tile (a key's, moved whole) and
+// of a V chunk: two dims and both key halves, a nibble each of the sixteen keys of
+// its lane group, taken from the sixteen bytes that hold it.  Where a page's keys come
+// from a few pages, as they do while little is dropped, those pages' values are
+// staged in LDS (2304 keys of 256 heads to 2048: 61 us; 107 with a load a nibble
+// from global memory).
+constexpr int kMovePages = 3;
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_move(Kv4Evict e, int per_row) {
     using P = Page<HD>;
-    constexpr int NB = P::NB, KD = 8 * HD / 256, SD = (128 * NB + 255) / 256;
-    __shared__ unsigned s_i[kPageKeys];
-    const int t = threadIdx.x;
+    constexpr int NB = P::NB, VB = 32 * HD, SD = (128 * NB + 255) / 256;
+    __shared__ unsigned s_i[kPageKeys], s_pg[kPageKeys], s_d[kPageKeys];
+    __shared__ uint4_t s_v[kMovePages * VB / 16];
+    const int t = threadIdx.x, lane = t & 63, wv = wave_id(), g = lane >> 4, r = lane & 15;
     const size_t rowi = blockIdx.x / per_row;
     const int b = (int)(rowi / e.n_kv % e.n_seqs);
     if (rowi < (size_t)e.n_seqs * e.n_kv && rowi % e.n_kv == 0 && blockIdx.x % per_row == 0 &&
@@ -1306,77 +1324,102 @@ __global__ __launch_bounds__(256) void k_kv4_move(Kv4Evict e, int per_row) {
     for (unsigned pg = blockIdx.x % per_row; pg < n_pg; pg += per_row) {
         const unsigned key0 = pg * kPageKeys;
         __syncthreads();  // the previous page's indexes are read, its stores issued
-        if (t < kPageKeys) s_i[t] = key0 + t < e.keep ? kept[key0 + t] : MRI_NO_TOKEN;
+        if (t < kPageKeys) {
+            const unsigned i = key0 + t < e.keep ? kept[key0 + t] : MRI_NO_TOKEN;
+            int sg, sh, sj;
+            P::v_place(i % kPageKeys, &sg, &sh, &sj);
+            s_i[t] = i;
+            s_pg[t] = i / kPageKeys;
+            s_d[t] = sg * 256 | sh << 5 | 4 * nibble_of(sj);  // lane group's bytes, half, shift
+        }
         __syncthreads();
         if (s_i[0] == MRI_NO_TOKEN) return;  // (the kept ones come first)
-        if (in_place && (s_i[kPageKeys - 1] == key0 + kPageKeys - 1)) continue;  // all in place
-        unsigned kq[KD], vq[KD], vm[KD], sc[SD];
-        float wt = 0.0f;
-#pragma unroll
-        for (int u = 0; u < KD; ++u) {
-            const int x = t + 256 * u;
-            const int tile = x / (64 * NB), l = (x / NB) & 63, blk = x % NB;
-            const unsigned i = s_i[16 * tile + (l & 15)];
-            kq[u] = 0;
-            if (i != MRI_NO_TOKEN)
-                kq[u] = *reinterpret_cast<const unsigned *>(
-                    src + (size_t)(i / kPageKeys) * P::kBytes +
-                    P::k_dword(i % kPageKeys, l >> 4, blk));
+        if (in_place && s_i[kPageKeys - 1] == key0 + kPageKeys - 1) continue;  // all in place
+        const int n = __popcll(__ballot(s_i[lane] != MRI_NO_TOKEN));  // keys of the page
+        const unsigned from = s_pg[0], n_src = s_pg[n - 1] - from + 1;
+        const bool staged = n_src <= kMovePages;
+        if (staged) {
+            for (unsigned x = t; x < n_src * (VB / 16); x += 256)
+                s_v[x] = *reinterpret_cast<const uint4_t *>(
+                    src + (size_t)(from + x / (VB / 16)) * P::kBytes + P::kV + x % (VB / 16) * 16);
         }
+        // K: 16 (or 8) bytes of key 16 wv + r
+        unsigned kq[NB];
+        const int kkey = 16 * wv + r;
+        if (kkey < n) {
+            const unsigned *p = reinterpret_cast<const unsigned *>(
+                src + (size_t)s_pg[kkey] * P::kBytes +
+                P::k_dword(s_i[kkey] % kPageKeys, g, 0));
 #pragma unroll
-        for (int u = 0; u < KD; ++u) {
-            const int x = t + 256 * u;
-            const int l = (x >> 2) & 63, dim = 16 * (2 * (x >> 8) + ((x >> 1) & 1)) + (l & 15);
-            vq[u] = vm[u] = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const unsigned i = s_i[P::v_key(l >> 4, x & 1, j)];
-                if (i == MRI_NO_TOKEN) continue;
-                int sg, sh, sj;
-                P::v_place(i % kPageKeys, &sg, &sh, &sj);
-                const unsigned d = *reinterpret_cast<const unsigned *>(
-                    src + (size_t)(i / kPageKeys) * P::kBytes + P::v_dword(dim, sg, sh));
-                vq[u] |= (d >> (4 * nibble_of(sj)) & 0xfu) << (4 * nibble_of(j));
-                vm[u] |= 0xfu << (4 * nibble_of(j));
-            }
+            for (int u = 0; u < NB; ++u) kq[u] = p[u];
         }
+        unsigned sc[SD];
 #pragma unroll
         for (int u = 0; u < SD; ++u) {
             const int x = t + 256 * u, which = x >= 64 * NB, rest = x % (64 * NB);
             sc[u] = 0;
-            const unsigned i = s_i[rest / NB];
-            if (x < 128 * NB && i != MRI_NO_TOKEN)
+            if (x < 128 * NB && rest / NB < n)
                 sc[u] = *reinterpret_cast<const uint16_t *>(
-                    src + (size_t)(i / kPageKeys) * P::kBytes + (which ? P::kVs : P::kKs) +
-                    P::scale(i % kPageKeys, rest % NB));
+                    src + (size_t)s_pg[rest / NB] * P::kBytes + (which ? P::kVs : P::kKs) +
+                    P::scale(s_i[rest / NB] % kPageKeys, rest % NB));
         }
-        if (t < kPageKeys && s_i[t] != MRI_NO_TOKEN) wt = w[s_i[t]];
+        float wt = 0.0f;
+        if (t < n) wt = w[s_i[t]];
+        __syncthreads();  // the staged values
+        // V: chunk wv
+        unsigned vq[4] = {0, 0, 0, 0}, vm[2] = {0, 0};
         uint8_t *pb = dst + (size_t)pg * P::kBytes;
-        unsigned old[KD];
+        uint4_t *vto = reinterpret_cast<uint4_t *>(pb + P::kV + wv * 1024 + lane * 16);
+        uint4_t old = {0, 0, 0, 0};
+        auto gather = [&](auto st) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < KD; ++u) {
-            old[u] = 0;
-            if (vm[u] != 0xffffffffu && vm[u])
-                old[u] = *reinterpret_cast<const unsigned *>(pb + P::kV + 4 * (t + 256 * u));
+            for (int h = 0; h < 2; ++h) {
+                uint4_t x[8];
+                unsigned d[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int key = P::v_key(g, h, j), k0 = min(key, n - 1);
+                    d[j] = s_d[k0];
+                    const unsigned at = (d[j] & ~63u) + wv * 1024 + r * 16;
+                    if constexpr (decltype(st)::value)
+                        x[j] = s_v[(s_pg[k0] - from) * (VB / 16) + at / 16];
+                    else
+                        x[j] = *reinterpret_cast<const uint4_t *>(
+                            src + (size_t)s_pg[k0] * P::kBytes + P::kV + at);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int sh = d[j] & 31, to = 4 * nibble_of(j);
+                    const bool hi = d[j] & 32, in = P::v_key(g, h, j) < n;
+                    vq[h] |= ((hi ? x[j].y : x[j].x) >> sh & 0xfu) << to;
+                    vq[2 + h] |= ((hi ? x[j].w : x[j].z) >> sh & 0xfu) << to;
+                    vm[h] |= (in ? 0xfu : 0u) << to;
+                }
+            }
+        };
+        if (wv < NB) {
+            if (staged) gather(std::true_type{});
+            else gather(std::false_type{});
+            if (n < kPageKeys) old = *vto;
         }
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's loads have ended
         __syncthreads();
+        if (kkey < n) {
+            unsigned *p = reinterpret_cast<unsigned *>(pb + P::k_dword(kkey, g, 0));
 #pragma unroll
-        for (int u = 0; u < KD; ++u) {
-            const int x = t + 256 * u;
-            if (s_i[16 * (x / (64 * NB)) + ((x / NB) & 15)] != MRI_NO_TOKEN)
-                *reinterpret_cast<unsigned *>(pb + 4 * x) = kq[u];
-            if (vm[u])
-                *reinterpret_cast<unsigned *>(pb + P::kV + 4 * x) = (old[u] & ~vm[u]) | vq[u];
+            for (int u = 0; u < NB; ++u) p[u] = kq[u];
         }
+        if (wv < NB && (vm[0] | vm[1]))
+            *vto = uint4_t{(old.x & ~vm[0]) | (vq[0] & vm[0]), (old.y & ~vm[1]) | (vq[1] & vm[1]),
+                           (old.z & ~vm[0]) | (vq[2] & vm[0]), (old.w & ~vm[1]) | (vq[3] & vm[1])};
 #pragma unroll
         for (int u = 0; u < SD; ++u) {
             const int x = t + 256 * u, which = x >= 64 * NB, rest = x % (64 * NB);
-            if (x < 128 * NB && s_i[rest / NB] != MRI_NO_TOKEN)
+            if (x < 128 * NB && rest / NB < n)
                 *reinterpret_cast<uint16_t *>(pb + (which ? P::kVs : P::kKs) +
                                               P::scale(rest / NB, rest % NB)) = (uint16_t)sc[u];
         }
-        if (t < kPageKeys && s_i[t] != MRI_NO_TOKEN) wo[key0 + t] = wt;
+        if (t < n) wo[key0 + t] = wt;
     }
 }
 
