@@ -323,6 +323,15 @@ __device__ inline float block_max(float v) {
     return v;
 }
 
+__device__ inline float quad_max(float v) {  // over four neighbouring lanes
+    const auto swap = [](float x, auto perm) __attribute__((always_inline)) {
+        return __uint_as_float(__builtin_amdgcn_update_dpp(
+            0, __float_as_uint(x), decltype(perm)::value, 0xf, 0xf, true));
+    };
+    v = fmaxf(v, swap(v, std::integral_constant<int, 0xb1>{}));  // lanes 1, 0, 3, 2
+    return fmaxf(v, swap(v, std::integral_constant<int, 0x4e>{}));  // lanes 2, 3, 0, 1
+}
+
 // A tile's columns are 16 queries; with FEW they are 16 / NB queries times the NB
 // blocks of the head dim, column b * 16 / NB + query.  Such a column holds its own
 // block of the query only, so the products with all of K's blocks leave its block's
@@ -330,14 +339,13 @@ __device__ inline float block_max(float v) {
 // probabilities need the scales of its own block only, a quarter of the work at head
 // dim 128, and its sums count for that block's dims.
 //
-// What lane (g, r) loads of a tile: dims 8 g .. of the blocks of column r.
+// What a lane loads of a tile: dims 8 g .. of a column's blocks (FEW: of block own).
 template <int HD, bool FEW>
 struct QRaw {
     static constexpr int NB = HD / 32, NQ = FEW ? 16 / NB : 16, N = FEW ? 1 : NB;
     float x[N][8];
     // src null: an empty column; vec: 16-byte loads are aligned
-    __device__ void load(const float *src, int lane, bool vec) {
-        const int g = lane >> 4, own = (lane & 15) / NQ;
+    __device__ void load(const float *src, int g, int own, bool vec) {
 #pragma unroll
         for (int b = 0; b < N; ++b) {
             const float *p = src + 32 * (FEW ? own : b) + 8 * g;
@@ -360,13 +368,15 @@ struct QTile {
     static constexpr int NB = HD / 32, NQ = R::NQ, N = R::N;
     half8_t hi[NB], lo[NB];
     float inv;  // what the raw products are multiplied by (log2 units)
+    // QUAD: a column's four lanes are neighbours
+    template <bool QUAD = false>
     __device__ void make(const R &raw, int lane) {
         float mx = 0.0f;
 #pragma unroll
         for (int b = 0; b < N; ++b)
 #pragma unroll
             for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(raw.x[b][j]));
-        mx = col_max(mx);
+        mx = QUAD ? quad_max(mx) : col_max(mx);
         if constexpr (FEW) mx = block_max<NB>(mx);
         // the row's largest magnitude to [2^14, 2^15)
         const int e = mx > 0.0f && mx < INFINITY ? min(14 - ilogbf(mx), 120) : 0;
@@ -763,7 +773,7 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     const bool real = qi < n_q;
     QRaw<HD, FEW> raw;
     raw.load(real ? q + row_index(a, b, row) * qs + (head * groups + qi % groups) * HD : nullptr,
-             lane, vec);
+             g, r / NQ, vec);
     QTile<HD, FEW> qtile;
     qtile.make(raw, lane);
     const long see = real ? (long)p0 + row + 1 : 0;      // keys this column sees
@@ -967,7 +977,7 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
     QTile<HD, false> qtile;
     {
         QRaw<HD, false> raw;
-        raw.load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, lane, vec);
+        raw.load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, g, 0, vec);
         qtile.make(raw, lane);
     }
     const long see = real ? (long)p0 + row + 1 : 0;  // keys this column sees
@@ -1061,11 +1071,13 @@ __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
     QRaw<HD, false> raw;
     float z_next = 0.0f;
     unsigned see_next = 0;
+    // (a column's four lanes are neighbours here, for whole lines a load)
+    const int fr = lane >> 2, fg = lane & 3;
     auto fetch = [&](int t) {
-        const int qi = t * 16 + r, row = qi / groups;
+        const int qi = t * 16 + fr, row = qi / groups;
         const bool real = qi < n_q;
         const int qh = head * groups + qi % groups;
-        raw.load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, lane, vec);
+        raw.load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, fg, 0, vec);
         see_next = real ? p0 + row + 1 : 0;
         z_next = real ? lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] : 0.0f;
     };
@@ -1074,16 +1086,16 @@ __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
         const int nt = min(kWtWaves, n_qt - q0);
         {
             QTile<HD, false> qt;
-            qt.make(raw, lane);
+            qt.template make<true>(raw, lane);
 #pragma unroll
             for (int c = 0; c < NB; ++c) {
-                s_q[wv][c][0][lane] = qt.hi[c];
-                s_q[wv][c][1][lane] = qt.lo[c];
+                s_q[wv][c][0][fg * 16 + fr] = qt.hi[c];
+                s_q[wv][c][1][fg * 16 + fr] = qt.lo[c];
             }
-            if (g == 0) {
-                s_inv[wv][r] = qt.inv;
-                s_z[wv][r] = z_next;
-                s_see[wv][r] = see_next;
+            if (fg == 0) {
+                s_inv[wv][fr] = qt.inv;
+                s_z[wv][fr] = z_next;
+                s_see[wv][fr] = see_next;
             }
         }
         __syncthreads();
