@@ -248,7 +248,7 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4Rows a, size_t layer_bytes,
 //  * q is split into two f16 halves (22 bits) after a power-of-two scaling of
 //    its row, and so is p * d_v, the probability times the value block's
 //    scale, under a power of two that follows the largest d_v seen (what is
-//    below 2^-39 of that largest product is lost).
+//    below 2^-33 of that largest product is lost).
 //  * The key blocks' scales multiply the 32-dim partial products in f32.
 typedef float float2_t __attribute__((ext_vector_type(2)));
 
@@ -503,11 +503,15 @@ __device__ inline float4_t score_tile(const Src &pl, const unsigned *s_ks, int t
     return s;
 }
 
-// The running softmax of a wave's 16 columns.
+// The running softmax of a wave's 16 columns.  Its reference m follows the scores
+// only when one is 2^kLazy times larger (sixteen columns would otherwise rescale
+// at most pages): p < 2^kLazy and d_v < 2^(ve + 1), so p d_v 2^(kUp - ve) stays
+// below 2^15.
+constexpr int kLazy = 6, kUp = 14 - kLazy;
 template <int HD>
 struct Softmax {
-    float m = -INFINITY;  // per column, log2 units
-    float l = 0.0f;       // of this lane's keys; l and o in units of 2^(ve - 14)
+    float m = -INFINITY;  // per column, log2 units: within kLazy of the largest score
+    float l = 0.0f;       // of this lane's keys; l and o in units of 2^(ve - kUp)
     int ve = -100;        // 2^ve <= the largest d_v seen < 2^(ve + 1)
     float4_t o[HD / 16];
     __device__ Softmax() {
@@ -549,7 +553,7 @@ __device__ inline void attend_page(const Src &pl, const unsigned *s_ks, const un
 #pragma unroll
     for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[i]);
     const float m_new = fmaxf(st.m, col_max(pm) * q.inv);
-    if (__any(m_new > st.m || dmax >= ldexpf(1.0f, st.ve + 1))) {
+    if (__any(m_new > st.m + (float)kLazy || dmax >= ldexpf(1.0f, st.ve + 1))) {
 #pragma unroll
         for (int x = 1; x < kWave; x <<= 1) dmax = fmaxf(dmax, __shfl_xor(dmax, x, kWave));
         const int ve = max(dmax > 0.0f ? ilogbf(dmax) : -24, st.ve);
@@ -561,8 +565,8 @@ __device__ inline void attend_page(const Src &pl, const unsigned *s_ks, const un
         st.m = m_new;
         st.ve = ve;
     }
-    // p 2^(14 - ve)
-    const float m0 = (st.m == -INFINITY ? 0.0f : st.m) - (float)(14 - st.ve);
+    // p 2^(kUp - ve)
+    const float m0 = (st.m == -INFINITY ? 0.0f : st.m) - (float)(kUp - st.ve);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], q.inv, -m0));
@@ -797,7 +801,7 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     }
     // o holds 2^-9 of the quants; l and o back to their own units, the
     // column's sum over its four lane groups, then the waves
-    const float down = ldexpf(1.0f, st.ve - 14);
+    const float down = ldexpf(1.0f, st.ve - kUp);
     st.l = col_sum(st.l) * down;
     if (g == 0 && r < NQ) {
         s_m[wv][r] = st.m;
@@ -1005,13 +1009,14 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
     if (!real) return;
     // l and o share their power of two; o holds 2^-9 of the quants
     float *to = out + row_index(a, b, row) * os + qh * HD + 4 * g;
+    const float inv = 0x1p9f / l;
 #pragma unroll
     for (int e = 0; e < HD / 16; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) to[16 * e + i] = st.o[e][i] * 0x1p9f / l;
+        for (int i = 0; i < 4; ++i) to[16 * e + i] = st.o[e][i] * inv;
     if (lse && g == 0)
         lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] =
-            st.m + __log2f(l * ldexpf(1.0f, st.ve - 14));
+            st.m + __log2f(l * ldexpf(1.0f, st.ve - kUp));
 }
 
 // The keys' attention weights: a wave a page of a KV head goes over all the

@@ -15,10 +15,11 @@ Attention is compared in f64.  With hd dims, u = 2^-24:
    64 roundings of a page's matrix products, and pages and waves add a few more.
 So |out - ref| <= (160 u * max(1, top) + 128 u) * sum p |v| + tiny, top the largest
 sum |q k| / sqrt(hd) of the row: 2^-24 * 288 = 1.7e-5 of it at top = 1.
-The halves of p d are f16 below 2^15 in units of 2^(e - 14), 2^e <= the largest d: what
-both leave is at most half of f16's smallest step, 2^-25, so 2^-39 of the largest d, times
-a quant of 8 at most and added over the keys (the sum of p is 1 or more before its
-division): tiny = keys * 2^-39 * max |v|, for the largest |v| is 8 of the largest d."""
+The halves of p d are f16 in units of 2^(e - 8), 2^e <= the largest d (p may reach 2^6
+before its reference follows): what both leave is at most half of f16's smallest step,
+2^-25, so 2^-33 of the largest d, times a quant of 8 at most and added over the keys (the
+sum of p, before its division, is at least the probability of the key that set the
+reference, 1): tiny = keys * 2^-33 * max |v|, for the largest |v| is 8 of the largest d."""
 import numpy as np
 import pytest
 
@@ -204,7 +205,7 @@ def check_attend(hd, kv, grp, b, m, pos, cnt=None, weights=True, seed=0, scale=1
         sk = R.stored(k[i, :end]).reshape(end, kv, hd)
         sv = R.stored(v[i, :end]).reshape(end, kv, hd)
         ref, rw, mag, top = R.attend(q[i, :n], sk, sv, pos[i], kv * grp)
-        tiny = end * 2.0 ** -39 * np.abs(sv).max()
+        tiny = end * 2.0 ** -33 * np.abs(sv).max()
         err, tol = np.abs(got[i, :n] - ref), (160 * np.maximum(1, top) + 128) * U * mag + tiny
         worst = (err / tol).max()
         assert worst <= 1, (i, worst, err.max())
@@ -284,7 +285,7 @@ def test_attend_value_scales(first, second):
         c.attend(0, dev(q), out, pos)
         sk, sv = (R.stored(x).reshape(n, 1, hd) for x in (k, v))
         ref, _, mag, top = R.attend(q, sk, sv, pos, 1)
-        tiny = n * 2.0 ** -39 * np.abs(sv).max()
+        tiny = n * 2.0 ** -33 * np.abs(sv).max()
         assert (np.abs(host(out) - ref) <= (160 * np.maximum(1, top) + 128) * U * mag + tiny).all()
 
 
