@@ -1069,10 +1069,13 @@ __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
 #pragma unroll
             for (int c = 0; c < NB; ++c) kq[t][c] = quants(pl.k[t][c]);
     }
-    // from the first row that sees the group's first key on; a tile's queries are
-    // loaded while the batch before it is computed
-    const int qt0 = (key0 > p0 ? (int)(key0 - p0) : 0) * groups / 16;
+    // Batches from the last down to the first whose rows see the group's first key:
+    // all groups of a head go over the same tiles at the same time, so that their
+    // XCD's cache serves most of them.  A tile's queries are loaded while the batch
+    // before it is computed.
+    const int qt0 = (key0 > p0 ? (int)(key0 - p0) : 0) * groups / 16 / kWtWaves * kWtWaves;
     const int n_qt = (n_q + 15) / 16, step = n_parts * kWtWaves;
+    const int last = ((n_qt - 1) / kWtWaves - mine) / n_parts * n_parts + mine;
     QRaw<HD, false> raw;
     float z_next = 0.0f;
     unsigned see_next = 0;
@@ -1086,8 +1089,9 @@ __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
         see_next = real ? p0 + row + 1 : 0;
         z_next = real ? lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] : 0.0f;
     };
-    fetch(qt0 + mine * kWtWaves + wv);
-    for (int q0 = qt0 + mine * kWtWaves; q0 < n_qt; q0 += step) {
+    const int q_last = (n_qt - 1) / kWtWaves >= mine ? last * kWtWaves : -1;
+    if (q_last >= qt0) fetch(q_last + wv);
+    for (int q0 = q_last; q0 >= qt0; q0 -= step) {
         const int nt = min(kWtWaves, n_qt - q0);
         {
             QTile<HD, false> qt;
@@ -1104,7 +1108,7 @@ __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
             }
         }
         __syncthreads();
-        fetch(q0 + step + wv);
+        if (q0 - step >= qt0) fetch(q0 - step + wv);
         // the first of the tiles whose last row sees this wave's page
         for (int u = 0; u < nt && has; ++u) {
             const int c0 = (q0 + u) * 16, c1 = min(c0 + 16, n_q) - 1;
