@@ -75,8 +75,10 @@ __device__ inline size_t row_index(const Kv4Rows &a, int b, size_t i) {
 // is rounded exactly: n = rint(x * (1 / d)) is off by one at most, the rest
 // x - n d is exact in f32 (n d has 15 bits and is near x), and comparing it
 // with d / 2 settles n.  The quants go through LDS, key by key, and leave as
-// the page's dwords; where keys of a V dword are not the call's, their nibbles
-// are kept (a dword has one writer).
+// the page's dwords, 16 bytes a thread; where keys of a V dword are not the call's,
+// their nibbles are kept (a dword has one writer; what it held is loaded with the
+// rows).  A thread's loads of eight rows are in flight together (2 x 2048 rows of
+// 32 heads of 128, one after the other: 49 us).
 __device__ inline int quant_of(float x, float d, float inv) {
     float n = rintf(x * inv);
     n = fminf(fmaxf(n, -9.0f), 9.0f);
@@ -85,16 +87,52 @@ __device__ inline int quant_of(float x, float d, float inv) {
     if (fabsf(r) > h || (fabsf(r) == h && ((int)n & 1))) n = n + up;
     return (int)fminf(fmaxf(n, -8.0f), 7.0f) + 8;
 }
+// The other lanes' values of a group of eight, step by step: 1 and 2 within the
+// four, then the mirrored four.
+template <int STEP>
+__device__ inline float lane8(float v) {
+    constexpr int c = STEP == 0 ? 0xb1 : STEP == 1 ? 0x4e : 0x141;
+    return __uint_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_uint(v), c, 0xf, 0xf, true));
+}
+// Quantizes a lane's four values with its group's: the quants + 8 as bytes, the
+// block's scale bits.
+__device__ inline unsigned quantize4(float4_t f, unsigned short *scale) {
+    float mx = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+    float mn = fminf(fminf(f[0], f[1]), fminf(f[2], f[3]));
+    float bad = 0.0f;  // 1: a value that is not finite
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad = fabsf(f[i]) < INFINITY ? bad : 1.0f;
+    mx = fmaxf(mx, lane8<0>(mx));
+    mn = fminf(mn, lane8<0>(mn));
+    bad = fmaxf(bad, lane8<0>(bad));
+    mx = fmaxf(mx, lane8<1>(mx));
+    mn = fminf(mn, lane8<1>(mn));
+    bad = fmaxf(bad, lane8<1>(bad));
+    mx = fmaxf(mx, lane8<2>(mx));
+    mn = fminf(mn, lane8<2>(mn));
+    bad = fmaxf(bad, lane8<2>(bad));
+    const float am = mx >= -mn ? mx : mn;
+    const _Float16 d16 = (_Float16)fminf(fmaxf(am * -0.125f, -65504.0f), 65504.0f);
+    const float d = (float)d16, inv = 1.0f / d;
+    const bool none = bad != 0.0f || d == 0.0f;
+    unsigned w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (unsigned)(none ? 8 : quant_of(f[i], d, inv)) << (8 * i);
+    *scale = bad != 0.0f ? 0x7e00 : __builtin_bit_cast(unsigned short, d16);
+    return w;
+}
 
 template <int HD, bool V4>
 __global__ __launch_bounds__(256) void k_kv4_append(Kv4Rows a, const float *__restrict__ k,
                                                     const float *__restrict__ v, size_t stride,
                                                     int n_pg) {
     using P = Page<HD>;
-    constexpr int NB = P::NB, LD = HD + 4, R4 = HD / 4;
+    constexpr int NB = P::NB, LD = HD + 8, R4 = HD / 4, RP = 256 / R4;  // rows a pass
+    constexpr int U = 4;  // passes in flight
     __shared__ __attribute__((aligned(16))) uint8_t s_q[2][kPageKeys][LD];
     __shared__ uint16_t s_d[2][kPageKeys][NB];
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wv = wave_id(), g = lane >> 4, r = lane & 15;
     unsigned x = blockIdx.x;
     const int pg = x % n_pg;
     x /= n_pg;
@@ -105,75 +143,73 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4Rows a, const float *__re
     if (cnt == 0 || key0 >= p0 + cnt) return;
     const int lo = (int)(max(p0, key0) - key0);
     const int hi = (int)(min(p0 + cnt, key0 + kPageKeys) - key0);
-    const int items = (hi - lo) * R4;
-    for (int it = t; it < 2 * items; it += 256) {
-        const int which = it >= items, rest = which ? it - items : it;
-        const int key = lo + rest / R4, e = rest % R4;
-        const size_t row = row_index(a, b, key0 + key - p0);
-        const float *src = (which ? v : k) + row * stride + head * HD + 4 * e;
-        float f[4];
-        if constexpr (V4) {
-            const float4 w = *reinterpret_cast<const float4 *>(src);
-            f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = src[i];
-        }
-        float mx = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
-        float mn = fminf(fminf(f[0], f[1]), fminf(f[2], f[3]));
-        int bad = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= !(fabsf(f[i]) < INFINITY);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-            mx = fmaxf(mx, __shfl_xor(mx, o, kWave));
-            mn = fminf(mn, __shfl_xor(mn, o, kWave));
-            bad |= __shfl_xor(bad, o, kWave);
-        }
-        const float am = mx >= -mn ? mx : mn;
-        const _Float16 d16 = (_Float16)fminf(fmaxf(am * -0.125f, -65504.0f), 65504.0f);
-        const float d = (float)d16;
-        const float inv = 1.0f / d;
-        unsigned w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int q = bad || d == 0.0f ? 8 : quant_of(f[i], d, inv);
-            w |= (unsigned)q << (8 * i);
-        }
-        *reinterpret_cast<unsigned *>(&s_q[which][key][4 * e]) = w;
-        if ((e & 7) == 0)
-            s_d[which][key][e >> 3] = bad ? 0x7e00 : __builtin_bit_cast(unsigned short, d16);
-    }
-    __syncthreads();
     uint8_t *pb = a.pages + (((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages + page) *
                                 P::kBytes;
-    for (int w = t; w < 8 * HD; w += 256) {  // K dwords
-        const int tile = w / (64 * NB), l = (w / NB) & 63, blk = w % NB;
-        const int key = 16 * tile + (l & 15), g = l >> 4;
-        if (key < lo || key >= hi) continue;
-        const uint2 q = *reinterpret_cast<const uint2 *>(&s_q[0][key][32 * blk + 8 * g]);
-        // bytes of even elements are nibbles 0..3, of odd ones nibbles 4..7
-        const unsigned e0 = q.x & 0x000f000f, o0 = (q.x >> 8) & 0x000f000f;
-        const unsigned e1 = q.y & 0x000f000f, o1 = (q.y >> 8) & 0x000f000f;
-        const unsigned ev = (e0 & 0xf) | (e0 >> 12) | (e1 & 0xf) << 8 | (e1 >> 4 & 0xf000);
-        const unsigned od = (o0 & 0xf) | (o0 >> 12) | (o1 & 0xf) << 8 | (o1 >> 4 & 0xf000);
-        *reinterpret_cast<unsigned *>(pb + 4 * w) = ev | od << 16;
-    }
-    for (int w = t; w < 8 * HD; w += 256) {  // V dwords
-        const int c = w >> 8, l = (w >> 2) & 63, e = 2 * c + ((w >> 1) & 1), h = w & 1;
-        const int dim = 16 * e + (l & 15), g = l >> 4;
-        unsigned val = 0, mask = 0;
+    uint4_t *vto = reinterpret_cast<uint4_t *>(pb + P::kV + wv * 1024 + lane * 16);
+    uint4_t old = {0, 0, 0, 0};
+    if (wv < NB && hi - lo < kPageKeys) old = *vto;
+    const int e = t % R4, first = lo + t / R4;
+    const size_t base = row_index(a, b, 0) * stride + head * HD + 4 * e;
+    for (int k0 = first; k0 < hi; k0 += U * RP) {
+        float4_t f[2][U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int key = P::v_key(g, h, j), sh = 4 * nibble_of(j);
-            if (key >= lo && key < hi) {
-                val |= (unsigned)s_q[1][key][dim] << sh;
-                mask |= 0xfu << sh;
+        for (int u = 0; u < U; ++u) {
+            // (the last row again past the end)
+            const size_t at = base + (size_t)(key0 + min(k0 + u * RP, hi - 1) - p0) * stride;
+            if constexpr (V4) {
+                f[0][u] = *reinterpret_cast<const float4_t *>(k + at);
+                f[1][u] = *reinterpret_cast<const float4_t *>(v + at);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[0][u][i] = k[at + i], f[1][u][i] = v[at + i];
             }
         }
-        unsigned *dst = reinterpret_cast<unsigned *>(pb + P::kV + 4 * w);
-        if (mask == 0xffffffffu) *dst = val;
-        else if (mask) *dst = (*dst & ~mask) | val;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int key = k0 + u * RP;
+            if (key >= hi) break;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                unsigned short d;
+                *reinterpret_cast<unsigned *>(&s_q[w][key][4 * e]) = quantize4(f[w][u], &d);
+                if ((e & 7) == 0) s_d[w][key][e >> 3] = d;
+            }
+        }
+    }
+    __syncthreads();
+    const int kkey = 16 * wv + r;  // K: key kkey, dims 32 blk + 8 g ..
+    if (kkey >= lo && kkey < hi) {
+        unsigned *to = reinterpret_cast<unsigned *>(pb + P::k_dword(kkey, g, 0));
+        unsigned w[NB];
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) {
+            const uint2 q = *reinterpret_cast<const uint2 *>(&s_q[0][kkey][32 * blk + 8 * g]);
+            // bytes of even elements are nibbles 0..3, of odd ones nibbles 4..7
+            const unsigned e0 = q.x & 0x000f000f, o0 = (q.x >> 8) & 0x000f000f;
+            const unsigned e1 = q.y & 0x000f000f, o1 = (q.y >> 8) & 0x000f000f;
+            const unsigned ev = (e0 & 0xf) | (e0 >> 12) | (e1 & 0xf) << 8 | (e1 >> 4 & 0xf000);
+            const unsigned od = (o0 & 0xf) | (o0 >> 12) | (o1 & 0xf) << 8 | (o1 >> 4 & 0xf000);
+            w[blk] = ev | od << 16;
+        }
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) to[blk] = w[blk];
+    }
+    if (wv < NB) {  // V: chunk wv, dims 32 wv + 16 dt + r, both halves
+        unsigned val[2][2] = {{0, 0}, {0, 0}}, mask[2] = {0, 0};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = P::v_key(g, h, j), sh = 4 * nibble_of(j);
+                if (key >= lo && key < hi) {
+                    val[0][h] |= (unsigned)s_q[1][key][32 * wv + r] << sh;
+                    val[1][h] |= (unsigned)s_q[1][key][32 * wv + 16 + r] << sh;
+                    mask[h] |= 0xfu << sh;
+                }
+            }
+        if (mask[0] | mask[1])
+            *vto = uint4_t{(old.x & ~mask[0]) | val[0][0], (old.y & ~mask[1]) | val[0][1],
+                           (old.z & ~mask[0]) | val[1][0], (old.w & ~mask[1]) | val[1][1]};
     }
     for (int w = t; w < 2 * 64 * NB; w += 256) {  // scales
         const int which = w >= 64 * NB, rest = which ? w - 64 * NB : w;
@@ -185,13 +221,14 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4Rows a, const float *__re
 }
 
 // ---- read ---------------------------------------------------------------------------
-// Four consecutive dims of one row's key and value a thread.
+// A workgroup a page: a thread takes eight dims of a key from one K dword at a time,
+// then eight keys of four dims from four V dwords.
 template <int HD, bool V4>
 __global__ __launch_bounds__(256) void k_kv4_read(Kv4Rows a, size_t layer_bytes,
                                                   float *__restrict__ k, float *__restrict__ v,
                                                   size_t stride, int n_pg) {
     using P = Page<HD>;
-    constexpr int R4 = HD / 4;
+    constexpr int NB = P::NB, R4 = HD / 4;
     unsigned x = blockIdx.x;
     const int pg = x % n_pg;
     x /= n_pg;
@@ -207,31 +244,50 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4Rows a, size_t layer_bytes,
     const uint8_t *pb = a.pages + layer * layer_bytes +
                         (((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages + page) *
                             P::kBytes;
-    for (int it = threadIdx.x; it < (hi - lo) * R4; it += 256) {
-        const int key = lo + it / R4, e = it % R4, blk = e >> 3;
-        const size_t row =
-            (size_t)layer * a.n_seqs * a.ld_rows + row_index(a, b, key0 + key - p0);
-        const float dk = (float)*reinterpret_cast<const _Float16 *>(pb + P::kKs + P::scale(key, blk));
-        const float dv = (float)*reinterpret_cast<const _Float16 *>(pb + P::kVs + P::scale(key, blk));
-        const unsigned kw =
-            *reinterpret_cast<const unsigned *>(pb + P::k_dword(key, (e >> 1) & 3, blk));
-        int g, h, j;
-        P::v_place(key, &g, &h, &j);
-        float fk[4], fv[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            fk[i] = (float)((int)(kw >> (4 * nibble_of(4 * (e & 1) + i)) & 0xf) - 8) * dk;
-            const unsigned vw =
-                *reinterpret_cast<const unsigned *>(pb + P::v_dword(4 * e + i, g, h));
-            fv[i] = (float)((int)(vw >> (4 * nibble_of(j)) & 0xf) - 8) * dv;
-        }
-        float *ko = k + row * stride + head * HD + 4 * e, *vo = v + row * stride + head * HD + 4 * e;
+    // where row 0 of the call goes, and a key of the page
+    const size_t base = ((size_t)layer * a.n_seqs * a.ld_rows + row_index(a, b, 0)) * stride +
+                        head * HD;
+    auto at = [&](int key) { return base + (size_t)(key0 + key - p0) * stride; };
+    auto put = [](float *to, const float *f) __attribute__((always_inline)) {
         if constexpr (V4) {
-            *reinterpret_cast<float4 *>(ko) = float4{fk[0], fk[1], fk[2], fk[3]};
-            *reinterpret_cast<float4 *>(vo) = float4{fv[0], fv[1], fv[2], fv[3]};
+            *reinterpret_cast<float4_t *>(to) = float4_t{f[0], f[1], f[2], f[3]};
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ko[i] = fk[i], vo[i] = fv[i];
+            for (int i = 0; i < 4; ++i) to[i] = f[i];
+        }
+    };
+    for (int it = threadIdx.x; it < (hi - lo) * (HD / 8); it += 256) {
+        const int key = lo + it / (HD / 8), c = it % (HD / 8), blk = c >> 2, g = c & 3;
+        const float d = (float)*reinterpret_cast<const _Float16 *>(pb + P::kKs + P::scale(key, blk));
+        const unsigned w = *reinterpret_cast<const unsigned *>(pb + P::k_dword(key, g, blk));
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (float)((int)(w >> (4 * nibble_of(j)) & 0xf) - 8) * d;
+        float *to = k + at(key) + 32 * blk + 8 * g;
+        put(to, f);
+        put(to + 4, f + 4);
+    }
+    for (int it = threadIdx.x; it < R4 * 8; it += 256) {
+        const int e = it % R4, g = it / R4 & 3, h = it / R4 >> 2, blk = e >> 3;
+        if (32 * h + 4 * g >= hi || 32 * h + 20 + 4 * g <= lo) continue;  // none of its keys
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = *reinterpret_cast<const unsigned *>(pb + P::v_dword(4 * e + i, g, h));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint2 d = *reinterpret_cast<const uint2 *>(
+                pb + P::kVs + (((2 * h + u) * 4 + g) * NB + blk) * 8);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = 32 * h + 16 * u + 4 * g + j, sh = 4 * nibble_of(4 * u + j);
+                const unsigned dw = (j & 2 ? d.y : d.x) >> (16 * (j & 1));
+                const float dv = f16_bits_to_f32(dw & 0xffff);
+                float f[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = (float)((int)(w[i] >> sh & 0xf) - 8) * dv;
+                if (key >= lo && key < hi) put(v + at(key) + 4 * e, f);
+            }
         }
     }
 }
