@@ -646,10 +646,14 @@ __device__ inline void attend_page(const Src &pl, const unsigned *s_ks, const un
         *hi = join(hh[0], hh[1], hh[2], hh[3]);
         *lo = join(ll[0], ll[1], ll[2], ll[3]);
     };
-    auto sum = [&](int e, int h, half8_t hi, half8_t lo) __attribute__((always_inline)) {
-        const half8_t vq = pl.vop(e, h);
-        st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, lo, st.o[e], 0, 0, 0);
-        st.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vq, hi, st.o[e], 0, 0, 0);
+    // the dims of block b (two tiles in turn, so that no product waits for the last)
+    auto sum = [&](int b, int h, half8_t hi, half8_t lo) __attribute__((always_inline)) {
+        const half8_t v0 = pl.vop(2 * b, h), v1 = pl.vop(2 * b + 1, h);
+        float4_t o0 = st.o[2 * b], o1 = st.o[2 * b + 1];
+        o0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, lo, o0, 0, 0, 0);
+        o1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, lo, o1, 0, 0, 0);
+        st.o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, hi, o0, 0, 0, 0);
+        st.o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, hi, o1, 0, 0, 0);
     };
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -664,7 +668,7 @@ __device__ inline void attend_page(const Src &pl, const unsigned *s_ks, const un
             half8_t hi, lo;
             weigh(h, d, &hi, &lo);
 #pragma unroll
-            for (int e = 0; e < HD / 16; ++e) sum(e, h, hi, lo);
+            for (int b = 0; b < NB; ++b) sum(b, h, hi, lo);
         } else {
             unsigned dv[2][2 * NB];  // the scales of tiles 2 h and 2 h + 1
 #pragma unroll
@@ -678,8 +682,7 @@ __device__ inline void attend_page(const Src &pl, const unsigned *s_ks, const un
                                           {dv[1][2 * b], dv[1][2 * b + 1]}};
                 half8_t hi, lo;
                 weigh(h, d, &hi, &lo);
-                sum(2 * b, h, hi, lo);
-                sum(2 * b + 1, h, hi, lo);
+                sum(b, h, hi, lo);
             }
         }
     }
