@@ -226,8 +226,11 @@ mri_status mri_llama_forward_kv4(mri_llama *model, const uint32_t *tokens, size_
 
 /* Probabilities of rows of n logits (device, x_stride / out_stride floats
  * apart; out may be x): out = exp((x - max x) / temperature) / sum.  A row of
- * -inf only becomes zeros.  InvalidArgument unless temperature > 0 and finite;
- * InvalidShape for n = 0 or a stride below n. */
+ * -inf only becomes zeros, one with NaN or +inf NaN.  Few rows are cut into
+ * parts, whose statistics pass through 1 MiB kept per (device, stream); a call
+ * that is being captured uses none, takes longer and gives the same bits.
+ * InvalidArgument unless temperature > 0 and finite; InvalidShape for n = 0 or a
+ * stride below n. */
 mri_status mri_softmax(const float *x, size_t rows, size_t n, size_t x_stride, float temperature,
                        float *out, size_t out_stride, void *stream);
 
@@ -243,7 +246,9 @@ mri_status mri_softmax(const float *x, size_t rows, size_t n, size_t x_stride, f
  * uniforms[k] times the total.  accepted[b] = a; tokens [n_seqs, k + 1] = the
  * accepted drafts, the drawn token, then MRI_NO_TOKEN.  A draft id >= n is
  * rejected; where no token has a positive probability the drawn token is
- * MRI_NO_TOKEN.  NaN probabilities count as 0.  InvalidShape for n = 0. */
+ * MRI_NO_TOKEN.  A NaN target probability counts as 0; a token whose draft
+ * probability is NaN is neither accepted nor drawn in its place.  InvalidShape
+ * for n = 0. */
 #define MRI_NO_TOKEN 0xffffffffu
 mri_status mri_verify_drafts(const uint32_t *drafts, const float *draft_probs,
                              const float *target_probs, const float *uniforms,

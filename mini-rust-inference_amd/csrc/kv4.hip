@@ -1044,7 +1044,8 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
         qtile.make(raw, lane);
     }
     const long see = real ? (long)p0 + row + 1 : 0;  // keys this column sees
-    const unsigned all = p0 + q0 / groups + 1;       // keys every real column of the wave sees
+    // keys every real column of the wave sees
+    const unsigned all = q0 < n_q ? p0 + q0 / groups + 1 : 0;
     // pages that the wave's last row sees
     const unsigned my_pg =
         q0 < n_q ? (p0 + (min(q0 + 16, n_q) - 1) / groups) / kPageKeys + 1 : 0;
@@ -1505,10 +1506,11 @@ __global__ __launch_bounds__(256) void k_kv4_move(Kv4Evict e, int per_row) {
 
 inline bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-// Workgroups of one launch: 2^32 threads at most.
+// Workgroups of one launch (512 threads each at most; a launch takes 2^32).
+constexpr size_t kMostWgs = 1u << 22;
 mri_status grid_ok(size_t blocks) {
-    return blocks < (1u << 22) ? MRI_OK
-                               : set_error(MRI_ERR_UNSUPPORTED, "kv4: more than 2^22 workgroups");
+    return blocks <= kMostWgs ? MRI_OK
+                              : set_error(MRI_ERR_UNSUPPORTED, "kv4: more than 2^22 workgroups");
 }
 
 template <class F>
@@ -1622,11 +1624,24 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
         if (groups_all > kKv4PartTiles ||
             groups_all * parts * kWtWaves * kPageKeys > kv4_part_floats(HD))
             parts = 1;
-        if (const mri_status e = grid_ok(groups_all * parts)) return e;
-        hipLaunchKernelGGL((k_kv4_weights<HD>), dim3((unsigned)(groups_all * parts)),
-                           dim3(kWtWaves * kWave), 0, s, a, q, qs, vec, groups, (int)n_grp,
-                           (int)parts, lse, weights, part, cnts);
-        MRI_LAUNCHED("k_kv4_weights");
+        // (positions on the device: the pages are those of the longest possible
+        // sequence, so many sequences of a long cache take more than one launch)
+        const size_t seqs = std::min<size_t>(
+            a.n_seqs, std::max<size_t>(1, kMostWgs / (n_grp * a.n_kv * parts)));
+        if (const mri_status e = grid_ok(n_grp * a.n_kv * parts)) return e;
+        for (size_t b = 0; b < (size_t)a.n_seqs; b += seqs) {
+            Kv4Rows c = a;
+            c.first_seq += (int)b;
+            c.n_seqs = (int)std::min<size_t>(seqs, a.n_seqs - b);
+            if (c.pos) c.pos += b;
+            if (c.count) c.count += b;
+            hipLaunchKernelGGL((k_kv4_weights<HD>),
+                               dim3((unsigned)(n_grp * c.n_kv * c.n_seqs * parts)),
+                               dim3(kWtWaves * kWave), 0, s, c, q + b * a.ld_rows * qs, qs, vec,
+                               groups, (int)n_grp, (int)parts, lse + b * a.rows * n_heads, weights,
+                               part, cnts);
+            MRI_LAUNCHED("k_kv4_weights");
+        }
     }
     return MRI_OK;
 }
@@ -1668,14 +1683,15 @@ mri_status launch_kv4_attend(const Kv4Rows &a, size_t hd, const float *q, size_t
 
 mri_status launch_kv4_evict(const Kv4Evict &e, size_t hd, hipStream_t s) {
     const size_t rows = (size_t)e.n_layers * e.n_seqs * e.n_kv;
-    if (const mri_status st = grid_ok(rows * 4)) return st;
+    if (const mri_status st = grid_ok(rows * 2)) return st;  // (1024 threads each)
     if (e.src_max <= kSelRegs * kSelThreads)
         hipLaunchKernelGGL(k_kv4_select<true>, dim3((unsigned)rows), dim3(kSelThreads), 0, s, e);
     else
         hipLaunchKernelGGL(k_kv4_select<false>, dim3((unsigned)rows), dim3(kSelThreads), 0, s, e);
     MRI_LAUNCHED("k_kv4_select");
-    const size_t per_row = e.src == e.dst ? 1 : (e.keep + kPageKeys - 1) / kPageKeys;
-    if (const mri_status st = grid_ok(rows * per_row)) return st;
+    const size_t n_pg = ((size_t)e.keep + kPageKeys - 1) / kPageKeys;
+    const size_t per_row =
+        e.src == e.dst ? 1 : std::max<size_t>(1, std::min(n_pg, kMostWgs / rows));
     by_head(hd, [&](auto h) {
         constexpr int HD = decltype(h)::value;
         hipLaunchKernelGGL((k_kv4_move<HD>), dim3((unsigned)(rows * per_row)), dim3(256), 0, s, e,

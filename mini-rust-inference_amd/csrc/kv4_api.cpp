@@ -106,6 +106,7 @@ mri_status mri_kv4_cache_create(size_t n_layers, size_t n_seqs, size_t max_seq, 
         (e = hipMalloc(&c->cnts, kKv4PartTiles * sizeof(int))) ||
         (e = hipMemset(c->cnts, 0, kKv4PartTiles * sizeof(int))) ||
         (e = hipStreamSynchronize(nullptr))) {
+        (void)hipGetLastError();  // a refused allocation is no later launch's error
         mri_kv4_cache_destroy(c);
         return hip_error(e, "kv4_cache_create");
     }

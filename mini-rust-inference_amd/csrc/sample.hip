@@ -311,11 +311,12 @@ mri_status launch_softmax(const float *x, size_t rows, size_t n, size_t x_stride
     // Rows in parts where whole rows leave CUs idle.  The parts' workspace is the
     // stream's: a call that is being captured uses none, so that graphs recorded on one
     // stream may run side by side.
-    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     if (parts > 1 && rows < 4 * (size_t)std::max(device_cus(), 1)) {
-        MRI_HIP(hipStreamIsCapturing(s, &capture));
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
         void *ws = nullptr;
-        if (capture == hipStreamCaptureStatusNone) {
+        if (hipStreamIsCapturing(s, &capture) != hipSuccess) {
+            (void)hipGetLastError();
+        } else if (capture == hipStreamCaptureStatusNone) {
             const mri_status st = softmax_ws_get(s, &ws);
             if (st) return st;
         }

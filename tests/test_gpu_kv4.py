@@ -257,6 +257,57 @@ def test_attend_many_sequences():
     check_attend(64, 1, 2, 70, 1, pos, [int(x) for x in rng.integers(0, 2, 70)])
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attend_more_sequences_than_cus(hd):
+    """Enough tiles that none splits its keys, one and several columns a tile."""
+    rng = np.random.default_rng(hd)
+    pos = [int(x) for x in rng.integers(0, 150, 450)]
+    check_attend(hd, 2, 2, 450, 1, pos, [int(x) for x in rng.integers(0, 2, 450)])
+    check_attend(hd, 1, 6, 400, 2, pos[:400], [int(x) for x in rng.integers(0, 3, 400)])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kv,grp,b,m,pos,cnt", [
+    (8, 2, 8, 130, 0, None),                    # 64 queries a workgroup, a short last one
+    (8, 1, 7, 300, 70, (300, 0, 1, 64, 65, 299, 17)),
+    (4, 3, 16, 100, 5, None),                   # tiles that end inside a row's heads
+])
+def test_attend_prompts(hd, kv, grp, b, m, pos, cnt):
+    """Prompts large enough for the form that shares pages between queries."""
+    check_attend(hd, kv, grp, b, m, pos, cnt)
+
+
+def test_attend_prompt_strided_and_nan():
+    """The same form with rows of any spacing and alignment, and with NaN among the
+    queries, keys and values: only what sees it is spoilt."""
+    L, Q, torch = mods()
+    rng = np.random.default_rng(61)
+    kv, hd, m = 32, 64, 520
+    c = L.Kv4Cache(1, 1, m, kv, hd)
+    k, v = rows(rng, m, kv * hd), rows(rng, m, kv * hd)
+    q = rng.standard_normal((m, kv * hd)).astype(F32)
+    k[200, 3] = np.inf                 # head 0
+    v[100, hd + 40] = np.nan           # head 1, its second block
+    q[70, 2 * hd + 5] = np.nan         # head 2
+    c.append(0, dev(k), dev(v), 0)
+    a = torch.empty(m, kv * hd, device="cuda")
+    c.attend(0, dev(q), a, 0)
+    got = host(a).reshape(m, kv, hd)
+    bad = np.zeros((m, kv, hd), bool)
+    bad[200:, 0] = bad[70, 2] = True
+    bad[100:, 1, 32:] = True
+    assert np.array_equal(np.isnan(got), bad)
+    for pad, off in ((1, 3), (4, 0)):
+        buf = torch.zeros(m * (kv * hd + pad) + off, device="cuda")
+        qs = buf[off:].view(m, kv * hd + pad)
+        qs[:, :kv * hd] = dev(q)
+        ob = torch.full_like(buf, 9.0)
+        o = ob[off:].view(m, kv * hd + pad)
+        c.attend(0, qs[:, :kv * hd], o[:, :kv * hd], 0)
+        assert np.array_equal(host(o[:, :kv * hd]).reshape(got.shape), got, equal_nan=True)
+        assert bool((o[:, kv * hd:] == 9).all())
+
+
 def test_attend_long():
     check_attend(128, 1, 4, 1, 1, 20000)
 
@@ -413,6 +464,20 @@ def test_evict(hd, kv, n, keep, recent, lens, in_place):
                     so = R.stored(old[j]).astype(F32)
                     assert np.array_equal(gk[i, j, rest, lane], so[rest, lane])
                     assert np.array_equal(gv[i, j, rest, lane], so[rest, lane])
+
+
+def test_evict_many_positions():
+    """More weights a head than registers hold."""
+    L, Q, torch = mods()
+    rng = np.random.default_rng(37)
+    n, keep, recent = 40000, 5000, 700
+    w = np.exp(3 * rng.standard_normal((1, 2, 1, n))).astype(F32)
+    w[rng.random(w.shape) < 0.3] = 0.5
+    src, dst = L.Kv4Cache(1, 2, n, 1, 64), L.Kv4Cache(1, 2, keep, 1, 64)
+    kept, lo, wo = run_evict(src, dst, w, (n, n - 77), keep, recent)
+    for j, m in enumerate((n, n - 77)):
+        at = R.evict(w[0, j, 0], m, keep, recent)
+        assert np.array_equal(kept[0, j, 0], at) and np.array_equal(wo[0, j, 0], w[0, j, 0, at])
 
 
 def test_evict_special_weights():

@@ -36,7 +36,8 @@ def check_softmax(x, temperature, got):
 
 
 @pytest.mark.parametrize("rows,n", [(1, 1), (3, 2), (2, 63), (5, 64), (1, 1000), (7, 4099),
-                                    (2, 32000), (3, 50021), (1, 131072), (300, 33)])
+                                    (2, 32000), (3, 50021), (1, 131072), (300, 33),
+                                    (2, 300001), (1100, 5000)])
 @pytest.mark.parametrize("temperature", [0.3, 1.0, 2.5])
 def test_softmax(rows, n, temperature):
     L, Q, torch = mods()
@@ -116,7 +117,7 @@ def run_verify(drafts, p, u, q=None, counts=None):
 
 @pytest.mark.parametrize("b,k,n", [(1, 0, 1), (3, 0, 17), (40, 4, 2), (20, 3, 64), (20, 3, 65),
                                    (16, 8, 1000), (8, 4, 16385), (4, 7, 32000), (2, 2, 131072),
-                                   (3, 70, 200)])
+                                   (3, 70, 200), (2, 1, 300001)])
 @pytest.mark.parametrize("sampled", [True, False])
 def test_verify(b, k, n, sampled):
     rng = np.random.default_rng([b, k, n])
@@ -200,6 +201,7 @@ def test_sampling_graph_replays():
             step()
     for _ in range(5):
         z = (rng.standard_normal((b * (k + 1), n)) * 6).astype(F32)
+        z[1, ::3] = -np.inf
         x.copy_(dev(z))
         d = z.reshape(b, k + 1, n)[:, :k].argmax(2)
         drafts.copy_(dev(d.astype(np.int32)))
@@ -207,8 +209,10 @@ def test_sampling_graph_replays():
         u.copy_(dev(uu))
         graph.replay()
         torch.cuda.synchronize()
-        g_tok, g_acc = tok.clone(), acc.clone()
+        g_tok, g_acc, g_probs = tok.clone(), acc.clone(), probs_t.clone()
         step()
+        # (the captured softmax takes other launches than the eager one, to the same bits)
+        assert torch.equal(g_probs, probs_t)
         assert torch.equal(g_tok, tok) and torch.equal(g_acc, acc)
         pr = host(probs_t).reshape(b, k + 1, n)
         for i in range(b):
