@@ -78,7 +78,7 @@ mri_status launch_kv4_evict(const Kv4Evict &e, size_t hd, hipStream_t s);
 // sample.hip
 // The parts' statistics of rows in parts: per (device, stream), of one size, for
 // calls that are not being captured.  *ptr is null where the memory cannot be had.
-constexpr size_t kSoftmaxWsBytes = 1 << 20;
+constexpr size_t kSoftmaxWsBytes = 1 << 18;
 mri_status softmax_ws_get(hipStream_t stream, void **ptr);
 mri_status launch_softmax(const float *x, size_t rows, size_t n, size_t x_stride,
                           float temperature, float *out, size_t out_stride, hipStream_t s);

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "kv4.hpp"
 
@@ -17,7 +18,10 @@ constexpr int kWave = 64;
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // ---- softmax with a temperature ----------------------------------------------
-// p_i = exp((x_i - max x) / T) / sum.  A row is cut into `parts` parts of `len`
+// p_i = exp((x_i - max x) / T) / sum.  Bound by its reads and writes, and by the
+// launch where they are few.
+// A row of up to 32768 logits stays in the registers of one workgroup: read once,
+// one exponential a value (HELD).  A longer one is cut into `parts` parts of `len`
 // values (a multiple of four); 256 threads take a part's (max, sum of
 // exponentials under it), sixteen values a thread at a time.  Few rows: a
 // workgroup a part, then a second launch that joins a row's parts and writes; the
@@ -33,6 +37,68 @@ __device__ inline MaxSum join(MaxSum a, MaxSum b, float c) {
     const float m = fmaxf(a.m, b.m);
     return MaxSum{m, (a.m == m ? a.l : a.l * exp_scaled(a.m - m, c)) +
                          (b.m == m ? b.l : b.l * exp_scaled(b.m - m, c))};
+}
+
+// HELD: V times four values a thread.
+template <int V>
+__global__ __launch_bounds__(1024) void k_softmax_held(const float *x, size_t n, size_t xs,
+                                                       float c, float *out, size_t os) {
+    __shared__ float s_m[16], s_l[16];
+    const float *row = x + (size_t)blockIdx.x * xs;
+    const int t = threadIdx.x, lane = t % kWave, wave = t / kWave;
+    float v[4 * V];
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+        const size_t i = 4 * ((size_t)u * 1024 + t);
+        if (i + 4 <= n) {
+            const float4u w = *reinterpret_cast<const float4u *>(row + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * u + j] = w[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * u + j] = i + j < n ? row[i + j] : -INFINITY;
+        }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4 * V; ++j) m = fmaxf(m, v[j]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+    if (lane == 0) s_m[wave] = m;
+    __syncthreads();
+    m = s_m[lane % 16];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+    float l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4 * V; ++j) {
+        v[j] = v[j] == -INFINITY ? 0.0f : exp_scaled(v[j] - m, c);
+        l = l + v[j];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l = l + __shfl_xor(l, o, kWave);
+    if (lane == 0) s_l[wave] = l;
+    __syncthreads();
+    l = s_l[lane % 16];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) l = l + __shfl_xor(l, o, kWave);
+    // (every logit -inf: zeros)
+    const float inv = m == INFINITY ? NAN : m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+    float *to = out + (size_t)blockIdx.x * os;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+        const size_t i = 4 * ((size_t)u * 1024 + t);
+        if (i + 4 <= n) {
+            float4u p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = v[4 * u + j] * inv;
+            *reinterpret_cast<float4u *>(to + i) = p;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + j < n) to[i + j] = v[4 * u + j] * inv;
+        }
+    }
 }
 
 constexpr int kPartThreads = 256;
@@ -93,6 +159,8 @@ __device__ inline void write_probs(const float *x, size_t lo, size_t hi, int t, 
 }
 
 constexpr int kMaxParts = 64;
+constexpr size_t kSplitRows = 512;
+static_assert(kSplitRows * kMaxParts * sizeof(MaxSum) <= kSoftmaxWsBytes, "parts' workspace");
 __device__ inline MaxSum join_parts(const MaxSum *p, int parts, float c) {
     MaxSum a = p[0];
     for (int i = 1; i < parts; ++i) a = join(a, p[i], c);
@@ -305,13 +373,27 @@ mri_status launch_softmax(const float *x, size_t rows, size_t n, size_t x_stride
                           float temperature, float *out, size_t out_stride, hipStream_t s) {
     if (!rows) return MRI_OK;
     const float c = (float)fmin(1.4426950408889634074 / (double)temperature, (double)FLT_MAX);
+    // Held: 5 x 32000 5.8 us a call against 8.6 in parts (two launches) and 10 in row
+    // form, 320 rows 24 against 27, 512 rows 31 against 41.  Twice as many values a
+    // thread do not fit its registers beside the addresses: 50000 11 against 8.4.
+    const auto held = [&](auto v) {
+        hipLaunchKernelGGL(k_softmax_held<decltype(v)::value>, dim3((unsigned)rows), dim3(1024), 0,
+                           s, x, n, x_stride, c, out, out_stride);
+        MRI_LAUNCHED("k_softmax_held");
+        return MRI_OK;
+    };
+    if (n <= 4096) return held(std::integral_constant<int, 1>());
+    if (n <= 2 * 4096) return held(std::integral_constant<int, 2>());
+    if (n <= 4 * 4096) return held(std::integral_constant<int, 4>());
+    if (n <= 8 * 4096) return held(std::integral_constant<int, 8>());
     // parts of 4096 values at least, 64 of them at most
     const size_t len = round_up(std::max<size_t>((n + kMaxParts - 1) / kMaxParts, 4096), 4);
     const size_t parts = (n + len - 1) / len;
-    // Rows in parts where whole rows leave CUs idle.  The parts' workspace is the
-    // stream's: a call that is being captured uses none, so that graphs recorded on one
-    // stream may run side by side.
-    if (parts > 1 && rows < 4 * (size_t)std::max(device_cus(), 1)) {
+    // Rows in parts where whole rows leave CUs idle (100003 logits: 5 rows 9 us against
+    // 28, 128 rows 33 against 44, 320 rows 76 against 89, 512 rows 125 against 126).
+    // The parts' workspace is the stream's: a call that is being captured uses none,
+    // so that graphs recorded on one stream may run side by side.
+    if (rows < kSplitRows) {
         hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
         void *ws = nullptr;
         if (hipStreamIsCapturing(s, &capture) != hipSuccess) {
@@ -320,7 +402,7 @@ mri_status launch_softmax(const float *x, size_t rows, size_t n, size_t x_stride
             const mri_status st = softmax_ws_get(s, &ws);
             if (st) return st;
         }
-        if (ws && rows * parts * sizeof(MaxSum) <= kSoftmaxWsBytes) {
+        if (ws) {
             hipLaunchKernelGGL(k_softmax_stats, dim3((unsigned)(rows * parts)),
                                dim3(kPartThreads), 0, s, x, n, x_stride, c, len, (int)parts,
                                static_cast<MaxSum *>(ws));

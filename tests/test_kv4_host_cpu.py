@@ -167,29 +167,32 @@ def check_large_batches(h):
 
 
 def check_softmax_forms(h):
-    """Few rows in parts, through 1 MiB of the stream's; a captured call and one whose
-    memory is refused do the rows whole and take none; beside another stream's capture
-    the memory comes without breaking it."""
+    """Rows of up to 32768 logits in one launch without memory; few longer ones in
+    parts, through 256 KiB of the stream's; a captured call and one whose memory is
+    refused do the rows whole and take none; beside another stream's capture the memory
+    comes without breaking it."""
     def go(rows, n):
         return [name for name, _ in h.launched(lambda: h.lib.mri_softmax(
             X, rows, n, n, C.c_float(1.0), OUT, n, STREAM))]
 
     h.set("fake_refuse_malloc", 1)
-    assert ["k_softmax_row" in n for n in go(3, 32000)] == [True]
+    assert ["k_softmax_row" in n for n in go(3, 40000)] == [True]
     h.set("fake_refuse_malloc", 0)
     h.set("fake_capturing", 1)
-    assert ["k_softmax_row" in n for n in go(3, 32000)] == [True] and not h.live()
+    assert ["k_softmax_row" in n for n in go(3, 40000)] == [True] and not h.live()
     h.set("fake_capturing", 0)
     h.set("fake_other_capture", 1)
-    names = go(3, 32000)
+    names = go(3, 40000)
     assert ["stats" in n for n in names] == [True, False] and "write" in names[1]
     assert C.c_int.in_dll(h.f, "fake_broken_captures").value == 0
     h.set("fake_other_capture", 0)
-    assert [h.f.fake_alloc_bytes(i) for i in h.live()] == [1 << 20]
-    go(1000, 200000)
+    assert [h.f.fake_alloc_bytes(i) for i in h.live()] == [1 << 18]
+    assert len(go(511, 1 << 22)) == 2 and len(go(511, 200000)) == 2
     assert len(h.live()) == 1
-    assert ["k_softmax_row" in n for n in go(5000, 32000)] == [True]    # rows enough
-    assert ["k_softmax_row" in n for n in go(3, 4000)] == [True]        # one part
+    assert ["k_softmax_row" in n for n in go(512, 40000)] == [True]     # rows enough
+    for n in (1, 4096, 4097, 8192, 8193, 16384, 16385, 32768):
+        assert ["k_softmax_held" in name for name in go(3, n)] == [True]
+    assert len(h.live()) == 1
 
 
 CHECKS = [n for n in dir() if n.startswith("check_")]
