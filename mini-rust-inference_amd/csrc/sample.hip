@@ -210,9 +210,12 @@ __global__ __launch_bounds__(kPartThreads) void k_softmax_write(const float *x, 
 // ---- verification of drafted tokens ----------------------------------------------
 // One workgroup a sequence.  The acceptance tests are products of two floats
 // in f64, which are exact.  The row that the token is drawn from is summed in f64 by
-// chunks, a chunk a wave at a time, eight values a lane in flight; the chunk in
+// chunks, a chunk a wave at a time, sixteen values a lane in flight; the chunk in
 // which the cumulative sum passes the target is read again, a value a thread, until
 // it is no longer than the workgroup.
+// 4 drafts of 32000 tokens: 9 us, the latency of the loads in turn (ids, their
+// probabilities, the row, the chunk).  64 x 7 of 100003: 16.4 us, what 64 CUs can
+// read (3.1 TB/s); the next 1024 loaded ahead takes 18.6.
 struct Residual {
     const float *p, *q;  // q null: nothing is taken away, or 1 at `hot`
     size_t hot;
@@ -227,56 +230,91 @@ struct Residual {
 
 constexpr int kVerWaves = 16, kVerThreads = kVerWaves * kWave, kVerChunks = 128;
 
-__device__ inline double wave_sum_f64(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+// Another lane's value, as DPP control CTRL picks it in the rows ROWS; 0 elsewhere.
+template <int CTRL, int ROWS>
+__device__ inline double dpp_f64(double v) {
+    const int2 x = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(
+        double, int2{__builtin_amdgcn_update_dpp(0, x.x, CTRL, ROWS, 0xf, false),
+                     __builtin_amdgcn_update_dpp(0, x.y, CTRL, ROWS, 0xf, false)});
+}
+__device__ inline double read_lane_f64(double v, int l) {
+    const int2 x = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(
+        double, int2{__builtin_amdgcn_readlane(x.x, l), __builtin_amdgcn_readlane(x.y, l)});
+}
+// Sums of the lanes up to each: in rows of 16, then over the rows before.  (Moves
+// between lanes through LDS: 10.1 and 18.5 us a call for 8.9 and 17.4.)
+__device__ inline double wave_scan_f64(double v) {
+    v += dpp_f64<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_f64<0x112, 0xf>(v);
+    v += dpp_f64<0x114, 0xf>(v);
+    v += dpp_f64<0x118, 0xf>(v);
+    v += dpp_f64<0x142, 0xa>(v);  // lane 15 to row 1, 47 to row 3
+    v += dpp_f64<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
     return v;
 }
+__device__ inline double wave_sum_f64(double v) { return read_lane_f64(wave_scan_f64(v), 63); }
 // The first lane at which base and the lanes' values so far exceed the goal, or the
 // last one with a value; base becomes the sum before it.
 __device__ inline int find_lane(double v, double goal, double *base) {
-    const int lane = threadIdx.x % kWave;
-    double c = v;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const double y = __shfl_up(c, o, kWave);
-        if (lane >= o) c += y;
-    }
+    const double c = wave_scan_f64(v);
     const unsigned long long mass = __ballot(v > 0.0),
                              over = __ballot(v > 0.0 && *base + c > goal);
     const int l = over ? __ffsll((long long)over) - 1 : mass ? 63 - __clzll((long long)mass) : 0;
-    const double before = __shfl(c, max(l - 1, 0), kWave);
-    if (l > 0) *base += before;
+    if (l > 0) *base += read_lane_f64(c, l - 1);
     return l;
 }
 
-// A lane's share of the sum over [lo, hi), 4 values at 4 (lane + 64 u).
-template <bool Q>
-__device__ inline double lane_sum(const Residual &r, size_t lo, size_t hi, int lane) {
-    constexpr int U = 2;  // (four: registers spill; 64 x 7 of 100003 take 21.3 us, not 20.1)
-    double s = 0.0;
-    size_t i0 = lo;
-    for (; i0 + 4 * U * kWave <= hi; i0 += 4 * U * kWave) {
-        float4u p[U], q[U];
+// A lane's sixteen values of 1024, 4 at 4 (lane + 64 u).
+struct VerBlock {
+    float4u p[4], q[4];
+    // zeros from hi on
+    __device__ void load(const Residual &r, size_t i0, size_t hi, int lane) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const size_t i = i0 + 4 * (u * kWave + lane);
-            p[u] = *reinterpret_cast<const float4u *>(r.p + i);
-            if (Q) q[u] = *reinterpret_cast<const float4u *>(r.q + i);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                double v = (double)p[u][j];
-                if (Q) v = v - (double)q[u][j];
-                else if (i0 + 4 * (u * kWave + lane) + j == r.hot) v = v - 1.0;
-                s += Residual::pos(v);
-            }
+        for (int u = 0; u < 4; ++u) p[u] = q[u] = float4u{0.0f, 0.0f, 0.0f, 0.0f};
+        load_row(p, r.p, i0, hi, lane);
+        if (r.q) load_row(q, r.q, i0, hi, lane);
     }
-    for (size_t i = i0 + lane; i < hi; i += kWave) s += r(i);
-    return s;
-}
+    static __device__ void load_row(float4u (&v)[4], const float *x, size_t i0, size_t hi,
+                                    int lane) {
+        if (i0 + 1024 <= hi) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                v[u] = *reinterpret_cast<const float4u *>(x + i0 + 4 * (u * kWave + lane));
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const size_t i = i0 + 4 * (u * kWave + lane) + j;
+                    if (i < hi) v[u][j] = x[i];
+                }
+        }
+    }
+    __device__ double sum() const {
+        double s = 0.0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                s += Residual::pos((double)p[u][j] - (double)q[u][j]);
+        return s;
+    }
+    // Takes out the value that 1 is taken from, if it is the lane's: what is left of it.
+    __device__ double take(size_t hot, int lane) {
+        double s = 0.0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (4 * (u * kWave + lane) + j == (int)hot) {
+                    s = Residual::pos((double)p[u][j] - 1.0);
+                    p[u][j] = 0.0f;
+                }
+        return s;
+    }
+};
 
 __global__ __launch_bounds__(kVerThreads) void k_verify(
     const uint32_t *__restrict__ drafts, const float *__restrict__ dp,
@@ -290,6 +328,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify(
     const unsigned count = n_drafts ? min(n_drafts[b], k) : k;
     const uint32_t *x = drafts + b * k;
     const float *u = us + b * (k + 1);
+    const double draw = (double)u[k];
     if (threadIdx.x == 0) {
         s_first = count;
         s_tok = MRI_NO_TOKEN;
@@ -311,43 +350,43 @@ __global__ __launch_bounds__(kVerThreads) void k_verify(
         if (dp) r.q = dp + (b * k + a) * n;
         else r.hot = x[a];
     }
-    // the sums of the chunks of [lo, hi), `len` values each (whole 1024s), zeros past them; all waves return their total
-    size_t lo = 0, hi = n, len = 0;
-    auto sums = [&]() {
-        len = ((hi - lo + kVerChunks - 1) / kVerChunks + kVerThreads - 1) / kVerThreads *
-              kVerThreads;
+    double goal = -1.0, base = 0.0;  // (below 0: the total is not known yet)
+    size_t lo = 0, hi = n;
+    for (;;) {
+        // the sums of the chunks of [lo, hi), `len` values each (whole 1024s), zeros past them;
+        const size_t len = ((hi - lo + kVerChunks - 1) / kVerChunks + 1023) / 1024 * 1024;
         __syncthreads();
         for (int c = wv; c < kVerChunks; c += kVerWaves) {
             const size_t l0 = min(lo + c * len, hi), l1 = min(l0 + len, hi);
             double s = 0.0;
-            if (l0 < l1)
-                s = wave_sum_f64(r.q ? lane_sum<true>(r, l0, l1, lane)
-                                     : lane_sum<false>(r, l0, l1, lane));
+            for (size_t i = l0; i < l1; i += 1024) {
+                VerBlock cur;
+                cur.load(r, i, hi, lane);
+                if (r.hot - i < 1024) s += cur.take(r.hot - i, lane);
+                s += cur.sum();
+            }
+            if (l0 < l1) s = wave_sum_f64(s);
             if (lane == 0) s_sum[c] = s;
         }
         __syncthreads();
-        return wave_sum_f64(s_sum[2 * lane] + s_sum[2 * lane + 1]);
-    };
-    double total = sums();
-    if (a < count && !(total > 0.0)) {  // the draft covers the target: draw from the target
-        r.q = nullptr;
-        r.hot = n;
-        total = sums();
-    }
-    if (total > 0.0) {
-        const double goal = (double)u[k] * total;
-        double base = 0.0;
-        for (;;) {
-            const double c0 = s_sum[2 * lane], c1 = s_sum[2 * lane + 1];
-            const int l = find_lane(c0 + c1, goal, &base);
-            const double f0 = __shfl(c0, l, kWave), f1 = __shfl(c1, l, kWave);
-            const bool second = f1 > 0.0 && !(f0 > 0.0 && base + f0 > goal);
-            if (second) base += f0;
-            lo = lo + (size_t)(2 * l + second) * len;
-            hi = min(lo + len, hi);
-            if (hi - lo <= kVerThreads) break;
-            (void)sums();
+        const double c0 = s_sum[2 * lane], c1 = s_sum[2 * lane + 1];
+        if (goal < 0.0) {
+            const double total = wave_sum_f64(c0 + c1);
+            if (!(total > 0.0)) {
+                if (!(a < count) || (!r.q && r.hot == n)) break;  // no mass
+                r.q = nullptr;  // the draft covers the target: draw from the target
+                r.hot = n;
+                continue;
+            }
+            goal = draw * total;
         }
+        const int l = find_lane(c0 + c1, goal, &base);
+        const double f0 = read_lane_f64(c0, l), f1 = read_lane_f64(c1, l);
+        const bool second = f1 > 0.0 && !(f0 > 0.0 && base + f0 > goal);
+        if (second) base += f0;
+        lo = lo + (size_t)(2 * l + second) * len;
+        hi = min(lo + len, hi);
+        if (hi - lo > kVerThreads) continue;
         // a value a thread: the wave that passes the goal, then its lane
         const size_t i = lo + threadIdx.x;
         const double v = i < hi ? r(i) : 0.0;
@@ -360,6 +399,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify(
             const int l = find_lane(v, goal, &base);
             if (lane == 0) s_tok = (unsigned)(lo + wv * kWave + l);
         }
+        break;
     }
     __syncthreads();
     for (unsigned i = threadIdx.x; i <= k; i += kVerThreads)
