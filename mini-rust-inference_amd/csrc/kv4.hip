@@ -222,7 +222,8 @@ __global__ __launch_bounds__(256) void k_kv4_append(Kv4Rows a, const float *__re
 
 // ---- read ---------------------------------------------------------------------------
 // A workgroup a page: a thread takes eight dims of a key from one K dword at a time,
-// then eight keys of four dims from four V dwords.
+// then eight keys of four dims from four V dwords.  Bound by its stores: 537 MB of
+// f32 in 140 us (3.8 TB/s; non-temporal stores 180).
 template <int HD, bool V4>
 __global__ __launch_bounds__(256) void k_kv4_read(Kv4Rows a, size_t layer_bytes,
                                                   float *__restrict__ k, float *__restrict__ v,
@@ -794,6 +795,8 @@ constexpr int wgs_of(int hd) { return hd == 128 ? 1 : 3; }
 // (m, l, o) in `part` by device-scope stores that are complete before it counts
 // itself on the tile's counter; the one that counts last joins them in the order
 // of the runs and leaves the counter zero, so none waits for another.
+// A token of 32 heads over 8 of 128, 8 sequences of 32768 keys: 47 us for 196 MB of
+// pages (4.1 TB/s, 90 % of a large copy's rate).
 template <int HD, bool FEW, bool SPLIT>
 __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     Kv4Rows a, const float *__restrict__ q, size_t qs, bool vec, int groups, int n_qt,
@@ -963,7 +966,10 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
 // a tile of 16 a wave.  The waves turn each page's quants into f16 operands once,
 // a quarter each, and read them from LDS in the operands' order; the next page
 // comes in while this one is computed, into a second buffer (one barrier a page).
-// The workgroups with the most pages start first.
+// The workgroups with the most pages start first.  1999 rows of 32 heads of 128:
+// 124 us, 57 of them the products (both halves) at a large product's rate; the rest
+// is VALU work (unpacking, softmax, p d_v) that two waves a SIMD hide in part.
+// Eight waves a workgroup: 129.
 constexpr int kPromptWaves = 4;
 template <int HD>
 struct LdsPage {
@@ -1086,6 +1092,10 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
 // through LDS.  Where pages alone do not fill the CUs, n_parts workgroups take
 // every n_parts-th batch of four tiles, and the one that is done last adds their
 // sums in order: each key has one writer and one order of sums.
+// 1999 rows of 32 heads of 128: 91 us; scores alone are 29 at the rate of a large
+// product.  Two waves a SIMD (registers) wait for their products and the scales'
+// turns; eight waves to a tile batch 103, blocks outermost 98 (more chains, 219
+// registers), three waves a SIMD without tiles loaded ahead 102.
 constexpr int kWtWaves = 4;
 template <int HD>
 __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
@@ -1267,6 +1277,7 @@ __device__ inline unsigned weight_key(float w) {
 // exponent alone would put most weights on a few counters), then the positions
 // above it and the first of those equal to it, in order: each wave counts and
 // writes contiguous positions.  Up to 32768 weights are read once, into registers.
+// 256 rows of 2304: 13 us, three passes' latency; 128 of 32768: 23 us.
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / kWave, kSelBins = 2048;
 constexpr int kSelRegs = 32;
 template <bool REGS>
@@ -1582,7 +1593,11 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
         constexpr bool FEW = decltype(few_)::value;
         constexpr int NQ = QTile<HD, FEW>::NQ;
         const size_t n_qt = (n_q + NQ - 1) / NQ, tiles = n_qt * a.n_kv;
-        // a call with tiles for less than half of the CUs splits its keys
+        // A call with tiles for half of the CUs or less splits its keys.  A token of 32
+        // heads over 8 at 4000 keys: head dim 128, 1 sequence 14 us against 30, 16
+        // sequences 24 against 32, 24 sequences 31 against 32; head dim 64, 24 21
+        // against 23, 48 31 against 34, 72 49 against 46.  (At 500 keys the join
+        // costs a call 0.7 us: the positions may be the device's.)
         const size_t fill = std::min<size_t>(wgs_of(HD) * cus, kKv4PartTiles);
         if (tiles * a.n_seqs * 2 <= fill) {
             const size_t slots = fill / tiles;
@@ -1599,6 +1614,10 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
         MRI_LAUNCHED("k_kv4_attend");
         return MRI_OK;
     };
+    // Shared pages where they give every CU a workgroup.  32 heads of 128: 256 rows
+    // (half of the CUs) 20 us against 17, 512 rows 28 against 35, 1024 47 against 78,
+    // 1536 81 against 131; behind 4000 keys 256 rows 137 against 71, 512 145 against
+    // 131, 1024 220 against 269.
     const size_t n_qg = (n_q + kPromptWaves * 16 - 1) / (kPromptWaves * 16);
     const size_t prompt_wgs = n_qg * a.n_kv * a.n_seqs;
     if (n_q > 32 && prompt_wgs >= cus) {
@@ -1618,6 +1637,7 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
         const size_t n_grp = (n_pg + kWtWaves - 1) / kWtWaves;
         const size_t groups_all = n_grp * a.n_kv * a.n_seqs;
         // parts of the queries: three workgroups a CU, four query tiles a part at least
+        // (1999 rows of 32 heads of 128: 91 us; 98 to 114 with two or four a CU)
         size_t parts = 3 * cus / groups_all;
         parts = std::min(parts, ((n_q + 15) / 16 + kWtWaves - 1) / kWtWaves);
         parts = std::max<size_t>(1, std::min<size_t>(parts, 16));
