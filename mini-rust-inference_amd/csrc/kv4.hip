@@ -380,15 +380,6 @@ __device__ inline float block_max(float v) {
     return v;
 }
 
-__device__ inline float quad_max(float v) {  // over four neighbouring lanes
-    const auto swap = [](float x, auto perm) __attribute__((always_inline)) {
-        return __uint_as_float(__builtin_amdgcn_update_dpp(
-            0, __float_as_uint(x), decltype(perm)::value, 0xf, 0xf, true));
-    };
-    v = fmaxf(v, swap(v, std::integral_constant<int, 0xb1>{}));  // lanes 1, 0, 3, 2
-    return fmaxf(v, swap(v, std::integral_constant<int, 0x4e>{}));  // lanes 2, 3, 0, 1
-}
-
 // A tile's columns are 16 queries; with FEW they are 16 / NB queries times the NB
 // blocks of the head dim, column b * 16 / NB + query.  Such a column holds its own
 // block of the query only, so the products with all of K's blocks leave its block's
@@ -419,24 +410,32 @@ struct QRaw {
         }
     }
 };
+// Queries are scaled by 2^e: the row's largest magnitude to [2^14, 2^15).
+__device__ inline int up_exponent(float mx) {
+    return mx > 0.0f && mx < INFINITY ? min(14 - ilogbf(mx), 120) : 0;
+}
+// What the raw products are multiplied by (log2 units): 2^(9 - e) log2(e) / sqrt(HD),
+// rounded once.
+template <int HD>
+__device__ inline float score_scale(int e) {
+    constexpr float c = HD == 64 ? 0.18033688011112042592f : 0.12751743021347021697f;
+    return ldexpf(c, 9 - e);
+}
 template <int HD, bool FEW>
 struct QTile {
     using R = QRaw<HD, FEW>;
     static constexpr int NB = HD / 32, NQ = R::NQ, N = R::N;
     half8_t hi[NB], lo[NB];
     float inv;  // what the raw products are multiplied by (log2 units)
-    // QUAD: a column's four lanes are neighbours
-    template <bool QUAD = false>
     __device__ void make(const R &raw, int lane) {
         float mx = 0.0f;
 #pragma unroll
         for (int b = 0; b < N; ++b)
 #pragma unroll
             for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(raw.x[b][j]));
-        mx = QUAD ? quad_max(mx) : col_max(mx);
+        mx = col_max(mx);
         if constexpr (FEW) mx = block_max<NB>(mx);
-        // the row's largest magnitude to [2^14, 2^15)
-        const int e = mx > 0.0f && mx < INFINITY ? min(14 - ilogbf(mx), 120) : 0;
+        const int e = up_exponent(mx);
         const float up = ldexpf(1.0f, e);
 #pragma unroll
         for (int b = 0; b < N; ++b) {
@@ -454,9 +453,7 @@ struct QTile {
                 lo[b] = b == own ? l : z;
             }
         }
-        // 2^9 log2(e) / sqrt(HD), rounded once
-        constexpr float c = HD == 64 ? 0.18033688011112042592f : 0.12751743021347021697f;
-        inv = ldexpf(c, 9 - e);
+        inv = score_scale<HD>(e);
     }
 };
 
@@ -1092,11 +1089,64 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
 // through LDS.  Where pages alone do not fill the CUs, n_parts workgroups take
 // every n_parts-th batch of four tiles, and the one that is done last adds their
 // sums in order: each key has one writer and one order of sums.
-// 1999 rows of 32 heads of 128: 91 us; scores alone are 29 at the rate of a large
+// 1999 rows of 32 heads of 128: 76 us; scores alone are 29 at the rate of a large
 // product.  Two waves a SIMD (registers) wait for their products and the scales'
 // turns; eight waves to a tile batch 103, blocks outermost 98 (more chains, 219
 // registers), three waves a SIMD without tiles loaded ahead 102.
 constexpr int kWtWaves = 4;
+// A tile's 16 rows on their way to LDS, as a load takes four of them: sixteen lanes a
+// row, four dims of each 64.  (Whole lines a load: with a row's dims over four lanes,
+// 16 half lines a load, issuing the loads takes as long as the products: 91 us, not 76.)
+template <int HD>
+struct QRows {
+    static constexpr int N = HD / 64;
+    float4_t x[4][N];
+    // src null: an empty row
+    __device__ void load(int i, const float *src, int l, bool vec) {
+#pragma unroll
+        for (int h = 0; h < N; ++h) {
+            const float *p = src + 64 * h + 4 * l;
+            if (!src) {
+                x[i][h] = float4_t{0, 0, 0, 0};
+            } else if (vec) {
+                x[i][h] = *reinterpret_cast<const float4_t *>(p);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][h][j] = p[j];
+            }
+        }
+    }
+    // As the products take them: [block][hi, lo][lane group, row].
+    __device__ void store(half8_t (*to)[2][kWave], float *inv, int lane) const {
+        const int l = lane & 15;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 4 * i + (lane >> 4);
+            float mx = 0.0f;
+#pragma unroll
+            for (int h = 0; h < N; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fabsf(x[i][h][j]));
+            mx = fmaxf(mx, ror<8>(mx));
+            mx = fmaxf(mx, ror<4>(mx));
+            mx = fmaxf(mx, ror<2>(mx));
+            mx = fmaxf(mx, ror<1>(mx));
+            const int e = up_exponent(mx);
+            const float up = ldexpf(1.0f, e);
+#pragma unroll
+            for (int h = 0; h < N; ++h) {
+                half2_t hi[2], lo[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    split2(x[i][h][2 * u] * up, x[i][h][2 * u + 1] * up, &hi[u], &lo[u]);
+                half8_t *const at = &to[2 * h + (l >> 3)][0][(l >> 1 & 3) * 16 + row];
+                reinterpret_cast<uint2 *>(at)[l & 1] = __builtin_bit_cast(uint2, hi);
+                reinterpret_cast<uint2 *>(at + kWave)[l & 1] = __builtin_bit_cast(uint2, lo);
+            }
+            if (l == 0) inv[row] = score_scale<HD>(e);
+        }
+    }
+};
 template <int HD>
 __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
     Kv4Rows a, const float *__restrict__ q, size_t qs, bool vec, int groups, int n_grp,
@@ -1146,36 +1196,34 @@ __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
     const int qt0 = (key0 > p0 ? (int)(key0 - p0) : 0) * groups / 16 / kWtWaves * kWtWaves;
     const int n_qt = (n_q + 15) / 16, step = n_parts * kWtWaves;
     const int last = ((n_qt - 1) / kWtWaves - mine) / n_parts * n_parts + mine;
-    QRaw<HD, false> raw;
+    QRows<HD> rows;
     float z_next = 0.0f;
     unsigned see_next = 0;
-    // (a column's four lanes are neighbours here, for whole lines a load)
-    const int fr = lane >> 2, fg = lane & 3;
     auto fetch = [&](int t) {
-        const int qi = t * 16 + fr, row = qi / groups;
-        const bool real = qi < n_q;
-        const int qh = head * groups + qi % groups;
-        raw.load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, fg, 0, vec);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned qi = t * 16 + 4 * i + g, row = qi / (unsigned)groups;
+            rows.load(i,
+                      qi < (unsigned)n_q ? q + row_index(a, b, row) * qs +
+                                               (head * groups + qi % (unsigned)groups) * HD
+                                         : nullptr,
+                      r, vec);
+        }
+        const unsigned qi = t * 16 + r, row = qi / (unsigned)groups;
+        const bool real = qi < (unsigned)n_q;
         see_next = real ? p0 + row + 1 : 0;
-        z_next = real ? lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] : 0.0f;
+        z_next = real ? lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + head * groups +
+                            qi % (unsigned)groups]
+                      : 0.0f;
     };
     const int q_last = (n_qt - 1) / kWtWaves >= mine ? last * kWtWaves : -1;
     if (q_last >= qt0) fetch(q_last + wv);
     for (int q0 = q_last; q0 >= qt0; q0 -= step) {
         const int nt = min(kWtWaves, n_qt - q0);
-        {
-            QTile<HD, false> qt;
-            qt.template make<true>(raw, lane);
-#pragma unroll
-            for (int c = 0; c < NB; ++c) {
-                s_q[wv][c][0][fg * 16 + fr] = qt.hi[c];
-                s_q[wv][c][1][fg * 16 + fr] = qt.lo[c];
-            }
-            if (fg == 0) {
-                s_inv[wv][fr] = qt.inv;
-                s_z[wv][fr] = z_next;
-                s_see[wv][fr] = see_next;
-            }
+        rows.store(s_q[wv], s_inv[wv], lane);
+        if (g == 0) {
+            s_z[wv][r] = z_next;
+            s_see[wv][r] = see_next;
         }
         __syncthreads();
         if (q0 - step >= qt0) fetch(q0 - step + wv);
