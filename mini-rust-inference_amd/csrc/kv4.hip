@@ -1089,7 +1089,7 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
 // through LDS.  Where pages alone do not fill the CUs, n_parts workgroups take
 // every n_parts-th batch of four tiles, and the one that is done last adds their
 // sums in order: each key has one writer and one order of sums.
-// 1999 rows of 32 heads of 128: 76 us; scores alone are 29 at the rate of a large
+// 1999 rows of 32 heads of 128: 71 us; scores alone are 29 at the rate of a large
 // product.  Two waves a SIMD (registers) wait for their products and the scales'
 // turns; eight waves to a tile batch 103, blocks outermost 98 (more chains, 219
 // registers), three waves a SIMD without tiles loaded ahead 102.
@@ -1116,7 +1116,11 @@ struct QRows {
             }
         }
     }
-    // As the products take them: [block][hi, lo][lane group, row].
+    // As the products take them: [block][hi, lo][at].  The groups' and blocks' rows
+    // are turned against each other, so that a store's lanes have banks of their own.
+    static __device__ int at(int block, int g, int row) {
+        return 16 * g + (row ^ 4 * g ^ 2 * (block & 1));
+    }
     __device__ void store(half8_t (*to)[2][kWave], float *inv, int lane) const {
         const int l = lane & 15;
 #pragma unroll
@@ -1139,9 +1143,9 @@ struct QRows {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     split2(x[i][h][2 * u] * up, x[i][h][2 * u + 1] * up, &hi[u], &lo[u]);
-                half8_t *const at = &to[2 * h + (l >> 3)][0][(l >> 1 & 3) * 16 + row];
-                reinterpret_cast<uint2 *>(at)[l & 1] = __builtin_bit_cast(uint2, hi);
-                reinterpret_cast<uint2 *>(at + kWave)[l & 1] = __builtin_bit_cast(uint2, lo);
+                half8_t *const p = &to[2 * h + (l >> 3)][0][at(l >> 3, l >> 1 & 3, row)];
+                reinterpret_cast<uint2 *>(p)[l & 1] = __builtin_bit_cast(uint2, hi);
+                reinterpret_cast<uint2 *>(p + kWave)[l & 1] = __builtin_bit_cast(uint2, lo);
             }
             if (l == 0) inv[row] = score_scale<HD>(e);
         }
@@ -1200,16 +1204,18 @@ __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
     float z_next = 0.0f;
     unsigned see_next = 0;
     auto fetch = [&](int t) {
+        unsigned row = (t * 16 + g) / (unsigned)groups, col = (t * 16 + g) % (unsigned)groups;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const unsigned qi = t * 16 + 4 * i + g, row = qi / (unsigned)groups;
-            rows.load(i,
-                      qi < (unsigned)n_q ? q + row_index(a, b, row) * qs +
-                                               (head * groups + qi % (unsigned)groups) * HD
-                                         : nullptr,
+            const bool real = t * 16 + 4 * i + g < n_q;
+            rows.load(i, real ? q + row_index(a, b, row) * qs + (head * groups + col) * HD : nullptr,
                       r, vec);
+            row += 4 / groups;  // four queries on
+            col += 4 % groups;
+            if (col >= (unsigned)groups) ++row, col -= groups;
         }
-        const unsigned qi = t * 16 + r, row = qi / (unsigned)groups;
+        const unsigned qi = t * 16 + r;
+        row = qi / (unsigned)groups;
         const bool real = qi < (unsigned)n_q;
         see_next = real ? p0 + row + 1 : 0;
         z_next = real ? lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + head * groups +
@@ -1237,8 +1243,8 @@ __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
             half8_t hi[NB], lo[NB];
 #pragma unroll
             for (int c = 0; c < NB; ++c) {
-                hi[c] = s_q[u][c][0][lane];
-                lo[c] = s_q[u][c][1][lane];
+                hi[c] = s_q[u][c][0][rows.at(c, g, r)];
+                lo[c] = s_q[u][c][1][rows.at(c, g, r)];
             }
             float s[16];
 #pragma unroll
@@ -1685,7 +1691,7 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
         const size_t n_grp = (n_pg + kWtWaves - 1) / kWtWaves;
         const size_t groups_all = n_grp * a.n_kv * a.n_seqs;
         // parts of the queries: three workgroups a CU, four query tiles a part at least
-        // (1999 rows of 32 heads of 128: 91 us; 98 to 114 with two or four a CU)
+        // (1999 rows of 32 heads of 128: 76 us; two a CU 87, four 78, eight 90)
         size_t parts = 3 * cus / groups_all;
         parts = std::min(parts, ((n_q + 15) / 16 + kWtWaves - 1) / kWtWaves);
         parts = std::max<size_t>(1, std::min<size_t>(parts, 16));
