@@ -959,141 +959,6 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     }
 }
 
-// Prompts: a workgroup takes 64 queries of a KV head over all the pages they see,
-// a tile of 16 a wave.  The waves turn each page's quants into f16 operands once,
-// a quarter each, and read them from LDS in the operands' order; the next page
-// comes in while this one is computed, into a second buffer (one barrier a page).
-// The workgroups with the most pages start first.  1999 rows of 32 heads of 128:
-// 124 us, 57 of them the products (both halves) at a large product's rate; the rest
-// is VALU work (unpacking, softmax, p d_v) that two waves a SIMD hide in part.
-// Eight waves a workgroup: 129.
-constexpr int kPromptWaves = 4;
-template <int HD>
-struct LdsPage {
-    static constexpr int NB = HD / 32;
-    half8_t k[4][NB][kWave];
-    half8_t v[HD / 16][2][kWave];
-    unsigned d[2][kScaleWords<HD>];
-};
-template <int HD>
-struct LdsSrc {
-    const LdsPage<HD> &p;
-    int lane;
-    __device__ half8_t kop(int t, int b) const { return p.k[t][b][lane]; }
-    __device__ half8_t vop(int e, int h) const { return p.v[e][h][lane]; }
-    __device__ unsigned vscale(int u) const { return p.d[1][lane * (HD / 64) + u]; }
-};
-// What a thread holds of a page on its way to LDS: K tile `wave`, V chunk `wave`
-// (head dim 64: the first two waves), and the first wave K's scales, the second V's.
-template <int HD>
-struct PagePart {
-    using P = Page<HD>;
-    static constexpr int NB = HD / 32;
-    unsigned k[NB], v[4], d[NB / 2];
-    __device__ void load(const uint8_t *pb, int wv, int lane) {
-        const uint8_t *kp = pb + wv * 8 * HD + lane * 4 * NB;
-        if constexpr (HD == 128) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(kp);
-            k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
-        } else {
-            const uint2 x = *reinterpret_cast<const uint2 *>(kp);
-            k[0] = x.x, k[1] = x.y;
-        }
-        if (wv < NB) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(pb + P::kV + wv * 1024 + lane * 16);
-            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-        }
-        if (wv < 2) PageLoad<HD>::load_scales(pb + (wv ? P::kVs : P::kKs), lane, d);
-    }
-    __device__ void store(LdsPage<HD> &p, int wv, int lane) const {
-#pragma unroll
-        for (int b = 0; b < NB; ++b) p.k[wv][b][lane] = quants(k[b]);
-        if (wv < NB) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p.v[2 * wv + (i >> 1)][i & 1][lane] = quants(v[i]);
-        }
-        if (wv < 2) PageLoad<HD>::stage(d, lane, p.d[wv]);
-    }
-};
-
-template <int HD>
-__global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
-    Kv4Rows a, const float *__restrict__ q, size_t qs, bool vec, int groups, int n_qg,
-    float *__restrict__ out, size_t os, float *__restrict__ lse) {
-    using P = Page<HD>;
-    constexpr int QW = kPromptWaves * 16;  // queries of a workgroup
-    __shared__ LdsPage<HD> s_p[2];
-    const int lane = threadIdx.x & 63, wv = wave_id(), g = lane >> 4, r = lane & 15;
-    unsigned x = blockIdx.x;
-    const int head = x % a.n_kv;
-    x /= a.n_kv;
-    const int b = x % a.n_seqs, qg = n_qg - 1 - (int)(x / a.n_seqs);
-    unsigned p0;
-    const int cnt = (int)rows_of(a, b, &p0);
-    const int n_q = cnt * groups;
-    if (qg * QW >= n_q) return;
-    const unsigned n_pg = (p0 + (min(qg * QW + QW, n_q) - 1) / groups) / kPageKeys + 1;
-    const uint8_t *base =
-        a.pages + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages * P::kBytes;
-    PagePart<HD> next;
-    next.load(base, wv, lane);
-    const int q0 = qg * QW + wv * 16, qi = q0 + r, row = qi / groups;
-    const bool real = qi < n_q;
-    const int qh = head * groups + qi % groups;
-    QTile<HD, false> qtile;
-    {
-        QRaw<HD, false> raw;
-        raw.load(real ? q + row_index(a, b, row) * qs + qh * HD : nullptr, g, 0, vec);
-        qtile.make(raw, lane);
-    }
-    const long see = real ? (long)p0 + row + 1 : 0;  // keys this column sees
-    // keys every real column of the wave sees
-    const unsigned all = q0 < n_q ? p0 + q0 / groups + 1 : 0;
-    // pages that the wave's last row sees
-    const unsigned my_pg =
-        q0 < n_q ? (p0 + (min(q0 + 16, n_q) - 1) / groups) / kPageKeys + 1 : 0;
-    const unsigned end = q0 < n_q ? p0 + (min(q0 + 16, n_q) - 1) / groups + 1 : 0;
-    Softmax<HD> st;
-    next.store(s_p[0], wv, lane);
-    __syncthreads();
-    for (unsigned pg = 0; pg < n_pg; ++pg) {
-        const LdsSrc<HD> src{s_p[pg & 1], lane};
-        if (pg + 1 < n_pg) next.load(base + (size_t)(pg + 1) * P::kBytes, wv, lane);
-        const int lim = (int)min(see - (long)pg * kPageKeys, 64l);
-        if ((pg + 1) * kPageKeys <= all)
-            attend_page<HD, false, true>(src, src.p.d[0], src.p.d[1], lane, qtile, lim, 64, st);
-        else if (pg < my_pg)
-            attend_page<HD, false, false>(src, src.p.d[0], src.p.d[1], lane, qtile, lim,
-                                          (int)min(end - pg * kPageKeys, 64u), st);
-        if (pg + 1 < n_pg) next.store(s_p[(pg + 1) & 1], wv, lane);
-        __syncthreads();
-    }
-    const float l = col_sum(st.l);
-    if (!real) return;
-    // l and o share their power of two; o holds 2^-9 of the quants
-    float *to = out + row_index(a, b, row) * os + qh * HD + 4 * g;
-    const float inv = 0x1p9f / l;
-#pragma unroll
-    for (int e = 0; e < HD / 16; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) to[16 * e + i] = st.o[e][i] * inv;
-    if (lse && g == 0)
-        lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] =
-            st.m + __log2f(l * ldexpf(1.0f, st.ve - kUp));
-}
-
-// The keys' attention weights: a wave a page of a KV head goes over all the
-// queries that see it, with the scores of the attention itself and the rows'
-// log-sum-exps; the page's quants stay in its registers.  The four waves of a
-// workgroup (consecutive pages) prepare a query tile each and share the four
-// through LDS.  Where pages alone do not fill the CUs, n_parts workgroups take
-// every n_parts-th batch of four tiles, and the one that is done last adds their
-// sums in order: each key has one writer and one order of sums.
-// 1999 rows of 32 heads of 128: 71 us; scores alone are 29 at the rate of a large
-// product.  Two waves a SIMD (registers) wait for their products and the scales'
-// turns; eight waves to a tile batch 103, blocks outermost 98 (more chains, 219
-// registers), three waves a SIMD without tiles loaded ahead 102.
-constexpr int kWtWaves = 4;
 // A tile's 16 rows on their way to LDS, as a load takes four of them: sixteen lanes a
 // row, four dims of each 64.  (Whole lines a load: with a row's dims over four lanes,
 // 16 half lines a load, issuing the loads takes as long as the products: 91 us, not 76.)
@@ -1151,6 +1016,163 @@ struct QRows {
         }
     }
 };
+
+// Prompts: a workgroup takes 64 queries of a KV head over all the pages they see,
+// a tile of 16 a wave.  The waves turn each page's quants into f16 operands once,
+// a quarter each, and read them from LDS in the operands' order; the next page
+// comes in while this one is computed, into a second buffer (one barrier a page).
+// The workgroups with the most pages start first.  1999 rows of 32 heads of 128:
+// 123 us, 57 of them the products (both halves) at a large product's rate; the rest
+// is VALU work (unpacking, softmax, p d_v) that two waves a SIMD hide in part, and
+// each workgroup's first loads (5 us).
+// Eight waves a workgroup: 129.
+constexpr int kPromptWaves = 4;
+template <int HD>
+struct LdsPage {
+    static constexpr int NB = HD / 32;
+    half8_t k[4][NB][kWave];
+    half8_t v[HD / 16][2][kWave];
+    unsigned d[2][kScaleWords<HD>];
+};
+template <int HD>
+struct LdsSrc {
+    const LdsPage<HD> &p;
+    int lane;
+    __device__ half8_t kop(int t, int b) const { return p.k[t][b][lane]; }
+    __device__ half8_t vop(int e, int h) const { return p.v[e][h][lane]; }
+    __device__ unsigned vscale(int u) const { return p.d[1][lane * (HD / 64) + u]; }
+};
+// What a thread holds of a page on its way to LDS: K tile `wave`, V chunk `wave`
+// (head dim 64: the first two waves), and the first wave K's scales, the second V's.
+template <int HD>
+struct PagePart {
+    using P = Page<HD>;
+    static constexpr int NB = HD / 32;
+    unsigned k[NB], v[4], d[NB / 2];
+    __device__ void load(const uint8_t *pb, int wv, int lane) {
+        const uint8_t *kp = pb + wv * 8 * HD + lane * 4 * NB;
+        if constexpr (HD == 128) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(kp);
+            k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2 *>(kp);
+            k[0] = x.x, k[1] = x.y;
+        }
+        if (wv < NB) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(pb + P::kV + wv * 1024 + lane * 16);
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        }
+        if (wv < 2) PageLoad<HD>::load_scales(pb + (wv ? P::kVs : P::kKs), lane, d);
+    }
+    __device__ void store(LdsPage<HD> &p, int wv, int lane) const {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) p.k[wv][b][lane] = quants(k[b]);
+        if (wv < NB) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p.v[2 * wv + (i >> 1)][i & 1][lane] = quants(v[i]);
+        }
+        if (wv < 2) PageLoad<HD>::stage(d, lane, p.d[wv]);
+    }
+};
+
+template <int HD>
+__global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
+    Kv4Rows a, const float *__restrict__ q, size_t qs, bool vec, int groups, int n_qg,
+    float *__restrict__ out, size_t os, float *__restrict__ lse) {
+    using P = Page<HD>;
+    constexpr int QW = kPromptWaves * 16;  // queries of a workgroup
+    constexpr int NB = P::NB;
+    __shared__ LdsPage<HD> s_p[2];
+    __shared__ float s_inv[kPromptWaves][16];
+    const int lane = threadIdx.x & 63, wv = wave_id(), g = lane >> 4, r = lane & 15;
+    unsigned x = blockIdx.x;
+    const int head = x % a.n_kv;
+    x /= a.n_kv;
+    const int b = x % a.n_seqs, qg = n_qg - 1 - (int)(x / a.n_seqs);
+    unsigned p0;
+    const int cnt = (int)rows_of(a, b, &p0);
+    const int n_q = cnt * groups;
+    if (qg * QW >= n_q) return;
+    const unsigned n_pg = (p0 + (min(qg * QW + QW, n_q) - 1) / groups) / kPageKeys + 1;
+    const uint8_t *base =
+        a.pages + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages * P::kBytes;
+    PagePart<HD> next;
+    next.load(base, wv, lane);
+    const int q0 = qg * QW + wv * 16, qi = q0 + r, row = qi / groups;
+    const bool real = qi < n_q;
+    const int qh = head * groups + qi % groups;
+    // the queries pass through the second page's place
+    static_assert(sizeof(half8_t) * kPromptWaves * NB * 2 * kWave <= sizeof(LdsPage<HD>));
+    half8_t(*const s_q)[2][kWave] = reinterpret_cast<half8_t(*)[2][kWave]>(&s_p[1]) + wv * NB;
+    {
+        QRows<HD> rows;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = q0 + 4 * i + g;
+            rows.load(i,
+                      at < n_q ? q + row_index(a, b, at / groups) * qs +
+                                     (head * groups + at % groups) * HD
+                               : nullptr,
+                      r, vec);
+        }
+        rows.store(s_q, s_inv[wv], lane);
+    }
+    const long see = real ? (long)p0 + row + 1 : 0;  // keys this column sees
+    // keys every real column of the wave sees
+    const unsigned all = q0 < n_q ? p0 + q0 / groups + 1 : 0;
+    // pages that the wave's last row sees
+    const unsigned my_pg =
+        q0 < n_q ? (p0 + (min(q0 + 16, n_q) - 1) / groups) / kPageKeys + 1 : 0;
+    const unsigned end = q0 < n_q ? p0 + (min(q0 + 16, n_q) - 1) / groups + 1 : 0;
+    Softmax<HD> st;
+    next.store(s_p[0], wv, lane);
+    __syncthreads();
+    QTile<HD, false> qtile;
+#pragma unroll
+    for (int c = 0; c < NB; ++c) {
+        qtile.hi[c] = s_q[c][0][QRows<HD>::at(c, g, r)];
+        qtile.lo[c] = s_q[c][1][QRows<HD>::at(c, g, r)];
+    }
+    qtile.inv = s_inv[wv][r];
+    __syncthreads();
+    for (unsigned pg = 0; pg < n_pg; ++pg) {
+        const LdsSrc<HD> src{s_p[pg & 1], lane};
+        if (pg + 1 < n_pg) next.load(base + (size_t)(pg + 1) * P::kBytes, wv, lane);
+        const int lim = (int)min(see - (long)pg * kPageKeys, 64l);
+        if ((pg + 1) * kPageKeys <= all)
+            attend_page<HD, false, true>(src, src.p.d[0], src.p.d[1], lane, qtile, lim, 64, st);
+        else if (pg < my_pg)
+            attend_page<HD, false, false>(src, src.p.d[0], src.p.d[1], lane, qtile, lim,
+                                          (int)min(end - pg * kPageKeys, 64u), st);
+        if (pg + 1 < n_pg) next.store(s_p[(pg + 1) & 1], wv, lane);
+        __syncthreads();
+    }
+    const float l = col_sum(st.l);
+    if (!real) return;
+    // l and o share their power of two; o holds 2^-9 of the quants
+    float *to = out + row_index(a, b, row) * os + qh * HD + 4 * g;
+    const float inv = 0x1p9f / l;
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[16 * e + i] = st.o[e][i] * inv;
+    if (lse && g == 0)
+        lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] =
+            st.m + __log2f(l * ldexpf(1.0f, st.ve - kUp));
+}
+
+// The keys' attention weights: a wave a page of a KV head goes over all the
+// queries that see it, with the scores of the attention itself and the rows'
+// log-sum-exps; the page's quants stay in its registers.  The four waves of a
+// workgroup (consecutive pages) prepare a query tile each and share the four
+// through LDS.  Where pages alone do not fill the CUs, n_parts workgroups take
+// every n_parts-th batch of four tiles, and the one that is done last adds their
+// sums in order: each key has one writer and one order of sums.
+// 1999 rows of 32 heads of 128: 71 us; scores alone are 29 at the rate of a large
+// product.  Two waves a SIMD (registers) wait for their products and the scales'
+// turns; eight waves to a tile batch 103, blocks outermost 98 (more chains, 219
+// registers), three waves a SIMD without tiles loaded ahead 102.
+constexpr int kWtWaves = 4;
 template <int HD>
 __global__ __launch_bounds__(kWtWaves *kWave, 2) void k_kv4_weights(
     Kv4Rows a, const float *__restrict__ q, size_t qs, bool vec, int groups, int n_grp,
