@@ -55,9 +55,9 @@ def test_softmax(rows, n, temperature):
     assert np.array_equal(host(d), got)
 
 
-def test_softmax_special_rows():
+@pytest.mark.parametrize("n", [777, 9001, 30000, 40000])
+def test_softmax_special_rows(n):
     L, Q, torch = mods()
-    n = 777
     x = np.zeros((8, n), F32)
     x[0] = -np.inf                      # nothing left: zeros
     x[1], x[1, 5] = -np.inf, -3.0       # one left
@@ -160,6 +160,29 @@ def test_verify_borders():
     p[11, :, :200] = 0
     run_verify(drafts, p, u, q)
     run_verify(drafts, p, u)
+
+
+@pytest.mark.parametrize("n", [1, 1023, 1025, 2500, 4096, 140000])
+def test_verify_rejected_greedy_drafts(n):
+    """The rejected token leaves the target's row wherever it lies among its blocks;
+    where it held all the mass, or is no token, the target's row stays."""
+    rng = np.random.default_rng(n)
+    ids = np.unique([i for i in (0, 3, 1020, 1023, 1024, 2047, n // 2, n - 1) if i < n])
+    ids = np.concatenate([ids, [n, n + 7, 0xfffffffe]]).astype(np.uint32)
+    b = 2 * len(ids)
+    p = probs(rng, b, 2, n)
+    u = rng.random((b, 2)).astype(F32)
+    u[:, 0] = 1.0                                   # rejected unless p > 1
+    drafts = np.concatenate([ids, ids])[:, None]
+    p[len(ids):, 0] = 0                             # all mass at the draft
+    for i, x in enumerate(ids):
+        if x < n:
+            p[i, 0, x] = 0.75                       # (most of it: the rest is drawn)
+            p[len(ids) + i, 0, x] = 0.5
+    acc, tok = run_verify(drafts, p, u)
+    assert not acc.any()
+    for i, x in enumerate(ids):
+        assert tok[len(ids) + i, 0] == (x if x < n else R.NO_TOKEN)
 
 
 def test_verify_draws_the_targets_distribution():
