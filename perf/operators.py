@@ -165,18 +165,11 @@ def _values(g, seqs, rows, heads, hd):
     return x * (_randn(g, heads * hd) * 0.7).exp()
 
 
-def _library():
-    """The framework's binding (its folder's name is no package's)."""
-    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
-                      "mini-rust-inference_amd")
-    if at not in sys.path:
-        sys.path.insert(0, at)
-    import mri_llama
-    return mri_llama
-
-
 def _cache(layers, seqs, max_seq, kv_heads, head_dim):
-    return _library().Kv4Cache(layers, seqs, max_seq, kv_heads, head_dim)
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                                    "mini-rust-inference_amd"))
+    import mri_llama
+    return mri_llama.Kv4Cache(layers, seqs, max_seq, kv_heads, head_dim)
 
 
 def _raw(case, seed):
@@ -237,8 +230,6 @@ def prepare(case, seed):
     s = _raw(case, seed)
     op = case["op"]
     s["case"] = case
-    if own:
-        s["library"] = _library()
     for name in ("pos", "count", "lens", "n_drafts"):
         if s.get(name) is not None:
             s[name] = _int(s[name])
@@ -438,11 +429,12 @@ def run(s):
                          c["keep"], c["recent"], s["kept"])
         s["dst"].read(0, s["out"], s["out_v"], 0, count=s["new_lens"])
         return s["kept"], s["new_lens"], s["out_w"], s["out"], s["out_v"]
+    import mri_llama
     if op == "softmax":
-        s["library"].softmax(s["x"], s["out"], temperature=c["temperature"])
+        mri_llama.softmax(s["x"], s["out"], temperature=c["temperature"])
         return s["out"]
-    s["library"].verify_drafts(s["drafts"], s["target"], s["u"], s["tokens"], s["accepted"],
-                               draft_probs=s["draft"], n_drafts=s["n_drafts"])
+    mri_llama.verify_drafts(s["drafts"], s["target"], s["u"], s["tokens"], s["accepted"],
+                            draft_probs=s["draft"], n_drafts=s["n_drafts"])
     return s["tokens"], s["accepted"]
 
 
