@@ -228,7 +228,8 @@ mri_status mri_llama_forward_kv4(mri_llama *model, const uint32_t *tokens, size_
  * apart; out may be x): out = exp((x - max x) / temperature) / sum.  A row of
  * -inf only becomes zeros, one with NaN or +inf NaN.  Few rows of more than
  * 32768 logits are cut into parts, whose statistics pass through 256 KiB kept
- * per (device, stream); a call that is being captured uses none, takes longer
+ * per (device, stream), in two launches that no other thread's call on the
+ * stream comes between; a call that is being captured uses none, takes longer
  * and gives the same bits.
  * InvalidArgument unless temperature > 0 and finite; InvalidShape for n = 0 or a
  * stride below n. */

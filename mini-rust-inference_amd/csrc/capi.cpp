@@ -92,6 +92,18 @@ int device_cus() {
     return n;
 }
 
+static std::mutex g_turn_mu;
+static std::map<std::pair<int, hipStream_t>, std::recursive_mutex> g_turns;
+
+StreamTurn::StreamTurn(hipStream_t stream) {
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    std::unique_lock<std::mutex> lk(g_turn_mu);
+    std::recursive_mutex &turn = g_turns[{dev, stream}];
+    lk.unlock();
+    lk_ = std::unique_lock<std::recursive_mutex>(turn);
+}
+
 static std::mutex g_scratch_mu;
 static std::map<std::pair<int, hipStream_t>, Scratch> g_scratch;
 

@@ -195,6 +195,16 @@ class DeviceOnce {
 int device_cus();
 
 // ---- per-(device, stream) scratch ----------------------------------------
+// A call that takes memory of its stream holds the stream's turn until its last
+// launch: another thread's call on the stream does not put its launches in between.
+// (Recursive: entry points call others.)
+class StreamTurn {
+  public:
+    explicit StreamTurn(hipStream_t stream);
+
+  private:
+    std::unique_lock<std::recursive_mutex> lk_;
+};
 // Grow-only device buffer; growth synchronizes `stream` before freeing the
 // old buffer, so work already enqueued on it never sees freed memory.
 mri_status scratch_get(hipStream_t stream, size_t bytes, void **ptr);

@@ -434,6 +434,7 @@ mri_status launch_softmax(const float *x, size_t rows, size_t n, size_t x_stride
     // The parts' workspace is the stream's: a call that is being captured uses none,
     // so that graphs recorded on one stream may run side by side.
     if (rows < kSplitRows) {
+        const StreamTurn turn(s);  // no other thread's parts between this call's launches
         hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
         void *ws = nullptr;
         if (hipStreamIsCapturing(s, &capture) != hipSuccess) {
