@@ -92,26 +92,34 @@ int device_cus() {
     return n;
 }
 
+// hipStreamPerThread is one handle for a stream of every thread: what is kept for it
+// goes by the thread (whose streams end with it).
+using StreamKey = std::pair<int, hipStream_t>;
+static StreamKey stream_key(int dev, hipStream_t stream) {
+    static thread_local char thread;
+    return {dev, stream == hipStreamPerThread ? reinterpret_cast<hipStream_t>(&thread) : stream};
+}
+
 static std::mutex g_turn_mu;
-static std::map<std::pair<int, hipStream_t>, std::recursive_mutex> g_turns;
+static std::map<StreamKey, std::recursive_mutex> g_turns;
 
 StreamTurn::StreamTurn(hipStream_t stream) {
     int dev = 0;
     (void)hipGetDevice(&dev);
     std::unique_lock<std::mutex> lk(g_turn_mu);
-    std::recursive_mutex &turn = g_turns[{dev, stream}];
+    std::recursive_mutex &turn = g_turns[stream_key(dev, stream)];
     lk.unlock();
     lk_ = std::unique_lock<std::recursive_mutex>(turn);
 }
 
 static std::mutex g_scratch_mu;
-static std::map<std::pair<int, hipStream_t>, Scratch> g_scratch;
+static std::map<StreamKey, Scratch> g_scratch;
 
 mri_status scratch_get(hipStream_t stream, size_t bytes, void **ptr) {
     int dev = 0;
     MRI_HIP(hipGetDevice(&dev));
     std::lock_guard<std::mutex> lk(g_scratch_mu);
-    Scratch &sc = g_scratch[{dev, stream}];
+    Scratch &sc = g_scratch[stream_key(dev, stream)];
     if (sc.bytes < bytes) {
         size_t want = round_up(bytes < (1u << 20) ? (1u << 20) : bytes, 1u << 20);
         if (sc.ptr) {
@@ -133,14 +141,14 @@ mri_status scratch_get(hipStream_t stream, size_t bytes, void **ptr) {
 // The Q4_0 GEMM has its own: it uses it in no captured call, so it may grow
 // beside recorded graphs, whose INT8 and Q8_0 GEMMs replay with g_ws.
 static std::mutex g_ws_mu;
-static std::map<std::pair<int, hipStream_t>, Scratch> g_ws, g_q4ws, g_aws, g_sws;
+static std::map<StreamKey, Scratch> g_ws, g_q4ws, g_aws, g_sws;
 
-static mri_status zeroed_ws_get(std::map<std::pair<int, hipStream_t>, Scratch> &map,
+static mri_status zeroed_ws_get(std::map<StreamKey, Scratch> &map,
                                 hipStream_t stream, size_t bytes, void **ptr) {
     int dev = 0;
     MRI_HIP(hipGetDevice(&dev));
     std::lock_guard<std::mutex> lk(g_ws_mu);
-    Scratch &sc = map[{dev, stream}];
+    Scratch &sc = map[stream_key(dev, stream)];
     if (sc.bytes < bytes) {
         const size_t want = round_up(bytes, 1u << 20);
         if (sc.ptr) {
@@ -173,7 +181,7 @@ mri_status q4_ws_get(hipStream_t stream, size_t bytes, void **ptr) {
     int dev = 0;
     MRI_HIP(hipGetDevice(&dev));
     std::lock_guard<std::mutex> lk(g_ws_mu);
-    Scratch &sc = g_q4ws[{dev, stream}];
+    Scratch &sc = g_q4ws[stream_key(dev, stream)];
     *ptr = nullptr;
     if (sc.bytes < bytes) {
         const RelaxedCapture relaxed;
@@ -205,7 +213,7 @@ mri_status softmax_ws_get(hipStream_t stream, void **ptr) {
     int dev = 0;
     MRI_HIP(hipGetDevice(&dev));
     std::lock_guard<std::mutex> lk(g_ws_mu);
-    Scratch &sc = g_sws[{dev, stream}];
+    Scratch &sc = g_sws[stream_key(dev, stream)];
     if (!sc.ptr) {
         const RelaxedCapture relaxed;
         if (hipMalloc(&sc.ptr, kSoftmaxWsBytes) != hipSuccess) {

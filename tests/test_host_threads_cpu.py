@@ -67,6 +67,27 @@ def check_softmax(h):
                                               stream))
 
 
+def check_softmax_per_thread_stream(h):
+    """The per-thread stream has one handle and a stream a thread: each thread has
+    memory of its own, which its next call finds again."""
+    stream, done = 2, threading.Barrier(2)   # hipStreamPerThread
+    held = {}
+
+    def run(i):
+        for n in (40000, 50000):
+            h.m.check(h.llama.mri_softmax(X, 3, n, n, C.c_float(1.0), OUT, n, stream))
+        held[i] = True
+        done.wait()     # both threads live until both have called
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(held) == 2
+    assert [h.f.fake_alloc_bytes(i) for i in h.live()] == [1 << 18] * 2
+
+
 CHECKS = [n for n in dir() if n.startswith("check_")]
 
 
