@@ -707,6 +707,7 @@ mri_status mri_quantize_symmetric(const float *x, size_t len, int8_t *q, float *
     mri_status st = current_device(&dev);
     if (st) return st;
     auto s = static_cast<hipStream_t>(stream);
+    const StreamTurn turn(s);
     void *base = nullptr;
     st = scratch_get(s, 1024 * sizeof(float), &base);
     if (st) return st;
@@ -771,6 +772,7 @@ static mri_status matmul_int8_common(const char *fn, const int8_t *act_q, size_t
     mri_status st = current_device(&dev);
     if (st) return st;
     auto s = static_cast<hipStream_t>(stream);
+    const StreamTurn turn(s);
     if (m >= kGemmMinRows && gemm_rows_ok(m, d, act_q)) {
         // prefill on the caller's rows as they are
         void *ws = nullptr;
@@ -843,6 +845,7 @@ mri_status mri_matmul_int8_from_f32(const float *input, const size_t *dims, size
          gemv_int8_rows_fusable(m, k, d.kp, d.n_tiles, input)))
         return launch_gemv_int8(input, nullptr, m, nullptr, 0, 0.0f, d, out, act_q_out,
                                 act_scale_out, acc_out, s);
+    const StreamTurn turn(s);
     const bool gemm = m >= kGemmMinRows;
     Carver cv;
     const size_t o_act = cv.take(gemm ? gemm_pack_bytes(m, d.kp) : m * d.kp);
@@ -922,6 +925,7 @@ static mri_status matmul_blocks(const char *name, const float *input, const size
         gemv_q8_supported(true, m, d.n_tiles, k, d.kp))
         return launch_gemv_q8_0(input, nullptr, m, nullptr, d, out, block_dots_out,
                                 act_scales_out, s);
+    const StreamTurn turn(s);
     Carver cv;
     size_t mg = act_groups(m);
     // the fixed staging may hold the rows but not whole groups of 16
@@ -1063,6 +1067,7 @@ mri_status mri_matmul_q4_0_dequant_ordered(const float *input, const size_t *dim
     mri_status st = current_device(&dev);
     if (st) return st;
     auto s = static_cast<hipStream_t>(stream);
+    const StreamTurn turn(s);
     const float *x = input;
     if (!aligned(input, 16)) {
         void *base = nullptr;

@@ -196,8 +196,8 @@ int device_cus();
 
 // ---- per-(device, stream) scratch ----------------------------------------
 // A call that takes memory of its stream holds the stream's turn until its last
-// launch: another thread's call on the stream does not put its launches in between.
-// (Recursive: entry points call others.)
+// launch: another thread's call on the stream neither puts its launches in between nor
+// replaces the memory by a larger one.  (Recursive: entry points call others.)
 class StreamTurn {
   public:
     explicit StreamTurn(hipStream_t stream);

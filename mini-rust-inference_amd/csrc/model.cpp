@@ -748,6 +748,7 @@ mri_status mri_llama_forward_cached(mri_llama *m, const uint32_t *tokens, size_t
     TRY(check_tokens(m, tokens, n));
     if (!logits) return set_error(MRI_ERR_INVALID_ARGUMENT, "null logits");
     auto s = static_cast<hipStream_t>(stream);
+    const StreamTurn turn(s);
     if (n == 1 && row_path(m))
         return run_rows(m, nullptr, 1, start_pos, c, logits, s, Emb::kHost, tokens[0]);
     MRI_HIP(hipMemcpyAsync(m->tok, tokens, n * sizeof(uint32_t), hipMemcpyHostToDevice, s));
@@ -779,6 +780,7 @@ mri_status mri_llama_forward_kv4(mri_llama *m, const uint32_t *tokens, size_t n,
     if (!logits) return set_error(MRI_ERR_INVALID_ARGUMENT, "null logits");
     TRY(kv4_on_device(c));
     auto s = static_cast<hipStream_t>(stream);
+    const StreamTurn turn(s);
     const KvTarget kv(c, seq, cache_pos, weights);
     if (n == 1 && row_path(m))
         return run_rows(m, nullptr, 1, start_pos, kv, logits, s, Emb::kHost, tokens[0]);
@@ -800,6 +802,7 @@ mri_status mri_llama_generate_greedy(mri_llama *m, const uint32_t *prompt, size_
     TRY(check_tokens(m, prompt, n_prompt));
     if (!tokens_out) return set_error(MRI_ERR_INVALID_ARGUMENT, "null tokens_out");
     auto s = static_cast<hipStream_t>(stream);
+    const StreamTurn turn(s);
     const size_t V = m->cfg.vocab;
     // prefill logits of every prompt row (the per-tensor activation scale of
     // the INT8 output projection covers all of them, as LlamaModelInt8::forward)
@@ -872,7 +875,9 @@ mri_status mri_llama_generate_greedy(mri_llama *m, const uint32_t *prompt, size_
 mri_status mri_argmax(const float *v, size_t rows, size_t n, uint32_t *idx, void *stream) {
     if (rows && (!v || !idx)) return set_error(MRI_ERR_INVALID_ARGUMENT, "null pointer");
     if (rows && n == 0) return set_error(MRI_ERR_INVALID_SHAPE, "argmax: empty rows");
-    return launch_argmax(v, rows, n, idx, static_cast<hipStream_t>(stream));
+    auto s = static_cast<hipStream_t>(stream);
+    const StreamTurn turn(s);
+    return launch_argmax(v, rows, n, idx, s);
 }
 
 }  // extern "C"

@@ -10,7 +10,7 @@ import threading
 
 import pytest
 
-from test_host_calls_cpu import HERE, OUT, STREAM, X, Host
+from test_host_calls_cpu import HERE, OUT, STREAM, W, X, Host
 
 CALLS = 12
 
@@ -65,6 +65,28 @@ def check_softmax(h):
     for stream in (None, STREAM):
         h.ordered(lambda: h.llama.mri_softmax(X, 3, 40000, 40000, C.c_float(1.0), OUT, 40000,
                                               stream))
+
+
+def check_projections(h):
+    """Activations quantized into the stream's scratch, then the product."""
+    def dims(m, k):
+        return (C.c_size_t * 2)(m, k)
+
+    def int8(m, k, n):
+        w = C.c_void_p()
+        h.m.check(h.lib.mri_qmatrix_create_device(W, OUT, n, k, STREAM, C.byref(w)))
+        return w
+
+    h.ordered(h.q8_0(200, 4096, 6000))
+    w = int8(200, 4096, 6000)
+    h.ordered(lambda: h.lib.mri_matmul_int8_from_f32(X, dims(200, 4096), 2, w, OUT, None, None,
+                                                     None, STREAM))
+    odd = int8(3, 1000, 777)
+    h.ordered(lambda: h.lib.mri_matmul_int8(X + 1, 3 * 1000, C.c_float(1.0), odd, 3, OUT, None,
+                                            STREAM))
+    h.ordered(lambda: h.lib.mri_matmul_int8(X + 1, 200 * 4096, C.c_float(1.0), w, 200, OUT, None,
+                                            STREAM))
+    h.ordered(lambda: h.lib.mri_quantize_symmetric(X, 1 << 22, OUT, W, STREAM))
 
 
 def check_softmax_per_thread_stream(h):
