@@ -142,7 +142,8 @@ mri_status mri_argmax(const float *v, size_t rows, size_t n, uint32_t *idx, void
  * with another current device are InvalidArgument.  It owns the workspace of
  * its attention calls (fixed at creation, so captured graphs hold it as long
  * as the handle lives): calls on one handle must be ordered, as on
- * mri_kv_cache; handles are independent.  No call allocates memory.
+ * mri_kv_cache; handles are independent.  No call allocates memory; calls of
+ * more than 2^22 workgroups run in several launches.
  * InvalidShape for a zero size; Unsupported for a head dim other than 64 or
  * 128, or max_seq above 2^30. */
 typedef struct mri_kv4_cache mri_kv4_cache;
@@ -183,7 +184,8 @@ mri_status mri_kv4_read(const mri_kv4_cache *cache, size_t layer, size_t n_layer
  * position p = pos + i sees keys 0 .. p (append first).  q and out are
  * [n_seqs * rows] rows of n_heads * head_dim f32, q_stride / out_stride
  * floats apart; head h reads KV head h / (n_heads / n_kv_heads).
- * InvalidShape when n_heads % n_kv_heads != 0.
+ * InvalidShape when n_heads % n_kv_heads != 0; Unsupported for more than 2^20
+ * heads, or rows * (n_heads / n_kv_heads) above 2^30.
  * weights (nullable): [cache n_seqs][n_kv_heads][max_seq] f32 of this layer,
  * the attention weight that each cached key has got: key t of a KV head gets
  * the sum of its probabilities over the call's rows and the head's query
@@ -231,8 +233,9 @@ mri_status mri_llama_forward_kv4(mri_llama *model, const uint32_t *tokens, size_
  * per (device, stream), in two launches that no other thread's call on the
  * stream comes between; a call that is being captured uses none, takes longer
  * and gives the same bits.
- * InvalidArgument unless temperature > 0 and finite; InvalidShape for n = 0 or a
- * stride below n. */
+ * InvalidArgument unless temperature > 0 and finite, or for x = out with
+ * different strides; InvalidShape for n = 0 or a stride below n; Unsupported
+ * for more than 2^21 rows. */
 mri_status mri_softmax(const float *x, size_t rows, size_t n, size_t x_stride, float temperature,
                        float *out, size_t out_stride, void *stream);
 
@@ -250,7 +253,8 @@ mri_status mri_softmax(const float *x, size_t rows, size_t n, size_t x_stride, f
  * rejected; where no token has a positive probability the drawn token is
  * MRI_NO_TOKEN.  A NaN target probability counts as 0; a token whose draft
  * probability is NaN is neither accepted nor drawn in its place.  InvalidShape
- * for n = 0. */
+ * for n = 0; Unsupported for n = 2^32 - 1 and more, k above 2^20 or n_seqs
+ * above 2^21. */
 #define MRI_NO_TOKEN 0xffffffffu
 mri_status mri_verify_drafts(const uint32_t *drafts, const float *draft_probs,
                              const float *target_probs, const float *uniforms,

@@ -1362,7 +1362,7 @@ __global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
     __shared__ unsigned s_wave[kSelWaves], s_digit, s_left;
     __shared__ unsigned s_gt[kSelWaves], s_eq[kSelWaves];
     const int t = threadIdx.x, lane = t & 63, wv = wave_id();
-    const size_t rowi = blockIdx.x;
+    const size_t rowi = e.row0 + blockIdx.x;
     const int b = (int)(rowi / e.n_kv % e.n_seqs);
     const unsigned n = min(e.lens[b], e.src_max);
     uint32_t *kept = e.kept + rowi * e.keep;
@@ -1477,7 +1477,7 @@ __global__ __launch_bounds__(256) void k_kv4_move(Kv4Evict e, int per_row) {
     __shared__ unsigned s_i[kPageKeys], s_pg[kPageKeys], s_d[kPageKeys];
     __shared__ uint4_t s_v[kMovePages * VB / 16];
     const int t = threadIdx.x, lane = t & 63, wv = wave_id(), g = lane >> 4, r = lane & 15;
-    const size_t rowi = blockIdx.x / per_row;
+    const size_t rowi = e.row0 + blockIdx.x / per_row;
     const int b = (int)(rowi / e.n_kv % e.n_seqs);
     if (rowi < (size_t)e.n_seqs * e.n_kv && rowi % e.n_kv == 0 && blockIdx.x % per_row == 0 &&
         t == 0)
@@ -1593,12 +1593,9 @@ __global__ __launch_bounds__(256) void k_kv4_move(Kv4Evict e, int per_row) {
 
 inline bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-// Workgroups of one launch (512 threads each at most; a launch takes 2^32).
+// Workgroups of one launch (512 threads each at most; a launch takes fewer than 2^32).
+// Calls of more run in parts.
 constexpr size_t kMostWgs = 1u << 22;
-mri_status grid_ok(size_t blocks) {
-    return blocks <= kMostWgs ? MRI_OK
-                              : set_error(MRI_ERR_UNSUPPORTED, "kv4: more than 2^22 workgroups");
-}
 
 template <class F>
 void by_head(size_t hd, F &&f) {
@@ -1606,10 +1603,43 @@ void by_head(size_t hd, F &&f) {
     else f(std::integral_constant<int, 128>{});
 }
 
-// Pages that `rows` consecutive positions can touch.
+// Pages that the call's rows can touch.
 inline size_t pages_touched(const Kv4Rows &a) {
-    if (!a.pos) return (a.start + a.rows - 1) / kPageKeys - a.start / kPageKeys + 1;
+    const size_t p = (size_t)a.start + a.row0;
+    if (!a.pos) return (p + a.rows - 1) / kPageKeys - p / kPageKeys + 1;
     return ((size_t)a.rows + kPageKeys - 2) / kPageKeys + 1;
+}
+// Sequences b .. b + n - 1 of the call's.
+inline Kv4Rows some_seqs(const Kv4Rows &a, size_t b, size_t n) {
+    Kv4Rows c = a;
+    c.first_seq += (int)b;
+    c.n_seqs = (int)std::min<size_t>(n, a.n_seqs - b);
+    if (c.pos) c.pos += b;
+    if (c.count) c.count += b;
+    return c;
+}
+// Append and read, a workgroup a page, in launches of at most kMostWgs: f(rows, pages
+// of a sequence, first layer, layers, first sequence) for parts of the rows (where one
+// sequence's pages are too many), the sequences, then the layers.
+template <class F>
+mri_status by_pages(const Kv4Rows &a, size_t n_layers, F &&f) {
+    const size_t most = kMostWgs / a.n_kv;  // (n_kv <= 2^20: four pages or more)
+    const size_t rows = pages_touched(a) <= most ? a.rows : (most - 2) * kPageKeys;
+    for (size_t i = 0; i < a.rows; i += rows) {
+        Kv4Rows r = a;
+        r.row0 = (unsigned)i;
+        r.rows = (unsigned)std::min<size_t>(rows, a.rows - i);
+        const size_t n_pg = pages_touched(r);
+        const size_t seqs = std::min<size_t>(a.n_seqs, kMostWgs / (n_pg * a.n_kv));
+        const size_t layers =
+            seqs < (size_t)a.n_seqs ? 1 : kMostWgs / (n_pg * a.n_kv * a.n_seqs);
+        for (size_t b = 0; b < (size_t)a.n_seqs; b += seqs)
+            for (size_t l = 0; l < n_layers; l += layers)
+                if (const mri_status st = f(some_seqs(r, b, seqs), n_pg, l,
+                                            std::min(layers, n_layers - l), b))
+                    return st;
+    }
+    return MRI_OK;
 }
 
 }  // namespace
@@ -1617,39 +1647,45 @@ inline size_t pages_touched(const Kv4Rows &a) {
 mri_status launch_kv4_append(const Kv4Rows &a, size_t hd, const float *k, const float *v,
                              size_t stride, hipStream_t s) {
     if (!a.rows || !a.n_seqs) return MRI_OK;
-    const size_t n_pg = pages_touched(a), blocks = n_pg * a.n_kv * a.n_seqs;
-    if (const mri_status st = grid_ok(blocks)) return st;
     const bool v4 = stride % 4 == 0 && al16(k) && al16(v);
-    by_head(hd, [&](auto h) {
-        constexpr int HD = decltype(h)::value;
-        if (v4)
-            hipLaunchKernelGGL((k_kv4_append<HD, true>), dim3((unsigned)blocks), dim3(256), 0, s,
-                               a, k, v, stride, (int)n_pg);
-        else
-            hipLaunchKernelGGL((k_kv4_append<HD, false>), dim3((unsigned)blocks), dim3(256), 0, s,
-                               a, k, v, stride, (int)n_pg);
+    return by_pages(a, 1, [&](const Kv4Rows &c, size_t n_pg, size_t, size_t, size_t b) {
+        const dim3 grid((unsigned)(n_pg * c.n_kv * c.n_seqs));
+        const size_t at = b * a.ld_rows * stride;
+        by_head(hd, [&](auto h) {
+            constexpr int HD = decltype(h)::value;
+            if (v4)
+                hipLaunchKernelGGL((k_kv4_append<HD, true>), grid, dim3(256), 0, s, c, k + at,
+                                   v + at, stride, (int)n_pg);
+            else
+                hipLaunchKernelGGL((k_kv4_append<HD, false>), grid, dim3(256), 0, s, c, k + at,
+                                   v + at, stride, (int)n_pg);
+        });
+        MRI_LAUNCHED("k_kv4_append");
+        return MRI_OK;
     });
-    MRI_LAUNCHED("k_kv4_append");
-    return MRI_OK;
 }
 
 mri_status launch_kv4_read(const Kv4Rows &a, size_t hd, size_t n_layers, size_t layer_bytes,
                            float *k, float *v, size_t stride, hipStream_t s) {
     if (!a.rows || !a.n_seqs || !n_layers) return MRI_OK;
-    const size_t n_pg = pages_touched(a), blocks = n_pg * a.n_kv * a.n_seqs * n_layers;
-    if (const mri_status st = grid_ok(blocks)) return st;
     const bool v4 = stride % 4 == 0 && al16(k) && al16(v);
-    by_head(hd, [&](auto h) {
-        constexpr int HD = decltype(h)::value;
-        if (v4)
-            hipLaunchKernelGGL((k_kv4_read<HD, true>), dim3((unsigned)blocks), dim3(256), 0, s, a,
-                               layer_bytes, k, v, stride, (int)n_pg);
-        else
-            hipLaunchKernelGGL((k_kv4_read<HD, false>), dim3((unsigned)blocks), dim3(256), 0, s,
-                               a, layer_bytes, k, v, stride, (int)n_pg);
+    return by_pages(a, n_layers, [&](Kv4Rows c, size_t n_pg, size_t layer, size_t layers,
+                                     size_t b) {
+        const dim3 grid((unsigned)(n_pg * c.n_kv * c.n_seqs * layers));
+        c.pages += layer * layer_bytes;
+        const size_t at = (layer * a.n_seqs + b) * a.ld_rows * stride;
+        by_head(hd, [&](auto h) {
+            constexpr int HD = decltype(h)::value;
+            if (v4)
+                hipLaunchKernelGGL((k_kv4_read<HD, true>), grid, dim3(256), 0, s, c, layer_bytes,
+                                   k + at, v + at, stride, (int)n_pg);
+            else
+                hipLaunchKernelGGL((k_kv4_read<HD, false>), grid, dim3(256), 0, s, c, layer_bytes,
+                                   k + at, v + at, stride, (int)n_pg);
+        });
+        MRI_LAUNCHED("k_kv4_read");
+        return MRI_OK;
     });
-    MRI_LAUNCHED("k_kv4_read");
-    return MRI_OK;
 }
 
 namespace {
@@ -1681,9 +1717,7 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
                                dim3(waves_of(HD, true) * kWave), 0, s, a, q, qs, vec, groups,
                                (int)n_qt, (unsigned)slots, out, os, part, cnts, z);
         } else {
-            const size_t blocks = tiles * a.n_seqs;
-            if (const mri_status st = grid_ok(blocks)) return st;
-            hipLaunchKernelGGL((k_kv4_attend<HD, FEW, false>), dim3((unsigned)blocks),
+            hipLaunchKernelGGL((k_kv4_attend<HD, FEW, false>), dim3((unsigned)(tiles * a.n_seqs)),
                                dim3(waves_of(HD, false) * kWave), 0, s, a, q, qs, vec, groups,
                                (int)n_qt, 0u, out, os, part, cnts, z);
         }
@@ -1697,7 +1731,6 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
     const size_t n_qg = (n_q + kPromptWaves * 16 - 1) / (kPromptWaves * 16);
     const size_t prompt_wgs = n_qg * a.n_kv * a.n_seqs;
     if (n_q > 32 && prompt_wgs >= cus) {
-        if (const mri_status st = grid_ok(prompt_wgs)) return st;
         hipLaunchKernelGGL((k_kv4_prompt<HD>), dim3((unsigned)prompt_wgs),
                            dim3(kPromptWaves * kWave), 0, s, a, q, qs, vec, groups, (int)n_qg, out,
                            os, z);
@@ -1721,16 +1754,12 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
             groups_all * parts * kWtWaves * kPageKeys > kv4_part_floats(HD))
             parts = 1;
         // (positions on the device: the pages are those of the longest possible
-        // sequence, so many sequences of a long cache take more than one launch)
+        // sequence, so many sequences of a long cache take more than one launch; one
+        // sequence's groups of 256 threads fit one: 288 GB hold fewer than 2^24 groups)
         const size_t seqs = std::min<size_t>(
             a.n_seqs, std::max<size_t>(1, kMostWgs / (n_grp * a.n_kv * parts)));
-        if (const mri_status e = grid_ok(n_grp * a.n_kv * parts)) return e;
         for (size_t b = 0; b < (size_t)a.n_seqs; b += seqs) {
-            Kv4Rows c = a;
-            c.first_seq += (int)b;
-            c.n_seqs = (int)std::min<size_t>(seqs, a.n_seqs - b);
-            if (c.pos) c.pos += b;
-            if (c.count) c.count += b;
+            const Kv4Rows c = some_seqs(a, b, seqs);
             hipLaunchKernelGGL((k_kv4_weights<HD>),
                                dim3((unsigned)(n_grp * c.n_kv * c.n_seqs * parts)),
                                dim3(kWtWaves * kWave), 0, s, c, q + b * a.ld_rows * qs, qs, vec,
@@ -1756,20 +1785,17 @@ mri_status launch_kv4_attend(const Kv4Rows &a, size_t hd, const float *q, size_t
                                  s);
         });
     };
-    if (!weights || (size_t)a.n_seqs * a.rows * n_heads <= kKv4LseFloats) {
-        go(a, q, out);
-        return st;
-    }
-    // weights: as many sequences, or rows of one, as their log-sum-exps fit
-    const size_t seqs = std::max<size_t>(1, kKv4LseFloats / (a.rows * n_heads));
-    const size_t rows = std::min<size_t>(a.rows, std::max<size_t>(1, kKv4LseFloats / n_heads));
+    // as many rows of a sequence, and sequences, as a launch takes in tiles of 16
+    // queries; with weights, as their log-sum-exps fit
+    const size_t groups = n_heads / a.n_kv;
+    size_t rows = std::max<size_t>(1, (kMostWgs / a.n_kv - 1) * 16 / groups);
+    if (weights) rows = std::min(rows, std::max<size_t>(1, kKv4LseFloats / n_heads));
+    rows = std::min<size_t>(rows, a.rows);
+    size_t seqs = std::max<size_t>(1, kMostWgs / (a.n_kv * ((rows * groups + 15) / 16)));
+    if (weights) seqs = std::min(seqs, std::max<size_t>(1, kKv4LseFloats / (a.rows * n_heads)));
     for (size_t b = 0; b < (size_t)a.n_seqs && !st; b += seqs)
         for (size_t i = 0; i < a.rows && !st; i += rows) {
-            Kv4Rows c = a;
-            c.first_seq += (int)b;
-            c.n_seqs = (int)std::min<size_t>(seqs, a.n_seqs - b);
-            if (c.pos) c.pos += b;
-            if (c.count) c.count += b;
+            Kv4Rows c = some_seqs(a, b, seqs);
             c.row0 = (unsigned)i;
             c.rows = (unsigned)std::min<size_t>(rows, a.rows - i);
             go(c, q + b * a.ld_rows * q_stride, out + b * a.ld_rows * out_stride);
@@ -1777,23 +1803,30 @@ mri_status launch_kv4_attend(const Kv4Rows &a, size_t hd, const float *q, size_t
     return st;
 }
 
-mri_status launch_kv4_evict(const Kv4Evict &e, size_t hd, hipStream_t s) {
-    const size_t rows = (size_t)e.n_layers * e.n_seqs * e.n_kv;
-    if (const mri_status st = grid_ok(rows * 2)) return st;  // (1024 threads each)
-    if (e.src_max <= kSelRegs * kSelThreads)
-        hipLaunchKernelGGL(k_kv4_select<true>, dim3((unsigned)rows), dim3(kSelThreads), 0, s, e);
-    else
-        hipLaunchKernelGGL(k_kv4_select<false>, dim3((unsigned)rows), dim3(kSelThreads), 0, s, e);
-    MRI_LAUNCHED("k_kv4_select");
+mri_status launch_kv4_evict(const Kv4Evict &call, size_t hd, hipStream_t s) {
+    Kv4Evict e = call;
+    const size_t all = (size_t)e.n_layers * e.n_seqs * e.n_kv;
+    // every head's keys are chosen before any lengths are stored, maybe over the old
+    constexpr size_t kMostSel = kMostWgs / 2;  // (1024 threads each)
+    for (e.row0 = 0; e.row0 < all; e.row0 += kMostSel) {
+        const dim3 grid((unsigned)std::min(kMostSel, all - e.row0));
+        if (e.src_max <= kSelRegs * kSelThreads)
+            hipLaunchKernelGGL(k_kv4_select<true>, grid, dim3(kSelThreads), 0, s, e);
+        else
+            hipLaunchKernelGGL(k_kv4_select<false>, grid, dim3(kSelThreads), 0, s, e);
+        MRI_LAUNCHED("k_kv4_select");
+    }
     const size_t n_pg = ((size_t)e.keep + kPageKeys - 1) / kPageKeys;
-    const size_t per_row =
-        e.src == e.dst ? 1 : std::max<size_t>(1, std::min(n_pg, kMostWgs / rows));
-    by_head(hd, [&](auto h) {
-        constexpr int HD = decltype(h)::value;
-        hipLaunchKernelGGL((k_kv4_move<HD>), dim3((unsigned)(rows * per_row)), dim3(256), 0, s, e,
-                           (int)per_row);
-    });
-    MRI_LAUNCHED("k_kv4_move");
+    for (e.row0 = 0; e.row0 < all; e.row0 += kMostWgs) {
+        const size_t rows = std::min(kMostWgs, all - e.row0);
+        const size_t per_row = e.src == e.dst ? 1 : std::min(n_pg, kMostWgs / rows);
+        by_head(hd, [&](auto h) {
+            constexpr int HD = decltype(h)::value;
+            hipLaunchKernelGGL((k_kv4_move<HD>), dim3((unsigned)(rows * per_row)), dim3(256), 0, s,
+                               e, (int)per_row);
+        });
+        MRI_LAUNCHED("k_kv4_move");
+    }
     return MRI_OK;
 }
 

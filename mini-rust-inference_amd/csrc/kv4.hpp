@@ -63,6 +63,7 @@ mri_status launch_kv4_attend(const Kv4Rows &a, size_t hd, const float *q, size_t
 struct Kv4Evict {
     const uint8_t *src = nullptr;
     uint8_t *dst = nullptr;
+    size_t row0 = 0;  // the first (layer, sequence, KV head) of a launch
     int n_layers = 0, n_seqs = 0, n_kv = 0;
     int src_pages = 0, dst_pages = 0;
     unsigned src_max = 0, dst_max = 0;
