@@ -129,7 +129,8 @@ mri_status mri_argmax(const float *v, size_t rows, size_t n, uint32_t *idx, void
 /* a decode loop over it.  Extensions with no counterpart in the           */
 /* reference, whose cache is f32 and holds one sequence                    */
 /* (src/cache/kv_cache.rs), whose decoding is greedy                       */
-/* (src/sampling/mod.rs:144-151) and which evicts nothing.                 */
+/* (src/sampling/mod.rs:144-151) and which evicts nothing.  Device arrays  */
+/* that are not aligned to 4 bytes are InvalidArgument.                    */
 /* ===================================================================== */
 
 /* Keys and values of n_layers layers and n_seqs sequences of up to max_seq

@@ -23,7 +23,10 @@ mri_status bad_shape(const std::string &m) { return set_error(MRI_ERR_INVALID_SH
         if (_st != MRI_OK) return _st;         \
     } while (0)
 
-bool float_aligned(const void *p) { return ((uintptr_t)p & 3) == 0; }
+template <class... P>
+bool float_aligned(const P *...p) {
+    return ((... | (uintptr_t)p) & 3) == 0;
+}
 
 }  // namespace
 
@@ -49,7 +52,7 @@ mri_status kv4_rows(const mri_kv4_cache *c, size_t layer, const mri_kv4_rows *r,
         return bad_shape("kv4: positions " + std::to_string(r->start) + " + " +
                          std::to_string(r->rows) + " exceed the cache length " +
                          std::to_string(c->max_seq));
-    if (!float_aligned(r->pos) || !float_aligned(r->count))
+    if (!float_aligned(r->pos, r->count))
         return bad_arg("kv4: positions and counts must be 4-byte aligned");
     a->pages = c->pages + layer * c->layer_bytes();
     a->n_kv = (int)c->n_kv;
@@ -136,7 +139,7 @@ mri_status mri_kv4_append(mri_kv4_cache *c, size_t layer, const mri_kv4_rows *ro
     if (stride < c->n_kv * c->hd) return bad_shape("kv4_append: rows overlap");
     if (!a.rows || !a.n_seqs) return MRI_OK;
     if (!k || !v) return bad_arg("kv4_append: null pointer");
-    if (!float_aligned(k) || !float_aligned(v)) return bad_arg("kv4_append: unaligned rows");
+    if (!float_aligned(k, v)) return bad_arg("kv4_append: unaligned rows");
     TRY(kv4_on_device(c));
     return launch_kv4_append(a, c->hd, k, v, stride, static_cast<hipStream_t>(stream));
 }
@@ -152,7 +155,7 @@ mri_status mri_kv4_read(const mri_kv4_cache *c, size_t layer, size_t n_layers,
     if (stride < c->n_kv * c->hd) return bad_shape("kv4_read: rows overlap");
     if (!a.rows || !a.n_seqs || !n_layers) return MRI_OK;
     if (!k || !v) return bad_arg("kv4_read: null pointer");
-    if (!float_aligned(k) || !float_aligned(v)) return bad_arg("kv4_read: unaligned rows");
+    if (!float_aligned(k, v)) return bad_arg("kv4_read: unaligned rows");
     TRY(kv4_on_device(c));
     return launch_kv4_read(a, c->hd, n_layers, c->layer_bytes(), k, v, stride,
                            static_cast<hipStream_t>(stream));
@@ -172,7 +175,7 @@ mri_status mri_kv4_attend(mri_kv4_cache *c, size_t layer, const mri_kv4_rows *ro
         return bad_shape("kv4_attend: rows overlap");
     if (!a.rows || !a.n_seqs) return MRI_OK;
     if (!q || !out) return bad_arg("kv4_attend: null pointer");
-    if (!float_aligned(q) || !float_aligned(out) || !float_aligned(weights))
+    if (!float_aligned(q, out, weights))
         return bad_arg("kv4_attend: unaligned rows");
     TRY(kv4_on_device(c));
     return launch_kv4_attend(a, c->hd, q, q_stride, n_heads, out, out_stride, weights, c->part,
@@ -193,6 +196,8 @@ mri_status mri_kv4_evict(const mri_kv4_cache *src, mri_kv4_cache *dst, const flo
     if (recent > keep) return bad_arg("kv4_evict: recent > keep");
     if ((src == dst) != (weights == weights_out))
         return bad_arg("kv4_evict: weights_out is weights in place, and only there");
+    if (!float_aligned(weights, weights_out, lens, lens_out, kept))
+        return bad_arg("kv4_evict: unaligned arrays");
     TRY(kv4_on_device(src));
     TRY(kv4_on_device(dst));
     Kv4Evict e;
@@ -223,7 +228,7 @@ mri_status mri_softmax(const float *x, size_t rows, size_t n, size_t x_stride, f
         return bad_shape("softmax: empty or overlapping rows");
     if (!rows) return MRI_OK;
     if (!x || !out) return bad_arg("softmax: null pointer");
-    if (!float_aligned(x) || !float_aligned(out)) return bad_arg("softmax: unaligned rows");
+    if (!float_aligned(x, out)) return bad_arg("softmax: unaligned rows");
     if (x == out && x_stride != out_stride)
         return bad_arg("softmax: in place the strides must be equal");
     if (rows > (1u << 21))
@@ -244,6 +249,8 @@ mri_status mri_verify_drafts(const uint32_t *drafts, const float *draft_probs,
         return set_error(MRI_ERR_UNSUPPORTED, "verify_drafts: too many tokens or sequences");
     if (!target_probs || !uniforms || !tokens || !accepted || (k && !drafts))
         return bad_arg("verify_drafts: null pointer");
+    if (!float_aligned(drafts, draft_probs, target_probs, uniforms, n_drafts, tokens, accepted))
+        return bad_arg("verify_drafts: unaligned arrays");
     int dev;
     TRY(current_device(&dev));
     return launch_verify(drafts, draft_probs, target_probs, uniforms, n_drafts, n_seqs, k, n,

@@ -778,6 +778,8 @@ mri_status mri_llama_forward_kv4(mri_llama *m, const uint32_t *tokens, size_t n,
                                  cache_pos, n, c->max_seq));
     TRY(check_tokens(m, tokens, n));
     if (!logits) return set_error(MRI_ERR_INVALID_ARGUMENT, "null logits");
+    if (((uintptr_t)logits | (uintptr_t)weights) & 3)
+        return set_error(MRI_ERR_INVALID_ARGUMENT, "forward: unaligned logits or weights");
     TRY(kv4_on_device(c));
     auto s = static_cast<hipStream_t>(stream);
     const StreamTurn turn(s);
