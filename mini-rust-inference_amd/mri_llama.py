@@ -293,17 +293,21 @@ class Llama:
     def forward_kv4(self, tokens, start_pos, cache, logits, seq=0, cache_pos=None, weights=None,
                     stream=None):
         """cache_pos: start_pos unless keys were evicted.  weights: f32
-        [n_layers, n_seqs, n_kv_heads, max_seq] of the cache."""
+        [n_layers, n_seqs, n_kv_heads, max_seq] of the cache.  logits: f32, contiguous,
+        [len(tokens), vocab] or more rows."""
         import numpy as np
         t = np.ascontiguousarray(tokens, np.uint32)
         dev = _device()
+        lp = _tensor(logits, "logits", _F32, dev, logits.shape)
+        if logits.numel() < t.size * self.cfg["vocab"]:
+            raise _bad("InvalidShape", f"logits: shape {tuple(logits.shape)}, expected "
+                                       f"{(t.size, self.cfg['vocab'])}")
         wp = None if weights is None else _tensor(
             weights, "weights", _F32, dev,
             (cache.n_layers, cache.n_seqs, cache.n_kv_heads, cache.max_seq))
         Q.check(lib().mri_llama_forward_kv4(
             self.h, t.ctypes.data_as(P), t.size, start_pos, cache.h, seq,
-            start_pos if cache_pos is None else cache_pos, wp, C.c_void_p(logits.data_ptr()),
-            Q._stream(stream)))
+            start_pos if cache_pos is None else cache_pos, wp, lp, Q._stream(stream)))
 
     def forward_decode(self, token, pos, cache, logits, stream=None):
         Q.check(lib().mri_llama_forward_decode(self.h, int(token), pos, cache.h,

@@ -168,6 +168,24 @@ def test_forward_kv4_refusals():
         8, 2, kept)
 
 
+def test_forward_kv4_refuses_logits():
+    """Logits that the call would write past, or of another type, place or layout."""
+    import mri_qmatmul as Q
+    import torch as t
+    _, gpu, rng = build("q4_0", max_seq=48)
+    cache = gpu.kv4_cache(max_seq=40)
+    toks = [1, 2, 3]
+    for kind, logits in (("InvalidShape", empty((2, 300), t.float32)),
+                         ("InvalidShape", empty((3, 299), t.float32)),
+                         ("InvalidArgument", empty((3, 300), t.float16)),
+                         ("InvalidArgument", t.zeros(3, 300)),
+                         ("InvalidArgument", empty((3, 600), t.float32)[:, ::2])):
+        with pytest.raises(Q.MriError) as e:
+            gpu.forward_kv4(toks, 0, cache, logits)
+        assert e.value.kind == kind, e.value
+    gpu.forward_kv4(toks, 0, cache, empty((4, 300), t.float32))
+
+
 def test_speculative_decode_with_eviction():
     """The loop that the operators are for: a prompt with its keys' weights, steps
     of a token and three drafts, their softmax and verification, positions that
