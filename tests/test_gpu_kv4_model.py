@@ -168,6 +168,64 @@ def test_forward_kv4_refusals():
         8, 2, kept)
 
 
+class CacheOracle(Kv4Oracle):
+    """Kv4Oracle whose blocks attend to given keys and values: what a call does with
+    its cache, apart from how rounding moves what it writes there."""
+
+    def block(self, li, x, start_pos):
+        own = R.stored
+        try:
+            at = start_pos - self.shift
+            rows = iter((self.given_k[li, at:at + len(x)], self.given_v[li, at:at + len(x)]))
+            R.stored = lambda _: next(rows)
+            return super().block(li, x, start_pos)
+        finally:
+            R.stored = own
+
+
+@pytest.mark.parametrize("fmt,hd", [("q4_0", 64), ("q4_0", 128), ("q8_0", 64), ("int8", 128),
+                                    ("w4a8", 64), ("mixed", 64)])
+def test_forward_kv4_cache_and_logits(fmt, hd):
+    """What the call caches in the first layer, and its logits from what it cached.
+
+    The first layer's keys and values come from the embedding rows: their activations
+    differ from the oracle's by f32 rounding, which moves about one in 10^4 over a step of
+    its int8 rounding.  Such a step is 1 / 127 of the row's largest activation, of 4 * hd
+    that a key sums: under a hundredth of a key's usual size, where a 4-bit step is a third
+    of it.  So nearly all quants equal the oracle's, and the others are a step off; a
+    scale is at most an f16 rounding off, 2^-10 of the value.
+    From the cache on, both compute the same attention and the same projections of it:
+    the logits are as close as with an f32 cache, for every format (test_gpu_llama.py)."""
+    import torch as t
+    oracle, gpu, rng = build(fmt, seed=17, d=4 * hd, nh=4, nkv=2, max_seq=100)
+    toks = rng.integers(0, 300, 83).tolist()
+    cache = gpu.kv4_cache(n_seqs=2, max_seq=96)
+    w = t.zeros(2, 2, 2, 96, device="cuda")
+    got, at = [], 0
+    for n in (64, 1, 5, 1, 12):
+        logits = empty((n, 300), t.float32)
+        gpu.forward_kv4(toks[at:at + n], at, cache, logits, seq=1, weights=w)
+        got.append(host(logits))
+        at += n
+    k, v = (t.zeros(2, 2, 96, 2 * hd, device="cuda") for _ in range(2))
+    cache.read(0, k, v, 0)
+    ref = CacheOracle(oracle)
+    ref.given_k, ref.given_v = host(k)[:, 1], host(v)[:, 1]
+    free, done = Kv4Oracle(oracle), 0
+    for part in got:
+        n = len(part)
+        close(part, ref.forward_cached(toks[done:done + n], done), TOL)
+        free.forward_cached(toks[done:done + n], done)
+        done += n
+    close(host(w)[:, 1], ref.weights[:, :, :96], TOL)
+    for mine, want in ((ref.given_k, free.k_cache), (ref.given_v, free.v_cache)):
+        mine, want = mine[0, :at].reshape(-1, 32), want[0, :at].reshape(-1, 32)
+        top = np.abs(want).max(1, keepdims=True)
+        off = np.abs(mine - want)
+        assert (off <= top * (1 / 8 + 2.0 ** -9)).all()
+        assert (off > top * 2.0 ** -9).mean() <= 0.01
+
+
 def test_forward_kv4_refuses_logits():
     """Logits that the call would write past, or of another type, place or layout."""
     import mri_qmatmul as Q
