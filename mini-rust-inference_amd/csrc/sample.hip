@@ -27,22 +27,27 @@ typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 // workgroup a part, then a second launch that joins a row's parts and writes; the
 // values come from the device's cache then.  Else a workgroup of 1024 a row does
 // the same steps, four parts at a time, to the same bits.
-__device__ inline float exp_scaled(float d, float c) {
-    return __builtin_amdgcn_exp2f(d * c);  // c = log2(e) / T
-}
+struct Temp {
+    // exp((x - m) / T) = 2^((h x - h m) c): h is 1 / 2 where the temperature may bring
+    // logits together whose difference passes the largest float (T >= 1), else 1
+    float h, c;
+    __device__ float exp_diff(float x, float m) const {
+        return __builtin_amdgcn_exp2f(fmaf(x, h, -h * m) * c);
+    }
+};
 struct MaxSum {
     float m, l;  // l = sum of exp of what is not -inf; NaN stays in it
 };
-__device__ inline MaxSum join(MaxSum a, MaxSum b, float c) {
+__device__ inline MaxSum join(MaxSum a, MaxSum b, Temp c) {
     const float m = fmaxf(a.m, b.m);
-    return MaxSum{m, (a.m == m ? a.l : a.l * exp_scaled(a.m - m, c)) +
-                         (b.m == m ? b.l : b.l * exp_scaled(b.m - m, c))};
+    return MaxSum{m, (a.m == m ? a.l : a.l * c.exp_diff(a.m, m)) +
+                         (b.m == m ? b.l : b.l * c.exp_diff(b.m, m))};
 }
 
 // HELD: V times four values a thread.
 template <int V>
 __global__ __launch_bounds__(1024) void k_softmax_held(const float *x, size_t n, size_t xs,
-                                                       float c, float *out, size_t os) {
+                                                       Temp c, float *out, size_t os) {
     __shared__ float s_m[16], s_l[16];
     const float *row = x + (size_t)blockIdx.x * xs;
     const int t = threadIdx.x, lane = t % kWave, wave = t / kWave;
@@ -72,7 +77,7 @@ __global__ __launch_bounds__(1024) void k_softmax_held(const float *x, size_t n,
     float l = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4 * V; ++j) {
-        v[j] = v[j] == -INFINITY ? 0.0f : exp_scaled(v[j] - m, c);
+        v[j] = v[j] == -INFINITY ? 0.0f : c.exp_diff(v[j], m);
         l = l + v[j];
     }
 #pragma unroll
@@ -103,7 +108,7 @@ __global__ __launch_bounds__(1024) void k_softmax_held(const float *x, size_t n,
 
 constexpr int kPartThreads = 256;
 // (max, sum) of x[lo, hi) over 256 threads, t of them this one; s_ms: four entries.
-__device__ inline MaxSum part_stats(const float *x, size_t lo, size_t hi, int t, float c,
+__device__ inline MaxSum part_stats(const float *x, size_t lo, size_t hi, int t, Temp c,
                                     MaxSum *s_ms) {
     MaxSum a{-INFINITY, 0.0f};
     for (size_t i0 = lo; i0 < hi; i0 += 16 * kPartThreads) {
@@ -123,10 +128,10 @@ __device__ inline MaxSum part_stats(const float *x, size_t lo, size_t hi, int t,
         float m = a.m;
 #pragma unroll
         for (int j = 0; j < 16; ++j) m = fmaxf(m, v[j]);
-        float l = a.m == m ? a.l : a.l * exp_scaled(a.m - m, c);
+        float l = a.m == m ? a.l : a.l * c.exp_diff(a.m, m);
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-            l = l + (v[j] == -INFINITY ? 0.0f : exp_scaled(v[j] - m, c));
+            l = l + (v[j] == -INFINITY ? 0.0f : c.exp_diff(v[j], m));
         a = MaxSum{m, l};
     }
 #pragma unroll
@@ -140,7 +145,7 @@ __device__ inline MaxSum part_stats(const float *x, size_t lo, size_t hi, int t,
 }
 
 // A row's probabilities x[lo, hi) from its (max, sum), over n_t threads.
-__device__ inline void write_probs(const float *x, size_t lo, size_t hi, int t, int n_t, float c,
+__device__ inline void write_probs(const float *x, size_t lo, size_t hi, int t, int n_t, Temp c,
                                    MaxSum a, float *out) {
     const bool none = a.m == -INFINITY && a.l == 0.0f;  // every logit -inf
     const float inv = a.m == INFINITY ? NAN : 1.0f / a.l;
@@ -149,11 +154,11 @@ __device__ inline void write_probs(const float *x, size_t lo, size_t hi, int t, 
             const float4u w = *reinterpret_cast<const float4u *>(x + i);
             float4u p;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = none ? 0.0f : exp_scaled(w[j] - a.m, c) * inv;
+            for (int j = 0; j < 4; ++j) p[j] = none ? 0.0f : c.exp_diff(w[j], a.m) * inv;
             *reinterpret_cast<float4u *>(out + i) = p;
         } else {
             for (size_t j = i; j < hi; ++j)
-                out[j] = none ? 0.0f : exp_scaled(x[j] - a.m, c) * inv;
+                out[j] = none ? 0.0f : c.exp_diff(x[j], a.m) * inv;
         }
     }
 }
@@ -161,13 +166,13 @@ __device__ inline void write_probs(const float *x, size_t lo, size_t hi, int t, 
 constexpr int kMaxParts = 64;
 constexpr size_t kSplitRows = 512;
 static_assert(kSplitRows * kMaxParts * sizeof(MaxSum) <= kSoftmaxWsBytes, "parts' workspace");
-__device__ inline MaxSum join_parts(const MaxSum *p, int parts, float c) {
+__device__ inline MaxSum join_parts(const MaxSum *p, int parts, Temp c) {
     MaxSum a = p[0];
     for (int i = 1; i < parts; ++i) a = join(a, p[i], c);
     return a;
 }
 
-__global__ __launch_bounds__(1024) void k_softmax_row(const float *x, size_t n, size_t xs, float c,
+__global__ __launch_bounds__(1024) void k_softmax_row(const float *x, size_t n, size_t xs, Temp c,
                                                       size_t len, int parts, float *out,
                                                       size_t os) {
     __shared__ MaxSum s_ms[4][4], s_part[kMaxParts];
@@ -185,7 +190,7 @@ __global__ __launch_bounds__(1024) void k_softmax_row(const float *x, size_t n, 
 }
 
 __global__ __launch_bounds__(kPartThreads) void k_softmax_stats(const float *__restrict__ x,
-                                                                size_t n, size_t xs, float c,
+                                                                size_t n, size_t xs, Temp c,
                                                                 size_t len, int parts,
                                                                 MaxSum *__restrict__ ws) {
     __shared__ MaxSum s_ms[4];
@@ -195,7 +200,7 @@ __global__ __launch_bounds__(kPartThreads) void k_softmax_stats(const float *__r
 }
 
 __global__ __launch_bounds__(kPartThreads) void k_softmax_write(const float *x, size_t n,
-                                                                size_t xs, float c, size_t len,
+                                                                size_t xs, Temp c, size_t len,
                                                                 int parts,
                                                                 const MaxSum *__restrict__ ws,
                                                                 float *out, size_t os) {
@@ -412,7 +417,9 @@ __global__ __launch_bounds__(kVerThreads) void k_verify(
 mri_status launch_softmax(const float *x, size_t rows, size_t n, size_t x_stride,
                           float temperature, float *out, size_t out_stride, hipStream_t s) {
     if (!rows) return MRI_OK;
-    const float c = (float)fmin(1.4426950408889634074 / (double)temperature, (double)FLT_MAX);
+    const float half = temperature >= 1.0f ? 0.5f : 1.0f;
+    const Temp c{half, (float)fmin(1.4426950408889634074 / half / (double)temperature,
+                                   (double)FLT_MAX)};
     // Held: 5 x 32000 5.8 us a call against 8.6 in parts (two launches) and 10 in row
     // form, 320 rows 24 against 27, 512 rows 31 against 41.  Twice as many values a
     // thread do not fit its registers beside the addresses: 50000 11 against 8.4.

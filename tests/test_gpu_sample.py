@@ -78,6 +78,20 @@ def test_softmax_special_rows(n):
     assert got[5, 0] == 1 and not got[5, 1:].any()
 
 
+@pytest.mark.parametrize("rows,n", [(3, 777), (2, 8193), (2, 30000), (3, 40000), (514, 32769)])
+@pytest.mark.parametrize("temperature", [1e38, 3e38, 2e37])
+def test_softmax_wide_logits(rows, n, temperature):
+    """Logits that lie further apart than the type's largest value, under a temperature
+    that brings them together."""
+    L, Q, torch = mods()
+    rng = np.random.default_rng([rows, n])
+    x = (rng.uniform(-1, 1, (rows, n)) * 3.4e38).astype(F32)
+    x[:, 0], x[:, n - 1] = 3.4e38, -3.4e38
+    out = torch.empty(rows, n, device="cuda")
+    L.softmax(dev(x), out, temperature=temperature)
+    check_softmax(x, float(F32(temperature)), host(out))
+
+
 @pytest.mark.parametrize("pad,off", [(1, 0), (3, 1), (4, 0)])
 def test_softmax_strided(pad, off):
     L, Q, torch = mods()
