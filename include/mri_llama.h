@@ -193,7 +193,10 @@ mri_status mri_kv4_read(const mri_kv4_cache *cache, size_t layer, size_t n_layer
  * heads, added to what was there for t < pos and stored for the new keys
  * t >= pos (so a rejected draft's weight is gone with it).  The sums are in a
  * fixed order: equal calls give equal bits.
- * Outputs agree with f32 arithmetic on the cached values to f32 rounding. */
+ * Outputs agree with f32 arithmetic on the cached values to f32 rounding, and,
+ * for each key, to 2^-36 of the largest value that the call's rows see in the
+ * same 32 dims of the head; of a query row, what is below 2^-39 of its largest
+ * element is lost. */
 mri_status mri_kv4_attend(mri_kv4_cache *cache, size_t layer, const mri_kv4_rows *rows,
                           const float *q, size_t q_stride, size_t n_heads, float *out,
                           size_t out_stride, float *weights, void *stream);

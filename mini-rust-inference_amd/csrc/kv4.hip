@@ -303,9 +303,10 @@ __global__ __launch_bounds__(256) void k_kv4_read(Kv4Rows a, size_t layer_bytes,
 //    instructions align them as they are: 2.0e-7 of sum |a b| off in the mean
 //    against 1.8e-9.)
 //  * q is split into two f16 halves (22 bits) after a power-of-two scaling of
-//    its row, and so is p * d_v, the probability times the value block's
-//    scale, under a power of two that follows the largest d_v seen (what is
-//    below 2^-33 of that largest product is lost).
+//    its row (what is below 2^-39 of its largest element is lost), and so is
+//    p * d_v, the probability times the value block's scale, under a power of
+//    two of each of the head's blocks, which its largest d_v gives (what is
+//    below 2^-36 of that d_v is lost).
 //  * The key blocks' scales multiply the 32-dim partial products in f32.
 typedef float float2_t __attribute__((ext_vector_type(2)));
 
@@ -507,7 +508,6 @@ struct PageLoad {
     // the operands of a key tile's block and of a dim tile's key half
     __device__ half8_t kop(int t, int b) const { return quants(k[t][b]); }
     __device__ half8_t vop(int e, int h) const { return quants(v[e][h]); }
-    __device__ unsigned vscale(int u) const { return vs[u]; }
 };
 template <int HD>
 constexpr int kScaleWords = 64 * HD / 64;  // of the keys or the values of a page
@@ -557,44 +557,105 @@ __device__ inline float4_t score_tile(const Src &pl, const unsigned *s_ks, int t
     return s;
 }
 
+// The powers of two that a head's value scales are taken in: byte b is 15 + ve of its
+// block b, 2^ve <= the largest d_v < 2^(ve + 1), at least 2^-15.  A lane's dwords of a
+// page's scales are of one block.
+template <int HD>
+__device__ inline int scale_block(int lane) {
+    return HD == 128 ? lane & 3 : lane >> 1 & 1;
+}
+__device__ inline int exp_byte(unsigned e, int b) { return e >> 8 * b & 0xff; }
+// A lane's value scales of a page; those of keys from n_keys on become 0.
+template <int HD>
+struct ValueScales {
+    static constexpr int NB = HD / 32, N = NB / 2;
+    half2_t x[N];
+    __device__ ValueScales(const unsigned *d, int lane, int n_keys) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) x[u] = __builtin_bit_cast(half2_t, d[u]);
+        if (n_keys >= kPageKeys) return;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int w = lane * N + u, key = w / (2 * NB) * 4 + 2 * (w & 1);
+            if (key >= n_keys) x[u].x = (_Float16)0.0f;
+            if (key + 1 >= n_keys) x[u].y = (_Float16)0.0f;
+        }
+    }
+    __device__ half2_t most() const {  // (NaN is no maximum)
+        half2_t m = __builtin_elementwise_abs(x[0]);
+        if constexpr (N == 2) m = __builtin_elementwise_max(m, __builtin_elementwise_abs(x[1]));
+        return m;
+    }
+    // times the two powers of two in up: d 2^(15 - ve), below 2^16, and exact
+    __device__ void scale(half2_t up) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) x[u] = x[u] * half2_t{up.x, up.x} * half2_t{up.y, up.y};
+    }
+    __device__ void put(unsigned *d) const {
+#pragma unroll
+        for (int u = 0; u < N; ++u) d[u] = __builtin_bit_cast(unsigned, x[u]);
+    }
+};
+// The powers of two of the lanes' largest scales, at least those of e.
+template <int HD>
+__device__ inline unsigned exponents(half2_t most, unsigned e, int lane) {
+    float f = fmaxf((float)most.x, (float)most.y);
+    if constexpr (HD == 64) f = fmaxf(f, lane8<0>(f));  // the lanes of the block
+    f = fmaxf(f, ror<4>(f));
+    f = fmaxf(f, ror<8>(f));
+    f = col_max(f);
+    const int own = exp_byte(e, scale_block<HD>(lane));
+    const int byte = max(own, f > 0.0f ? 15 + ilogbf(f) : 0);
+    unsigned r = 0;
+#pragma unroll
+    for (int b = 0; b < HD / 32; ++b)
+        r |= __builtin_amdgcn_readlane(byte, HD == 128 ? b : 2 * b) << 8 * b;
+    return r;
+}
+// What the lane's scales are multiplied by: 2^(30 - byte), in two steps.
+template <int HD>
+__device__ inline half2_t scale_up(unsigned e, int lane) {
+    const int up = 30 - exp_byte(e, scale_block<HD>(lane)), half = up >> 1;
+    return half2_t{__builtin_bit_cast(_Float16, (short)((15 + half) << 10)),
+                   __builtin_bit_cast(_Float16, (short)((15 + up - half) << 10))};
+}
+
 // The running softmax of a wave's 16 columns.  Its reference m follows the scores
 // only when one is 2^kLazy times larger (sixteen columns would otherwise rescale
-// at most pages): p < 2^kLazy and d_v < 2^(ve + 1), so p d_v 2^(kUp - ve) stays
-// below 2^15.
-constexpr int kLazy = 6, kUp = 14 - kLazy;
+// at most pages): p < 2^kLazy, taken in units of 2^kUp, so that p d_v is below 2^15
+// in its block's units.  (2^6: three bits less of small p d_v, the same time to 1 %.)
+constexpr int kLazy = 3, kUp = kLazy + 1;
 template <int HD>
 struct Softmax {
     float m = -INFINITY;  // per column, log2 units: within kLazy of the largest score
-    float l = 0.0f;       // of this lane's keys; l and o in units of 2^(ve - kUp)
-    int ve = -100;        // 2^ve <= the largest d_v seen < 2^(ve + 1)
-    float4_t o[HD / 16];
+    float l = 0.0f;       // of this lane's keys; in units of 2^kUp
+    unsigned e = 0;       // the powers of two that the value scales are taken in
+    float4_t o[HD / 16];  // in units of 2^(kUp + ve - 15 + 9)
     __device__ Softmax() {
 #pragma unroll
         for (int e = 0; e < HD / 16; ++e) o[e] = float4_t{0, 0, 0, 0};
     }
+    __device__ void units(unsigned e_new) {
+#pragma unroll
+        for (int b = 0; b < HD / 32; ++b) {
+            const float f = ldexpf(1.0f, exp_byte(e, b) - exp_byte(e_new, b));
+            o[2 * b] = o[2 * b] * f;
+            o[2 * b + 1] = o[2 * b + 1] * f;
+        }
+        e = e_new;
+    }
+    // what brings o of a dim tile to l's units
+    __device__ float down(int tile) const { return ldexpf(1.0f, 9 - 30 + exp_byte(e, tile / 2)); }
 };
 
 // Adds one page.  WHOLE: every column sees its 64 keys; else keys [0, lim) of it
-// are seen by this lane's column (none if <= 0), the first n_keys by any.
-// s_ks, s_vs: its staged scales.
+// are seen by this lane's column (none if <= 0).  s_ks, s_vs: its staged scales, the
+// values' in the units of st.e.
 template <int HD, bool FEW, bool WHOLE, class Src>
 __device__ inline void attend_page(const Src &pl, const unsigned *s_ks, const unsigned *s_vs,
-                                   int lane, const QTile<HD, FEW> &q, int lim, int n_keys,
-                                   Softmax<HD> &st) {
+                                   int lane, const QTile<HD, FEW> &q, int lim, Softmax<HD> &st) {
     constexpr int NB = HD / 32;
     const int g = lane >> 4;
-    // the page's largest V scale; it seldom grows past the power of two in use
-    float dmax = 0.0f;
-#pragma unroll
-    for (int u = 0; u < NB / 2; ++u) {
-        half2_t d = __builtin_bit_cast(half2_t, pl.vscale(u) & 0x7fff7fffu);
-        if (!WHOLE) {  // what lies past the end counts for nothing
-            const int w = lane * (NB / 2) + u, key = w / (2 * NB) * 4 + 2 * (w & 1);
-            if (key >= n_keys) d.x = (_Float16)0.0f;
-            if (key + 1 >= n_keys) d.y = (_Float16)0.0f;
-        }
-        dmax = fmaxf(dmax, fmaxf((float)d.x, (float)d.y));
-    }
     float s[16];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -607,20 +668,15 @@ __device__ inline void attend_page(const Src &pl, const unsigned *s_ks, const un
 #pragma unroll
     for (int i = 1; i < 16; ++i) pm = fmaxf(pm, s[i]);
     const float m_new = fmaxf(st.m, col_max(pm) * q.inv);
-    if (__any(m_new > st.m + (float)kLazy || dmax >= ldexpf(1.0f, st.ve + 1))) {
-#pragma unroll
-        for (int x = 1; x < kWave; x <<= 1) dmax = fmaxf(dmax, __shfl_xor(dmax, x, kWave));
-        const int ve = max(dmax > 0.0f ? ilogbf(dmax) : -24, st.ve);
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-        const float f = ldexpf(__builtin_amdgcn_exp2f(st.m - m_use), st.ve - ve);
+    if (__any(m_new > st.m + (float)kLazy)) {
+        const float f = __builtin_amdgcn_exp2f(st.m - (m_new == -INFINITY ? 0.0f : m_new));
         st.l = st.l * f;
 #pragma unroll
         for (int e = 0; e < HD / 16; ++e) st.o[e] = st.o[e] * f;
         st.m = m_new;
-        st.ve = ve;
     }
-    // p 2^(kUp - ve)
-    const float m0 = (st.m == -INFINITY ? 0.0f : st.m) - (float)(kUp - st.ve);
+    // p 2^-kUp
+    const float m0 = (st.m == -INFINITY ? 0.0f : st.m) + (float)kUp;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], q.inv, -m0));
@@ -842,8 +898,20 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     const long see = real ? (long)p0 + row + 1 : 0;      // keys this column sees
     const unsigned all = p0 + (qt * NQ) / groups + 1;    // keys every real column sees
     Softmax<HD> st;
+    half2_t up = scale_up<HD>(st.e, lane);
     for (; pg < pg1; pg += kWaves) {
-        const PageLoad<HD> now = next;
+        PageLoad<HD> now = next;
+        ValueScales<HD> vs(now.vs, lane, (int)min(end - pg * kPageKeys, 64u)), up_vs = vs;
+        up_vs.scale(up);
+        const half2_t top = up_vs.most();
+        constexpr int kInf = 0x200;  // past 2^16: a block's power of two has to grow
+        if (__any(__builtin_amdgcn_classh(top.x, kInf) || __builtin_amdgcn_classh(top.y, kInf))) {
+            st.units(exponents<HD>(vs.most(), st.e, lane));
+            up = scale_up<HD>(st.e, lane);
+            up_vs = vs;
+            up_vs.scale(up);
+        }
+        up_vs.put(now.vs);
         __builtin_amdgcn_wave_barrier();  // the last page's scales are read (LDS is in order)
         PageLoad<HD>::stage(now.ks, lane, s_d[wv][0]);
         PageLoad<HD>::stage(now.vs, lane, s_d[wv][1]);
@@ -853,15 +921,12 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
         if (pg + kWaves < pg1) next.load(base + (size_t)(pg + kWaves) * P::kBytes, lane);
         const int lim = (int)min(see - (long)pg * kPageKeys, 64l);
         if ((pg + 1) * kPageKeys <= all)
-            attend_page<HD, FEW, true>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim, 64, st);
+            attend_page<HD, FEW, true>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim, st);
         else
-            attend_page<HD, FEW, false>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim,
-                                        (int)min(end - pg * kPageKeys, 64u), st);
+            attend_page<HD, FEW, false>(now, s_d[wv][0], s_d[wv][1], lane, qtile, lim, st);
     }
-    // o holds 2^-9 of the quants; l and o back to their own units, the
-    // column's sum over its four lane groups, then the waves
-    const float down = ldexpf(1.0f, st.ve - kUp);
-    st.l = col_sum(st.l) * down;
+    // the column's sum over its four lane groups, then the waves
+    st.l = col_sum(st.l);
     if (g == 0 && r < NQ) {
         s_m[wv][r] = st.m;
         s_l[wv][r] = st.l;
@@ -870,7 +935,7 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
     for (int e = 0; e < HD / 16; ++e)
         if (!FEW || e / 2 == r / NQ)
             *reinterpret_cast<float4_t *>(&s_o[wv][r % NQ][16 * e + 4 * g]) =
-                st.o[e] * (down * 0x1p9f);
+                st.o[e] * st.down(e);
     __syncthreads();
     const int cols = min(NQ, n_q - qt * NQ);
     const size_t z0 = ((size_t)b * a.rows) * (a.n_kv * groups);
@@ -881,7 +946,8 @@ __global__ __launch_bounds__(waves_of(HD, SPLIT) * kWave, 2) void k_kv4_attend(
 #pragma unroll
         for (int j = 0; j < 4; ++j) to[j] = o[j] / l;
         if (lse && d == 0)
-            lse[z0 + (size_t)(ci / groups) * (a.n_kv * groups) + oh] = m + __log2f(l);
+            lse[z0 + (size_t)(ci / groups) * (a.n_kv * groups) + oh] =
+                m + __log2f(l * ldexpf(1.0f, kUp));
     };
     const bool alone = !SPLIT || run.n == 1;
     // partial results of run i, column c
@@ -1025,7 +1091,9 @@ struct QRows {
 // 123 us, 57 of them the products (both halves) at a large product's rate; the rest
 // is VALU work (unpacking, softmax, p d_v) that two waves a SIMD hide in part, and
 // each workgroup's first loads (5 us).
-// Eight waves a workgroup: 129.
+// Eight waves a workgroup: 129.  The values' powers of two are found before the pages, from
+// their scales alone: following them page by page, as k_kv4_attend does, holds up the
+// barrier (131).
 constexpr int kPromptWaves = 4;
 template <int HD>
 struct LdsPage {
@@ -1040,7 +1108,6 @@ struct LdsSrc {
     int lane;
     __device__ half8_t kop(int t, int b) const { return p.k[t][b][lane]; }
     __device__ half8_t vop(int e, int h) const { return p.v[e][h][lane]; }
-    __device__ unsigned vscale(int u) const { return p.d[1][lane * (HD / 64) + u]; }
 };
 // What a thread holds of a page on its way to LDS: K tile `wave`, V chunk `wave`
 // (head dim 64: the first two waves), and the first wave K's scales, the second V's.
@@ -1064,12 +1131,18 @@ struct PagePart {
         }
         if (wv < 2) PageLoad<HD>::load_scales(pb + (wv ? P::kVs : P::kKs), lane, d);
     }
-    __device__ void store(LdsPage<HD> &p, int wv, int lane) const {
+    // up: the value scales' units; n_keys: of the page that count
+    __device__ void store(LdsPage<HD> &p, int wv, int lane, half2_t up, unsigned n_keys) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) p.k[wv][b][lane] = quants(k[b]);
         if (wv < NB) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) p.v[2 * wv + (i >> 1)][i & 1][lane] = quants(v[i]);
+        }
+        if (wv == 1) {
+            ValueScales<HD> vs(d, lane, (int)min(n_keys, 64u));
+            vs.scale(up);
+            vs.put(d);
         }
         if (wv < 2) PageLoad<HD>::stage(d, lane, p.d[wv]);
     }
@@ -1084,6 +1157,7 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
     constexpr int NB = P::NB;
     __shared__ LdsPage<HD> s_p[2];
     __shared__ float s_inv[kPromptWaves][16];
+    __shared__ unsigned s_e[kPromptWaves];
     const int lane = threadIdx.x & 63, wv = wave_id(), g = lane >> 4, r = lane & 15;
     unsigned x = blockIdx.x;
     const int head = x % a.n_kv;
@@ -1093,11 +1167,21 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
     const int cnt = (int)rows_of(a, b, &p0);
     const int n_q = cnt * groups;
     if (qg * QW >= n_q) return;
-    const unsigned n_pg = (p0 + (min(qg * QW + QW, n_q) - 1) / groups) / kPageKeys + 1;
+    const unsigned n_keys = p0 + (min(qg * QW + QW, n_q) - 1) / groups + 1;
+    const unsigned n_pg = (n_keys + kPageKeys - 1) / kPageKeys;
     const uint8_t *base =
         a.pages + ((size_t)(a.first_seq + b) * a.n_kv + head) * a.n_pages * P::kBytes;
     PagePart<HD> next;
     next.load(base, wv, lane);
+    // the largest value scales of all the pages, a quarter of them a wave
+    half2_t most = {(_Float16)0.0f, (_Float16)0.0f};
+#pragma unroll 4
+    for (unsigned pg = wv; pg < n_pg; pg += kPromptWaves) {
+        unsigned d[NB / 2];
+        PageLoad<HD>::load_scales(base + (size_t)pg * P::kBytes + P::kVs, lane, d);
+        const ValueScales<HD> vs(d, lane, (int)min(n_keys - pg * kPageKeys, 64u));
+        most = __builtin_elementwise_max(most, vs.most());
+    }
     const int q0 = qg * QW + wv * 16, qi = q0 + r, row = qi / groups;
     const bool real = qi < n_q;
     const int qh = head * groups + qi % groups;
@@ -1123,10 +1207,19 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
     // pages that the wave's last row sees
     const unsigned my_pg =
         q0 < n_q ? (p0 + (min(q0 + 16, n_q) - 1) / groups) / kPageKeys + 1 : 0;
-    const unsigned end = q0 < n_q ? p0 + (min(q0 + 16, n_q) - 1) / groups + 1 : 0;
     Softmax<HD> st;
-    next.store(s_p[0], wv, lane);
+    const unsigned most_e = exponents<HD>(most, 0, lane);
+    if (lane == 0) s_e[wv] = most_e;
     __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        int byte = 0;
+#pragma unroll
+        for (int w = 0; w < kPromptWaves; ++w) byte = max(byte, exp_byte(s_e[w], b));
+        st.e |= uniform((unsigned)byte) << 8 * b;
+    }
+    const half2_t up = scale_up<HD>(st.e, lane);
+    next.store(s_p[0], wv, lane, up, n_keys);
     QTile<HD, false> qtile;
 #pragma unroll
     for (int c = 0; c < NB; ++c) {
@@ -1140,25 +1233,26 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
         if (pg + 1 < n_pg) next.load(base + (size_t)(pg + 1) * P::kBytes, wv, lane);
         const int lim = (int)min(see - (long)pg * kPageKeys, 64l);
         if ((pg + 1) * kPageKeys <= all)
-            attend_page<HD, false, true>(src, src.p.d[0], src.p.d[1], lane, qtile, lim, 64, st);
+            attend_page<HD, false, true>(src, src.p.d[0], src.p.d[1], lane, qtile, lim, st);
         else if (pg < my_pg)
-            attend_page<HD, false, false>(src, src.p.d[0], src.p.d[1], lane, qtile, lim,
-                                          (int)min(end - pg * kPageKeys, 64u), st);
-        if (pg + 1 < n_pg) next.store(s_p[(pg + 1) & 1], wv, lane);
+            attend_page<HD, false, false>(src, src.p.d[0], src.p.d[1], lane, qtile, lim, st);
+        if (pg + 1 < n_pg)
+            next.store(s_p[(pg + 1) & 1], wv, lane, up, n_keys - (pg + 1) * kPageKeys);
         __syncthreads();
     }
     const float l = col_sum(st.l);
     if (!real) return;
-    // l and o share their power of two; o holds 2^-9 of the quants
     float *to = out + row_index(a, b, row) * os + qh * HD + 4 * g;
-    const float inv = 0x1p9f / l;
+    const float inv = 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < HD / 16; ++e)
+    for (int e = 0; e < HD / 16; ++e) {
+        const float f = st.down(e) * inv;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) to[16 * e + i] = st.o[e][i] * inv;
+        for (int i = 0; i < 4; ++i) to[16 * e + i] = st.o[e][i] * f;
+    }
     if (lse && g == 0)
         lse[((size_t)b * a.rows + row) * (a.n_kv * groups) + qh] =
-            st.m + __log2f(l * ldexpf(1.0f, st.ve - kUp));
+            st.m + __log2f(l * ldexpf(1.0f, kUp));
 }
 
 // The keys' attention weights: a wave a page of a KV head goes over all the

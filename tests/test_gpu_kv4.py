@@ -340,6 +340,68 @@ def test_attend_value_scales(first, second):
         assert (np.abs(host(out) - ref) <= (160 * np.maximum(1, top) + 128) * U * mag + tiny).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kv,m,pos", [(1, 1, 600), (2, 5, 600), (8, 520, 0)])
+@pytest.mark.parametrize("small", [1e-3, 2e-5])
+def test_attend_blocks_of_different_scales(hd, kv, m, pos, small):
+    """Value blocks of a head whose sizes lie far apart: each keeps f32 accuracy, the
+    small ones too.  Both halves' smallest steps are those of the block's own scales, and
+    p may reach 2^3 before its reference follows: tiny = keys * 2^-36 * max |v of the
+    block|."""
+    L, Q, torch = mods()
+    rng = np.random.default_rng([hd, kv, m])
+    n, nb = pos + m, hd // 32
+    k, v = (rng.standard_normal((n, kv, hd)).astype(F32) for _ in range(2))
+    for b in range(nb):         # every second block is small
+        if b % 2 == 0:
+            v[:, :, 32 * b:32 * b + 32] *= F32(small)
+    k, v = k.reshape(n, -1), v.reshape(n, -1)
+    c = L.Kv4Cache(1, 1, n, kv, hd)
+    c.append(0, dev(k), dev(v), 0)
+    q = rng.standard_normal((m, kv * 2 * hd)).astype(F32)
+    out = torch.empty(q.shape, device="cuda")
+    c.attend(0, dev(q), out, pos)
+    sk, sv = (R.stored(x).reshape(n, kv, hd) for x in (k, v))
+    ref, _, mag, top = R.attend(q, sk, sv, pos, 2 * kv)
+    most = np.abs(sv).reshape(n, kv, nb, 32).max((0, 3))                  # [kv, blocks]
+    tiny = n * 2.0 ** -36 * np.repeat(np.repeat(most, 2, 0), 32, 1).reshape(-1)
+    tol = (160 * np.maximum(1, top) + 128) * U * mag + tiny
+    err = np.abs(host(out) - ref)
+    assert (err <= tol).all(), (err / tol).max()
+    # and in the mean of a block, where roundings do not all point one way: a score's last
+    # roundings, under u * top, and as many steps as the output's own additions take
+    part = [x.reshape(m, -1, nb, 32).sum((0, 1, 3)) for x in (err, mag)]
+    assert (part[0] <= (np.maximum(1, top.max()) + 8) * U * part[1]).all(), part[0] / part[1] / U
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("m,at", [(1, 3), (1, 640), (300, 3), (300, 555)])
+def test_attend_large_value_that_is_not_attended(hd, m, at):
+    """A value block 1000 times the others' at a key of next to no weight, before and
+    among the rows' own keys: it stays out of the result, and what is lost beside it is
+    2^-36 of it a key at most."""
+    L, Q, torch = mods()
+    rng = np.random.default_rng([hd, m, at])
+    n, kv = 700, 8
+    k, v = (rng.standard_normal((n, kv, hd)).astype(F32) for _ in range(2))
+    q = rng.standard_normal((m, kv, hd)).astype(F32)
+    q[..., 0] = 4
+    k[at, :, 0] = -30 * np.sqrt(hd) / 4      # a score of -30 or so
+    v[at, :, :32] *= 1000
+    c = L.Kv4Cache(1, 1, n, kv, hd)
+    c.append(0, dev(k.reshape(n, -1)), dev(v.reshape(n, -1)), 0)
+    out = torch.empty(m, kv * hd, device="cuda")
+    c.attend(0, dev(q.reshape(m, -1)), out, n - m)
+    sk, sv = (R.stored(x.reshape(n, -1)).reshape(n, kv, hd) for x in (k, v))
+    ref, _, mag, _ = R.attend(q.reshape(m, -1), sk, sv, n - m, kv)
+    # (the keys that have weight: their scores are off by their own sizes)
+    near = np.delete(np.arange(n), at)
+    top = np.abs(q).max() * np.abs(sk[near]).sum(-1).max() / np.sqrt(hd)
+    most = np.abs(sv).reshape(n, kv, hd // 32, 32).max((0, 3))
+    tiny = n * 2.0 ** -36 * np.repeat(most, 32, 1).reshape(-1)
+    assert (np.abs(host(out) - ref) <= (160 * top + 128) * U * mag + tiny).all()
+
+
 def test_attend_nan_and_inf():
     """A query with NaN spoils its own row only; a NaN key every row that sees it; a
     NaN value its block's dims."""
