@@ -191,8 +191,11 @@ mri_status mri_kv4_read(const mri_kv4_cache *cache, size_t layer, size_t n_layer
  * the attention weight that each cached key has got: key t of a KV head gets
  * the sum of its probabilities over the call's rows and the head's query
  * heads, added to what was there for t < pos and stored for the new keys
- * t >= pos (so a rejected draft's weight is gone with it).  The sums are in a
- * fixed order: equal calls give equal bits.
+ * t >= pos: a rejected draft's own entry is gone once its position is written
+ * again.  What the rejected rows gave to the keys before them stays; weights of
+ * accepted rows only take a call of their own after the verification, with
+ * count = accepted + 1 (the call before it without weights).  The sums are in
+ * a fixed order: equal calls give equal bits.
  * Outputs agree with f32 arithmetic on the cached values to f32 rounding, and,
  * for each key, to 2^-36 of the largest value that the call's rows see in the
  * same 32 dims of the head; of a query row, what is below 2^-39 of its largest
@@ -256,7 +259,8 @@ mri_status mri_softmax(const float *x, size_t rows, size_t n, size_t x_stride, f
  * accepted drafts, the drawn token, then MRI_NO_TOKEN.  A draft id >= n is
  * rejected; where no token has a positive probability the drawn token is
  * MRI_NO_TOKEN.  A NaN target probability counts as 0; a token whose draft
- * probability is NaN is neither accepted nor drawn in its place.  InvalidShape
+ * probability is NaN is not accepted and has no part in the difference (where
+ * that has no mass, p_a is drawn from with it).  InvalidShape
  * for n = 0; Unsupported for n = 2^32 - 1 and more, k above 2^20 or n_seqs
  * above 2^21. */
 #define MRI_NO_TOKEN 0xffffffffu

@@ -1,7 +1,8 @@
 // kv4.hpp — the KV cache held in 4-bit blocks: its layout and launchers.
 //
 // A block is 32 consecutive dims of one head's key or value: an f16 scale d
-// and 32 quants q in [-8, 7] (value q * d), the arithmetic of GGUF's Q4_0.
+// and 32 quants q in [-8, 7] (value q * d), a block of GGUF's Q4_0 in what it holds;
+// the quants are nearer (Q4_0 files divide by the scale before its rounding to f16).
 // With mx, mn the block's extremes and a = mx if mx >= -mn else mn,
 // d = f16(a / -8) (saturated at +-65504) and q = clamp(rint(x / d), -8, 7); a
 // block with d = 0 holds zeros, one with a value that is not finite reads as
