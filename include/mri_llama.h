@@ -184,7 +184,8 @@ mri_status mri_kv4_read(const mri_kv4_cache *cache, size_t layer, size_t n_layer
 /* Causal grouped-query attention over the cache: query row i of a sequence at
  * position p = pos + i sees keys 0 .. p (append first).  q and out are
  * [n_seqs * rows] rows of n_heads * head_dim f32, q_stride / out_stride
- * floats apart; head h reads KV head h / (n_heads / n_kv_heads).
+ * floats apart (out may be q, with equal strides, where weights is null); head
+ * h reads KV head h / (n_heads / n_kv_heads).
  * InvalidShape when n_heads % n_kv_heads != 0; Unsupported for more than 2^20
  * heads, or rows * (n_heads / n_kv_heads) above 2^30.
  * weights (nullable): [cache n_seqs][n_kv_heads][max_seq] f32 of this layer,

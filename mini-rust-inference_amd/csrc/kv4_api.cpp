@@ -177,6 +177,10 @@ mri_status mri_kv4_attend(mri_kv4_cache *c, size_t layer, const mri_kv4_rows *ro
     if (!q || !out) return bad_arg("kv4_attend: null pointer");
     if (!float_aligned(q, out, weights))
         return bad_arg("kv4_attend: unaligned rows");
+    if (q == out && q_stride != out_stride)
+        return bad_arg("kv4_attend: in place the strides must be equal");
+    if (weights && q == out)  // the weights are summed from q after out is written
+        return bad_arg("kv4_attend: out is q, and weights are asked for");
     TRY(kv4_on_device(c));
     return launch_kv4_attend(a, c->hd, q, q_stride, n_heads, out, out_stride, weights, c->part,
                              c->cnts, c->lse, static_cast<hipStream_t>(stream));

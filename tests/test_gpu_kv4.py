@@ -308,6 +308,23 @@ def test_attend_prompt_strided_and_nan():
         assert bool((o[:, kv * hd:] == 9).all())
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("b,kv,grp,m,pos", [(2, 2, 2, 1, 900), (3, 2, 4, 5, 300), (8, 8, 2, 130, 0),
+                                            (300, 2, 2, 1, 20)])
+def test_attend_in_place(hd, b, kv, grp, m, pos):
+    """The output over the queries, in every form of the call."""
+    L, Q, torch = mods()
+    rng = np.random.default_rng([hd, b, kv])
+    c = L.Kv4Cache(1, b, pos + m, kv, hd)
+    k, v = (dev(rows(rng, b, pos + m, kv * hd)) for _ in range(2))
+    c.append(0, k, v, 0)
+    q = dev(rng.standard_normal((b, m, kv * grp * hd)).astype(F32))
+    out = torch.empty_like(q)
+    c.attend(0, q, out, pos)
+    c.attend(0, q, q, pos)
+    assert torch.equal(q, out)
+
+
 def test_attend_long():
     check_attend(128, 1, 4, 1, 1, 20000)
 

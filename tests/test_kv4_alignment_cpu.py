@@ -37,6 +37,19 @@ def check_verify(h):
             ("drafts", "q", "p", "u", "counts", "tokens", "accepted"))
 
 
+def check_attend_in_place(h):
+    """The weights read q once more after the output is written: not over q."""
+    c = h.cache()
+    r = h.rows(rows=3)
+    args = dict(c=c, layer=0, rows=r, q=X, qs=256, heads=4, out=X, os=256)
+    h.m.check(h.lib.mri_kv4_attend(*args.values(), None, STREAM))
+    at = h.f.fake_launches()
+    assert h.status(h.lib.mri_kv4_attend(*args.values(), W, STREAM)) == "InvalidArgument"
+    assert h.status(h.lib.mri_kv4_attend(*dict(args, os=257).values(), None, STREAM)) \
+        == "InvalidArgument"
+    assert h.f.fake_launches() == at
+
+
 def check_forward(h):
     L, d, vocab = h.L, 128, 64
     floats = (C.c_float * (vocab * d))()
