@@ -1088,7 +1088,7 @@ struct QRows {
 // a quarter each, and read them from LDS in the operands' order; the next page
 // comes in while this one is computed, into a second buffer (one barrier a page).
 // The workgroups with the most pages start first.  1999 rows of 32 heads of 128:
-// 123 us, 57 of them the products (both halves) at a large product's rate; the rest
+// 124 us, 57 of them the products (both halves) at a large product's rate; the rest
 // is VALU work (unpacking, softmax, p d_v) that two waves a SIMD hide in part, and
 // each workgroup's first loads (5 us).
 // Eight waves a workgroup: 129.  The values' powers of two are found before the pages, from
@@ -1446,7 +1446,9 @@ __device__ inline unsigned weight_key(float w) {
 // largest weight by three passes over its bits (11, 11 and 10, counts in LDS: an
 // exponent alone would put most weights on a few counters), then the positions
 // above it and the first of those equal to it, in order: each wave counts and
-// writes contiguous positions.  Up to 32768 weights are read once, into registers.
+// writes contiguous positions.  Weights of a cache of up to 32768 positions are read
+// once, into registers (128 heads of 32768 keys to 1024: 58 us a call; 103 in a cache of
+// 32832; 256 heads of 2304 keys to 2048: 63, and 57 in a cache of 32832).
 // 256 rows of 2304: 13 us, three passes' latency; 128 of 32768: 23 us.
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / kWave, kSelBins = 2048;
 constexpr int kSelRegs = 32;
@@ -1562,7 +1564,8 @@ __global__ __launch_bounds__(kSelThreads) void k_kv4_select(Kv4Evict e) {
 // its lane group, taken from the sixteen bytes that hold it.  Where a page's keys come
 // from a few pages, as they do while little is dropped, those pages' values are
 // staged in LDS (2304 keys of 256 heads to 2048: 61 us; 107 with a load a nibble
-// from global memory).
+// from global memory).  In place, one page of a head after the other, a call of it takes
+// 97 us for 63, and of 128 heads of 32768 keys to 1024 67 for 58.
 constexpr int kMovePages = 3;
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_move(Kv4Evict e, int per_row) {
@@ -1803,7 +1806,9 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
         // heads over 8 at 4000 keys: head dim 128, 1 sequence 14 us against 30, 16
         // sequences 24 against 32, 24 sequences 31 against 32; head dim 64, 24 21
         // against 23, 48 31 against 34, 72 49 against 46.  (At 500 keys the join
-        // costs a call 0.7 us: the positions may be the device's.)
+        // costs a call 0.7 us: the positions may be the device's.  The rule goes by
+        // the tiles alone: of 32768 keys 16 sequences take 115 us and 17, not split,
+        // 205.)
         const size_t fill = std::min<size_t>(wgs_of(HD) * cus, kKv4PartTiles);
         if (tiles * a.n_seqs * 2 <= fill) {
             const size_t slots = fill / tiles;
@@ -1840,7 +1845,11 @@ mri_status attend_rows(const Kv4Rows &a, const float *q, size_t qs, size_t n_hea
         const size_t n_grp = (n_pg + kWtWaves - 1) / kWtWaves;
         const size_t groups_all = n_grp * a.n_kv * a.n_seqs;
         // parts of the queries: three workgroups a CU, four query tiles a part at least
-        // (1999 rows of 32 heads of 128: 76 us; two a CU 87, four 78, eight 90)
+        // (1999 rows of 32 heads of 128: 76 us; two a CU 87, four 78, eight 90).  With
+        // positions on the device both go by the cache's length: a call of 500 rows of
+        // 32 heads over 8 takes 40 us in a cache of 512 positions, 55 in one of 4096, 165
+        // in one of 32768 (41 in each where the host gives the position); 16 x 5 rows at
+        // 4000 keys 37 in a cache of 4005, 38 in one of 32768, 72 in one of 262144.
         size_t parts = 3 * cus / groups_all;
         parts = std::min(parts, ((n_q + 15) / 16 + kWtWaves - 1) / kWtWaves);
         parts = std::max<size_t>(1, std::min<size_t>(parts, 16));
