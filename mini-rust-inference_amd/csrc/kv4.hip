@@ -1088,7 +1088,7 @@ struct QRows {
 // a quarter each, and read them from LDS in the operands' order; the next page
 // comes in while this one is computed, into a second buffer (one barrier a page).
 // The workgroups with the most pages start first.  1999 rows of 32 heads of 128:
-// 124 us, 57 of them the products (both halves) at a large product's rate; the rest
+// 123 us, 57 of them the products (both halves) at a large product's rate; the rest
 // is VALU work (unpacking, softmax, p d_v) that two waves a SIMD hide in part, and
 // each workgroup's first loads (5 us).
 // Eight waves a workgroup: 129.  The values' powers of two are found before the pages, from
@@ -1110,7 +1110,9 @@ struct LdsSrc {
     __device__ half8_t vop(int e, int h) const { return p.v[e][h][lane]; }
 };
 // What a thread holds of a page on its way to LDS: K tile `wave`, V chunk `wave`
-// (head dim 64: the first two waves), and the first wave K's scales, the second V's.
+// (head dim 64: the first two waves), and K's scales in the first wave, V's in the second.
+// (The others hold them too: with a branch around them, the second wave's products come
+// last before each barrier: 512 rows behind 32000 keys 1030 us for 1003.)
 template <int HD>
 struct PagePart {
     using P = Page<HD>;
@@ -1129,20 +1131,18 @@ struct PagePart {
             const uint4 x = *reinterpret_cast<const uint4 *>(pb + P::kV + wv * 1024 + lane * 16);
             v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
         }
-        if (wv < 2) PageLoad<HD>::load_scales(pb + (wv ? P::kVs : P::kKs), lane, d);
+        PageLoad<HD>::load_scales(pb + (wv & 1 ? P::kVs : P::kKs), lane, d);
     }
-    // up: the value scales' units; n_keys: of the page that count
-    __device__ void store(LdsPage<HD> &p, int wv, int lane, half2_t up, unsigned n_keys) {
+    // up: what the wave's scales are multiplied by (those past the end may become infinite)
+    __device__ void store(LdsPage<HD> &p, int wv, int lane, half2_t up) {
+        ValueScales<HD> ds(d, lane, kPageKeys);
+        ds.scale(up);
+        ds.put(d);
 #pragma unroll
         for (int b = 0; b < NB; ++b) p.k[wv][b][lane] = quants(k[b]);
         if (wv < NB) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) p.v[2 * wv + (i >> 1)][i & 1][lane] = quants(v[i]);
-        }
-        if (wv == 1) {
-            ValueScales<HD> vs(d, lane, (int)min(n_keys, 64u));
-            vs.scale(up);
-            vs.put(d);
         }
         if (wv < 2) PageLoad<HD>::stage(d, lane, p.d[wv]);
     }
@@ -1218,8 +1218,9 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
         for (int w = 0; w < kPromptWaves; ++w) byte = max(byte, exp_byte(s_e[w], b));
         st.e |= uniform((unsigned)byte) << 8 * b;
     }
-    const half2_t up = scale_up<HD>(st.e, lane);
-    next.store(s_p[0], wv, lane, up, n_keys);
+    const half2_t one = {(_Float16)1.0f, (_Float16)1.0f};
+    const half2_t up = wv == 1 ? scale_up<HD>(st.e, lane) : one;
+    next.store(s_p[0], wv, lane, up);
     QTile<HD, false> qtile;
 #pragma unroll
     for (int c = 0; c < NB; ++c) {
@@ -1236,8 +1237,7 @@ __global__ __launch_bounds__(kPromptWaves *kWave, 2) void k_kv4_prompt(
             attend_page<HD, false, true>(src, src.p.d[0], src.p.d[1], lane, qtile, lim, st);
         else if (pg < my_pg)
             attend_page<HD, false, false>(src, src.p.d[0], src.p.d[1], lane, qtile, lim, st);
-        if (pg + 1 < n_pg)
-            next.store(s_p[(pg + 1) & 1], wv, lane, up, n_keys - (pg + 1) * kPageKeys);
+        if (pg + 1 < n_pg) next.store(s_p[(pg + 1) & 1], wv, lane, up);
         __syncthreads();
     }
     const float l = col_sum(st.l);
